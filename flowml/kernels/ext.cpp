@@ -4,11 +4,12 @@
 
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
 
 #include <tuple>
 #include <vector>
 
-// ---- launcher decls (defined in tree_kernels.hip / mlp_kernels.hip) -------
+// ---- launcher decls (defined in the .hip TUs) -------
 
 extern "C" {
 void launch_bin_codes(const float*, const float*, uint8_t*, long long, int,
@@ -52,6 +53,14 @@ void launch_wgrad_bias_bf16(const void*, const void*, float*, long long, int,
 void wgrad_bias_plan(long long, int*, long long*, int*);
 void launch_wgrad_f32_splitk(const float*, const float*, float*, long long,
                              int, int, int, long long, void*);
+void launch_layer_norm(int, const void*, long long, const float*, const float*,
+                       void*, float*, float*, long long, int, float, int,
+                       void*);
+int layer_norm_grad_slabs(int, long long, int);
+void launch_layer_norm_grad(int, const void*, long long, const void*,
+                            long long, const void*, long long, const float*,
+                            const float*, const float*, void*, float*, float*,
+                            long long, int, int, void*);
 }
 
 static void* cur_stream() {
@@ -399,6 +408,97 @@ std::tuple<torch::Tensor, torch::Tensor> wgrad_f32(torch::Tensor X,
   return {m.slice(1, 0, F).contiguous(), m.select(1, F).contiguous()};
 }
 
+// ---- layer norm ------------------------------------------------------------
+
+static int norm_type(const torch::Tensor& t) {
+  switch (t.scalar_type()) {
+    case torch::kFloat32: return 0;
+    case torch::kBFloat16: return 1;
+    case torch::kFloat16: return 2;
+    default: TORCH_CHECK(false, "layer norm takes f32, bf16 or f16");
+  }
+}
+
+// rows x columns with neighbouring columns side by side, whatever the rows'
+// distance
+static void check_rows(const torch::Tensor& t, const torch::Tensor& like,
+                       const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name,
+              " must be on X's device");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name,
+              " must have X's type");
+  TORCH_CHECK(t.dim() == 2 && t.sizes() == like.sizes(), name,
+              " must have X's shape");
+  TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, name,
+              " must have unit column stride");
+}
+
+static const float* opt_columns(const c10::optional<torch::Tensor>& t,
+                                const torch::Tensor& like, const char* name) {
+  if (!t.has_value()) return nullptr;
+  TORCH_CHECK(t->device() == like.device() &&
+                  t->scalar_type() == torch::kFloat32 && t->is_contiguous() &&
+                  t->numel() == like.size(1),
+              name, " must be one contiguous f32 per column");
+  return t->data_ptr<float>();
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm(
+    torch::Tensor X, c10::optional<torch::Tensor> weight,
+    c10::optional<torch::Tensor> bias, double eps, int64_t act) {
+  check_rows(X, X, "X");
+  const int type = norm_type(X);
+  TORCH_CHECK(X.size(1) >= 1 && X.size(1) <= (1 << 28), "columns out of range");
+  const at::cuda::OptionalCUDAGuard guard(X.device());
+  const float* g = opt_columns(weight, X, "weight");
+  const float* b = opt_columns(bias, X, "bias");
+  const long long N = X.size(0);
+  const int D = (int)X.size(1);
+  auto Y = torch::empty({N, D}, X.options());
+  auto mean = torch::empty({N}, X.options().dtype(torch::kFloat32));
+  auto rstd = torch::empty_like(mean);
+  if (N)
+    launch_layer_norm(type, X.data_ptr(), X.stride(0), g, b, Y.data_ptr(),
+                      mean.data_ptr<float>(), rstd.data_ptr<float>(), N, D,
+                      (float)eps, (int)act, cur_stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {Y, mean, rstd};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_grad(
+    torch::Tensor dY, torch::Tensor X, torch::Tensor mean, torch::Tensor rstd,
+    c10::optional<torch::Tensor> weight, c10::optional<torch::Tensor> Y,
+    int64_t act) {
+  check_rows(X, X, "X");
+  check_rows(dY, X, "dY");
+  if (act) {
+    TORCH_CHECK(Y.has_value(), "an activation's gradient needs Y");
+    check_rows(*Y, X, "Y");
+  }
+  const int type = norm_type(X);
+  TORCH_CHECK(X.size(1) >= 1 && X.size(1) <= (1 << 28), "columns out of range");
+  const long long N = X.size(0);
+  const int D = (int)X.size(1);
+  for (const auto& t : {mean, rstd})
+    TORCH_CHECK(t.device() == X.device() && t.numel() == N &&
+                    t.scalar_type() == torch::kFloat32 && t.is_contiguous(),
+                "mean and rstd must be one contiguous f32 per row");
+  const at::cuda::OptionalCUDAGuard guard(X.device());
+  const float* g = opt_columns(weight, X, "weight");
+  const auto f32 = X.options().dtype(torch::kFloat32);
+  auto dX = torch::empty({N, D}, X.options());
+  auto out = torch::empty({2, D}, f32);
+  auto part = torch::empty({layer_norm_grad_slabs(type, N, D), 2, D}, f32);
+  launch_layer_norm_grad(type, dY.data_ptr(), dY.stride(0), X.data_ptr(),
+                         X.stride(0), act ? Y->data_ptr() : nullptr,
+                         act ? Y->stride(0) : 0, mean.data_ptr<float>(),
+                         rstd.data_ptr<float>(), g, dX.data_ptr(),
+                         part.data_ptr<float>(), out.data_ptr<float>(), N, D,
+                         (int)act, cur_stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dX, out[0], out[1]};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bin_codes", &bin_codes, "K4a quantile binning");
   m.def("tree_hist_cls", &tree_hist_cls, "K2 class histograms (all trees)");
@@ -412,5 +512,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("wgrad_f32", &wgrad_f32, "split-K f32 wgrad + bias grad (LR)");
   m.def("softmax_xent_grad", &softmax_xent_grad, "K6 softmax/xent grad");
   m.def("gemm_bias_act", &gemm_bias_act, "K5 fused MFMA GEMM+bias+act");
+  m.def("layer_norm", &layer_norm, "layer norm + activation, row statistics");
+  m.def("layer_norm_grad", &layer_norm_grad, "dX, dweight, dbias of layer norm");
   m.def("wgrad_bias", &wgrad_bias, "K7 split-N wgrad + fused bias grad");
 }

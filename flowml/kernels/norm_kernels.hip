@@ -1,0 +1,629 @@
+// CDNA4 (gfx950) layer norm with a fused activation, forward and backward.
+//
+//   mu = sum_j x_j / D          var = sum_j (x_j - mu)^2 / D
+//   rstd = 1 / sqrt(var + eps)  xh_j = (x_j - mu) rstd
+//   y_j = act(xh_j g_j + b_j)
+//
+//   dz = dy act'(y)             p = dz g
+//   dx = rstd (p - mean(p) - xh mean(p xh))
+//   dg = sum_rows dz xh         db = sum_rows dz
+//
+// Both passes are bound by HBM: each input is read once and each output is
+// written once.  A row lives in the registers of the lanes that share it, so
+// the variance is the centred sum of a second look at registers, not of a
+// second read (no E[x^2] - E[x]^2 cancellation).  The number of lanes on a
+// row is the smallest power of two that holds it in 16-byte pieces: a row of
+// 128 bf16 takes 16 lanes, four rows share a wave, and their sums are DPP
+// moves without LDS.  All sums and statistics are fp32; values are rounded
+// to the tensor's type once, at the store.
+//
+// The activation's derivative is taken from the stored output y (relu: y > 0,
+// sigmoid: y (1 - y)), as the dgrad kernel of the GEMM stack does: a sign
+// recomputed from x could differ from the one the forward pass acted on.
+//
+// dg and db are summed without atomics: a lane owns its columns over all rows
+// of its block, the block's row groups are added in LDS in a fixed order, and
+// a second kernel adds the blocks' slabs in a fixed order, so that two runs
+// agree bit for bit.
+
+#include <hip/hip_runtime.h>
+#include <hip/hip_bf16.h>
+#include <stdint.h>
+
+namespace {
+
+enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
+
+// 16-byte pieces at element alignment: the hardware takes unaligned global
+// accesses, so odd row lengths and odd strides use the same wide loads.
+template <typename T>
+struct Piece {
+  static constexpr int VEC = 16 / sizeof(T);
+  typedef T raw __attribute__((ext_vector_type(16 / sizeof(T))));
+  typedef raw vec __attribute__((aligned(sizeof(T))));
+};
+
+template <typename T>
+__device__ __forceinline__ void load_piece(const T* p, int left, float* v) {
+  constexpr int VEC = Piece<T>::VEC;
+  if (left >= VEC) {
+    const typename Piece<T>::raw r = *reinterpret_cast<const typename Piece<T>::vec*>(p);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = (float)r[k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = k < left ? (float)p[k] : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, int left, const float* v) {
+  constexpr int VEC = Piece<T>::VEC;
+  if (left >= VEC) {
+    typename Piece<T>::raw r;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) r[k] = (T)v[k];
+    *reinterpret_cast<typename Piece<T>::vec*>(p) = r;
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (k < left) p[k] = (T)v[k];
+  }
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+
+// Sum over groups of LANES <= 64 neighbouring lanes; every lane gets it, with
+// the same bits.  All lanes of the wave take part.
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+  if (LANES >= 2) v += dpp<0xB1>(v);   // quad_perm 1,0,3,2
+  if (LANES >= 4) v += dpp<0x4E>(v);   // quad_perm 2,3,0,1
+  if (LANES >= 8) v += dpp<0x141>(v);  // mirror within 8
+  if (LANES >= 16) v += dpp<0x140>(v); // mirror within 16
+  if (LANES >= 32) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (LANES >= 64) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+// Sum over the lanes that share a row: part of a wave, or the whole block.
+// `lds`: LANES / 64 floats that no wave still reads (callers alternate).
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float* lds) {
+  if constexpr (LANES <= 64) {
+    return lanes_sum<LANES>(v);
+  } else {
+    v = lanes_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < LANES / 64; ++k) s += lds[k];
+    return s;
+  }
+}
+
+// Two such sums behind one barrier; `lds`: 2 * LANES / 64 floats.
+template <int LANES>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float* lds) {
+  a = lanes_sum<(LANES < 64 ? LANES : 64)>(a);
+  b = lanes_sum<(LANES < 64 ? LANES : 64)>(b);
+  if constexpr (LANES > 64) {
+    constexpr int W = LANES / 64;
+    if ((threadIdx.x & 63) == 0) {
+      lds[threadIdx.x >> 6] = a;
+      lds[W + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+      a += lds[k];
+      b += lds[W + k];
+    }
+  }
+}
+
+__device__ __forceinline__ float activate(float z, int act) {
+  if (act == 1) return z < 0.f ? 0.f : z;  // keeps NaN
+  if (act == 2) return 1.f / (1.f + expf(-z));
+  return z;
+}
+
+__device__ __forceinline__ float activate_grad(float dy, float y, int act) {
+  if (act == 1) return y > 0.f ? dy : 0.f;
+  if (act == 2) return dy * (y * (1.f - y));
+  return dy;
+}
+
+// ---------------------------------------------------------------------------
+// forward: LANES lanes x NV pieces hold a row
+// ---------------------------------------------------------------------------
+
+template <typename T, int LANES, int NV>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm(
+    const T* __restrict__ X, long long ldx, const float* __restrict__ gamma,
+    const float* __restrict__ beta, T* __restrict__ Y, float* __restrict__ mean,
+    float* __restrict__ rstd, long long N, int D, float eps, int act) {
+  constexpr int VEC = Piece<T>::VEC;
+  constexpr int BLOCK = LANES > 256 ? LANES : 256;
+  constexpr int GROUPS = BLOCK / LANES;
+  __shared__ float s_red[2][LANES > 64 ? LANES / 64 : 1];
+  const int lane = threadIdx.x % LANES;
+  const int group = threadIdx.x / LANES;
+  const float d = (float)D;
+
+  float g[NV][VEC], b[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + lane) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      g[i][k] = (gamma && c + k < D) ? gamma[c + k] : 1.f;
+      b[i][k] = (beta && c + k < D) ? beta[c + k] : 0.f;
+    }
+  }
+
+  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < N;
+       row0 += (long long)gridDim.x * GROUPS) {
+    // lanes without a row of their own repeat the last one: the sums below
+    // need every lane of the wave
+    const bool live = row0 + group < N;
+    const long long row = live ? row0 + group : N - 1;
+    const T* x = X + row * ldx;
+    float v[NV][VEC];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * VEC;
+      load_piece<T>(x + c, D - c, v[i]);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s += v[i][k];
+    }
+    const float mu = row_sum<LANES>(s, s_red[0]) / d;
+    float q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * VEC;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        v[i][k] -= mu;
+        q += c + k < D ? v[i][k] * v[i][k] : 0.f;
+      }
+    }
+    const float r = 1.f / sqrtf(row_sum<LANES>(q, s_red[1]) / d + eps);
+    if (live) {
+      T* y = Y + row * D;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LANES + lane) * VEC;
+        if (c < D) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            v[i][k] = activate(v[i][k] * r * g[i][k] + b[i][k], act);
+          store_piece<T>(y + c, D - c, v[i]);
+        }
+      }
+      if (lane == 0) {
+        mean[row] = mu;
+        rstd[row] = r;
+      }
+    }
+  }
+}
+
+// Rows longer than a block's registers: three looks at the row.
+template <typename T>
+__global__ __launch_bounds__(1024) void flowml_layer_norm_long(
+    const T* __restrict__ X, long long ldx, const float* __restrict__ gamma,
+    const float* __restrict__ beta, T* __restrict__ Y, float* __restrict__ mean,
+    float* __restrict__ rstd, long long N, int D, float eps, int act) {
+  constexpr int VEC = Piece<T>::VEC;
+  __shared__ float s_red[2][16];
+  const float d = (float)D;
+  for (long long row = blockIdx.x; row < N; row += gridDim.x) {
+    const T* x = X + row * ldx;
+    float v[VEC];
+    float s = 0.f;
+    for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
+      load_piece<T>(x + c, D - c, v);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) s += v[k];
+    }
+    const float mu = row_sum<1024>(s, s_red[0]) / d;
+    float q = 0.f;
+    for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
+      load_piece<T>(x + c, D - c, v);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) q += c + k < D ? (v[k] - mu) * (v[k] - mu) : 0.f;
+    }
+    const float r = 1.f / sqrtf(row_sum<1024>(q, s_red[1]) / d + eps);
+    T* y = Y + row * D;
+    for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
+      load_piece<T>(x + c, D - c, v);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const bool in = c + k < D;
+        const float g = (gamma && in) ? gamma[c + k] : 1.f;
+        const float b = (beta && in) ? beta[c + k] : 0.f;
+        v[k] = activate((v[k] - mu) * r * g + b, act);
+      }
+      store_piece<T>(y + c, D - c, v);
+    }
+    if (threadIdx.x == 0) {
+      mean[row] = mu;
+      rstd[row] = r;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// backward: dx, and one slab (dg, db) per block in part[block][2][D]
+// ---------------------------------------------------------------------------
+
+template <typename T, int LANES, int NV, bool ACT>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm_grad(
+    const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
+    const T* __restrict__ Y, long long ldy, const float* __restrict__ mean,
+    const float* __restrict__ rstd, const float* __restrict__ gamma,
+    T* __restrict__ dX, float* __restrict__ part, long long N, int D, int act) {
+  constexpr int VEC = Piece<T>::VEC;
+  constexpr int BLOCK = LANES > 256 ? LANES : 256;
+  constexpr int GROUPS = BLOCK / LANES;
+  constexpr int WIDTH = LANES * NV * VEC;
+  __shared__ float s_red[2][LANES > 64 ? LANES / 32 : 1];
+  __shared__ float s_cols[GROUPS > 1 ? BLOCK * NV * VEC : 1];
+  const int lane = threadIdx.x % LANES;
+  const int group = threadIdx.x / LANES;
+  const float d = (float)D;
+
+  float g[NV][VEC], dg[NV][VEC], db[NV][VEC];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * LANES + lane) * VEC;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      g[i][k] = (gamma && c + k < D) ? gamma[c + k] : 1.f;
+      dg[i][k] = db[i][k] = 0.f;
+    }
+  }
+
+  int turn = 0;  // the block-wide sums of two neighbouring rows use other words
+  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < N;
+       row0 += (long long)gridDim.x * GROUPS, turn ^= 1) {
+    const bool live = row0 + group < N;
+    const long long row = live ? row0 + group : N - 1;
+    const float mu = mean[row], r = rstd[row];
+    float xh[NV][VEC], dz[NV][VEC];
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * VEC;
+      load_piece<T>(X + row * ldx + c, D - c, xh[i]);
+      load_piece<T>(dY + row * lddy + c, D - c, dz[i]);
+      if constexpr (ACT) {
+        float y[VEC];
+        load_piece<T>(Y + row * ldy + c, D - c, y);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dz[i][k] = activate_grad(dz[i][k], y[k], act);
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        xh[i][k] = (xh[i][k] - mu) * r;
+        // past the row's end dz is 0, and with it p and both sums
+        const float p = dz[i][k] * g[i][k];
+        s += p;
+        q += c + k < D ? p * xh[i][k] : 0.f;
+        if (live) {
+          dg[i][k] += dz[i][k] * xh[i][k];
+          db[i][k] += dz[i][k];
+        }
+      }
+    }
+    row_sum2<LANES>(s, q, s_red[turn]);
+    s /= d;
+    q /= d;
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (i * LANES + lane) * VEC;
+        if (c < D) {
+          float o[VEC];
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            o[k] = r * (dz[i][k] * g[i][k] - s - xh[i][k] * q);
+          store_piece<T>(dX + row * D + c, D - c, o);
+        }
+      }
+    }
+  }
+
+  float* slab = part + (long long)blockIdx.x * 2 * D;
+  if constexpr (GROUPS == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * VEC;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (c + k < D) {
+          slab[c + k] = dg[i][k];
+          slab[D + c + k] = db[i][k];
+        }
+    }
+  } else {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          s_cols[group * WIDTH + (i * LANES + lane) * VEC + k] = half ? db[i][k] : dg[i][k];
+      __syncthreads();
+      for (int c = threadIdx.x; c < D; c += BLOCK) {
+        float t = 0.f;
+        for (int o = 0; o < GROUPS; ++o) t += s_cols[o * WIDTH + c];
+        slab[half * D + c] = t;
+      }
+    }
+  }
+}
+
+// Long rows: dx alone, two looks at the row ...
+template <typename T>
+__global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
+    const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
+    const T* __restrict__ Y, long long ldy, const float* __restrict__ mean,
+    const float* __restrict__ rstd, const float* __restrict__ gamma,
+    T* __restrict__ dX, long long N, int D, int act) {
+  constexpr int VEC = Piece<T>::VEC;
+  __shared__ float s_red[2][32];
+  const float d = (float)D;
+  int turn = 0;
+  for (long long row = blockIdx.x; row < N; row += gridDim.x, turn ^= 1) {
+    const float mu = mean[row], r = rstd[row];
+    float s = 0.f, q = 0.f;
+    for (int look = 0; look < 2; ++look) {
+      for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
+        float x[VEC], dz[VEC], y[VEC];
+        load_piece<T>(X + row * ldx + c, D - c, x);
+        load_piece<T>(dY + row * lddy + c, D - c, dz);
+        if (act) load_piece<T>(Y + row * ldy + c, D - c, y);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+          const bool in = c + k < D;
+          const float p = (act ? activate_grad(dz[k], y[k], act) : dz[k]) *
+                          ((gamma && in) ? gamma[c + k] : 1.f);
+          const float xh = (x[k] - mu) * r;
+          if (look == 0) {
+            s += p;
+            q += in ? p * xh : 0.f;
+          } else {
+            x[k] = r * (p - s - xh * q);
+          }
+        }
+        if (look) store_piece<T>(dX + row * D + c, D - c, x);
+      }
+      if (look == 0) {
+        row_sum2<1024>(s, q, s_red[turn]);
+        s /= d;
+        q /= d;
+      }
+    }
+  }
+}
+
+// ... and the columns: a block sums 256 columns over a chunk of the rows
+template <typename T>
+__global__ __launch_bounds__(256) void flowml_layer_norm_grad_cols(
+    const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
+    const T* __restrict__ Y, long long ldy, const float* __restrict__ mean,
+    const float* __restrict__ rstd, float* __restrict__ part, long long N, int D,
+    long long chunk, int act) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= D) return;
+  const long long lo = blockIdx.y * chunk;
+  const long long hi = lo + chunk < N ? lo + chunk : N;
+  float dg = 0.f, db = 0.f;
+  for (long long row = lo; row < hi; ++row) {
+    const float x = (float)X[row * ldx + c];
+    float dz = (float)dY[row * lddy + c];
+    if (act) dz = activate_grad(dz, (float)Y[row * ldy + c], act);
+    dg += dz * ((x - mean[row]) * rstd[row]);
+    db += dz;
+  }
+  float* slab = part + (long long)blockIdx.y * 2 * D;
+  slab[c] = dg;
+  slab[D + c] = db;
+}
+
+// out[c] = sum of part[s][c] over the slabs, in an order that G alone sets:
+// 32 columns x 32 runs of slabs per block.
+__global__ __launch_bounds__(1024) void flowml_layer_norm_slabs(
+    const float* __restrict__ part, float* __restrict__ out, int G, int W) {
+  __shared__ float s[32][33];
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31);
+  const int run = threadIdx.x >> 5;
+  float t = 0.f;
+  if (c < W)
+    for (int k = run; k < G; k += 32) t += part[(long long)k * W + c];
+  s[run][threadIdx.x & 31] = t;
+  __syncthreads();
+  if (run == 0 && c < W) {
+    float u = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) u += s[k][threadIdx.x];
+    out[c] = u;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// launch plans
+// ---------------------------------------------------------------------------
+
+constexpr int kCUs = 256;
+
+// lanes and pieces for a row of D values of VEC to the piece: one piece per
+// lane up to a wave, then more pieces, then more waves.
+struct Shape {
+  int lanes, nv;
+};
+
+Shape shape_for(int D, int vec) {
+  const int pieces = (D + vec - 1) / vec;
+  for (int l = 1; l <= 64; l *= 2)
+    if (pieces <= l) return {l, 1};
+  if (pieces <= 128) return {64, 2};
+  if (pieces <= 256) return {256, 1};
+  if (pieces <= 512) return {256, 2};
+  if (pieces <= 1024) return {1024, 1};
+  if (pieces <= 2048) return {1024, 2};
+  if (vec == 4 && pieces <= 4096) return {1024, 4};
+  return {0, 0};
+}
+
+int rows_per_block(Shape s) { return s.lanes > 256 ? 1 : 256 / s.lanes; }
+
+template <typename T>
+void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, float* mean,
+             float* rstd, long long N, int D, float eps, int act, hipStream_t st) {
+  const Shape s = shape_for(D, Piece<T>::VEC);
+  if (!s.lanes) {
+    const int grid = (int)(N < 2 * kCUs ? N : 2 * kCUs);
+    hipLaunchKernelGGL((flowml_layer_norm_long<T>), dim3(grid), dim3(1024), 0, st, X, ldx, g, b, Y,
+                       mean, rstd, N, D, eps, act);
+    return;
+  }
+  const int rpb = rows_per_block(s);
+  const long long want = (N + rpb - 1) / rpb;
+  const long long most = (long long)kCUs * 8;
+  const int grid = (int)(want < most ? want : most);
+#define LN_CASE(L, V)                                                              \
+  if (s.lanes == L && s.nv == V)                                                   \
+    hipLaunchKernelGGL((flowml_layer_norm<T, L, V>), dim3(grid),                   \
+                       dim3(L > 256 ? L : 256), 0, st, X, ldx, g, b, Y, mean, rstd, N, D, eps, act)
+  LN_CASE(1, 1);
+  LN_CASE(2, 1);
+  LN_CASE(4, 1);
+  LN_CASE(8, 1);
+  LN_CASE(16, 1);
+  LN_CASE(32, 1);
+  LN_CASE(64, 1);
+  LN_CASE(64, 2);
+  LN_CASE(256, 1);
+  LN_CASE(256, 2);
+  LN_CASE(1024, 1);
+  LN_CASE(1024, 2);
+  if constexpr (Piece<T>::VEC == 4) LN_CASE(1024, 4);
+#undef LN_CASE
+}
+
+// slabs (and blocks) of the backward pass
+int grad_slabs(long long N, int D, int vec) {
+  const Shape s = shape_for(D, vec);
+  long long want, most;
+  if (!s.lanes) {
+    // columns kernel: 256 columns to a block, chunks of rows to fill the chip
+    want = (N + 15) / 16;
+    most = (4 * kCUs * 256LL + D - 1) / D;
+    if (most < 1) most = 1;
+  } else {
+    const int rpb = rows_per_block(s);
+    want = (N + rpb - 1) / rpb;
+    most = s.lanes > 256 ? kCUs : 4 * kCUs;
+  }
+  return (int)(want < most ? want : most);
+}
+
+template <typename T>
+void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y, long long ldy,
+              const float* mean, const float* rstd, const float* g, T* dX, float* part,
+              float* out, long long N, int D, int act, hipStream_t st) {
+  const Shape s = shape_for(D, Piece<T>::VEC);
+  const int slabs = N ? grad_slabs(N, D, Piece<T>::VEC) : 0;
+  if (slabs && !s.lanes) {
+    const int grid = (int)(N < 2 * kCUs ? N : 2 * kCUs);
+    hipLaunchKernelGGL((flowml_layer_norm_grad_long<T>), dim3(grid), dim3(1024), 0, st, dY, lddy, X,
+                       ldx, Y, ldy, mean, rstd, g, dX, N, D, act);
+    const long long chunk = (N + slabs - 1) / slabs;
+    hipLaunchKernelGGL((flowml_layer_norm_grad_cols<T>), dim3((D + 255) / 256, slabs),
+                       dim3(256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, part, N, D, chunk, act);
+  } else if (slabs) {
+#define LN_CASE1(L, V, A)                                                               \
+  hipLaunchKernelGGL((flowml_layer_norm_grad<T, L, V, A>), dim3(slabs),                 \
+                     dim3(L > 256 ? L : 256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act)
+#define LN_CASE(L, V)                \
+  if (s.lanes == L && s.nv == V) {   \
+    if (act)                         \
+      LN_CASE1(L, V, true);          \
+    else                             \
+      LN_CASE1(L, V, false);         \
+  }
+    LN_CASE(1, 1);
+    LN_CASE(2, 1);
+    LN_CASE(4, 1);
+    LN_CASE(8, 1);
+    LN_CASE(16, 1);
+    LN_CASE(32, 1);
+    LN_CASE(64, 1);
+    LN_CASE(64, 2);
+    LN_CASE(256, 1);
+    LN_CASE(256, 2);
+    LN_CASE(1024, 1);
+    LN_CASE(1024, 2);
+    if constexpr (Piece<T>::VEC == 4) LN_CASE(1024, 4);
+#undef LN_CASE
+#undef LN_CASE1
+  }
+  hipLaunchKernelGGL(flowml_layer_norm_slabs, dim3((2 * D + 31) / 32), dim3(1024), 0, st,
+                     part, out, slabs, 2 * D);
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// host launchers (type: 0 f32, 1 bf16, 2 f16; strides in values)
+// ---------------------------------------------------------------------------
+
+extern "C" void launch_layer_norm(int type, const void* X, long long ldx, const float* g,
+                                  const float* b, void* Y, float* mean, float* rstd, long long N,
+                                  int D, float eps, int act, void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  if (type == T_F32)
+    forward((const float*)X, ldx, g, b, (float*)Y, mean, rstd, N, D, eps, act, st);
+  else if (type == T_BF16)
+    forward((const __bf16*)X, ldx, g, b, (__bf16*)Y, mean, rstd, N, D, eps, act, st);
+  else
+    forward((const _Float16*)X, ldx, g, b, (_Float16*)Y, mean, rstd, N, D, eps, act, st);
+}
+
+// slabs of 2 * D floats that the backward pass wants as a workspace
+extern "C" int layer_norm_grad_slabs(int type, long long N, int D) {
+  return N ? grad_slabs(N, D, type == T_F32 ? 4 : 8) : 0;
+}
+
+extern "C" void launch_layer_norm_grad(int type, const void* dY, long long lddy, const void* X,
+                                       long long ldx, const void* Y, long long ldy,
+                                       const float* mean, const float* rstd, const float* g,
+                                       void* dX, float* part, float* out, long long N, int D,
+                                       int act, void* stream) {
+  hipStream_t st = (hipStream_t)stream;
+  if (type == T_F32)
+    backward((const float*)dY, lddy, (const float*)X, ldx, (const float*)Y, ldy, mean, rstd, g,
+             (float*)dX, part, out, N, D, act, st);
+  else if (type == T_BF16)
+    backward((const __bf16*)dY, lddy, (const __bf16*)X, ldx, (const __bf16*)Y, ldy, mean, rstd, g,
+             (__bf16*)dX, part, out, N, D, act, st);
+  else
+    backward((const _Float16*)dY, lddy, (const _Float16*)X, ldx, (const _Float16*)Y, ldy, mean,
+             rstd, g, (_Float16*)dX, part, out, N, D, act, st);
+}

@@ -648,6 +648,119 @@ def mlp_grad(
     return loss, gWs, gBs
 
 
+# ---------------------------------------------------------------------------
+# Layer norm with a fused activation
+# ---------------------------------------------------------------------------
+
+_NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _norm_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
+    """Check one of layer norm's N×D operands against X; columns side by side."""
+    if t.dim() != 2 or t.shape != like.shape:
+        raise ValueError(f"{name} must be N×D like X, got {tuple(t.shape)}")
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must have X's type and device")
+    # any distance between rows is taken as it is, an expanded row (0) too
+    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _norm_columns(t: Optional[torch.Tensor], X: torch.Tensor, name: str):
+    if t is None:
+        return None
+    if t.shape != (X.shape[1],):
+        raise ValueError(f"{name} must have one value per column, got {tuple(t.shape)}")
+    if t.device != X.device:
+        raise ValueError(f"{name} must be on X's device")
+    return t.to(torch.float32).contiguous()
+
+
+def _check_norm(X: torch.Tensor, activation: str) -> None:
+    if X.dim() != 2 or X.shape[1] < 1:
+        raise ValueError(f"layer norm takes N×D with D >= 1, got {tuple(X.shape)}")
+    if X.dtype not in _NORM_TYPES:
+        raise ValueError(f"layer norm takes f32, bf16 or f16, got {X.dtype}")
+    if activation not in ("none", "relu", "sigmoid"):
+        raise ValueError(f"Unsupported activation {activation!r}")
+
+
+def layer_norm(
+    X: torch.Tensor,  # N×D f32, bf16 or f16
+    weight: Optional[torch.Tensor] = None,  # D (None = 1)
+    bias: Optional[torch.Tensor] = None,    # D (None = 0)
+    eps: float = 1e-5,
+    activation: str = "none",
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Y = act((X − mean) · rstd · weight + bias), each row by its own mean and
+    variance. Returns (Y like X, mean N, rstd N); the statistics are fp32 and
+    are what ``layer_norm_grad`` takes. rstd = 1/√(var + eps), var over D.
+    Rows may lie any distance apart; N = 0 gives empty results.
+    """
+    _check_norm(X, activation)
+    X = _norm_rows(X, X, "X")
+    weight = _norm_columns(weight, X, "weight")
+    bias = _norm_columns(bias, X, "bias")
+    if hip_available(X):
+        return get_ext().layer_norm(X, weight, bias, float(eps), _act_code(activation))
+    x = X.to(torch.float32)
+    mean = x.mean(dim=1)
+    x = x - mean.unsqueeze(1)
+    rstd = 1.0 / torch.sqrt((x * x).mean(dim=1) + eps)
+    z = x * rstd.unsqueeze(1)
+    if weight is not None:
+        z = z * weight
+    if bias is not None:
+        z = z + bias
+    return _act(z, activation).to(X.dtype), mean, rstd
+
+
+def layer_norm_grad(
+    dY: torch.Tensor,    # N×D: gradient of Y
+    X: torch.Tensor,     # N×D: the input
+    mean: torch.Tensor,  # N f32, from layer_norm
+    rstd: torch.Tensor,  # N f32, from layer_norm
+    weight: Optional[torch.Tensor] = None,
+    y: Optional[torch.Tensor] = None,  # N×D: the output, if there is an activation
+    activation: str = "none",
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Backward pass of ``layer_norm``: (dX like X, dweight D f32, dbias D f32).
+
+    The activation's derivative is taken from the output ``y`` (relu: y > 0,
+    sigmoid: y·(1 − y)), as in the rest of the MLP backward. dweight and dbias
+    are sums over the local rows in a fixed order (two runs agree bit for bit);
+    they are given for a missing weight or bias too. N = 0 gives zeros.
+    """
+    _check_norm(X, activation)
+    X = _norm_rows(X, X, "X")
+    dY = _norm_rows(dY, X, "dY")
+    if activation == "none":
+        y = None
+    elif y is None:
+        raise ValueError(f"the gradient of activation {activation!r} needs the output y")
+    else:
+        y = _norm_rows(y, X, "y")
+    weight = _norm_columns(weight, X, "weight")
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.shape != (X.shape[0],) or t.dtype != torch.float32 or t.device != X.device:
+            raise ValueError(f"{name} must be one f32 per row on X's device")
+    if hip_available(X):
+        return get_ext().layer_norm_grad(
+            dY, X, mean.contiguous(), rstd.contiguous(), weight, y, _act_code(activation)
+        )
+    xh = (X.to(torch.float32) - mean.unsqueeze(1)) * rstd.unsqueeze(1)
+    dz = dY.to(torch.float32)
+    if activation == "relu":
+        dz = torch.where(y > 0, dz, torch.zeros_like(dz))
+    elif activation == "sigmoid":
+        yf = y.to(torch.float32)
+        dz = dz * (yf * (1.0 - yf))
+    p = dz if weight is None else dz * weight
+    dX = rstd.unsqueeze(1) * (
+        p - p.mean(dim=1, keepdim=True) - xh * (p * xh).mean(dim=1, keepdim=True)
+    )
+    return dX.to(X.dtype), (dz * xh).sum(dim=0), dz.sum(dim=0)
+
+
 def softmax_xent_grad(
     logits: torch.Tensor, y: torch.Tensor, w: Optional[torch.Tensor] = None
 ) -> Tuple[torch.Tensor, torch.Tensor]:
