@@ -32,6 +32,7 @@ def build(verbose: bool = True) -> str:
         os.path.join(_HERE, "tree_kernels.hip"),
         os.path.join(_HERE, "mlp_kernels.hip"),
         os.path.join(_HERE, "norm_kernels.hip"),
+        os.path.join(_HERE, "muon_kernels.hip"),
     ]
     cflags = ["-O3"]
     # packed fp32 instructions (v_pk_*_f32) stay off: some of their forms have

@@ -61,6 +61,10 @@ void launch_layer_norm_grad(int, const void*, long long, const void*,
                             long long, const void*, long long, const float*,
                             const float*, const float*, void*, float*, float*,
                             long long, int, int, void*);
+long long muon_workspace(int, const int*, const int*);
+void launch_muon(int, const int*, const int*, const void* const*, float* const*,
+                 void* const*, const float*, int, int, float, float, float, int,
+                 int, const float*, float, int, void*, void*);
 }
 
 static void* cur_stream() {
@@ -410,12 +414,12 @@ std::tuple<torch::Tensor, torch::Tensor> wgrad_f32(torch::Tensor X,
 
 // ---- layer norm ------------------------------------------------------------
 
-static int norm_type(const torch::Tensor& t) {
+static int float_type(const torch::Tensor& t) {
   switch (t.scalar_type()) {
     case torch::kFloat32: return 0;
     case torch::kBFloat16: return 1;
     case torch::kFloat16: return 2;
-    default: TORCH_CHECK(false, "layer norm takes f32, bf16 or f16");
+    default: TORCH_CHECK(false, "expected f32, bf16 or f16");
   }
 }
 
@@ -447,7 +451,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm(
     torch::Tensor X, c10::optional<torch::Tensor> weight,
     c10::optional<torch::Tensor> bias, double eps, int64_t act) {
   check_rows(X, X, "X");
-  const int type = norm_type(X);
+  const int type = float_type(X);
   TORCH_CHECK(X.size(1) >= 1 && X.size(1) <= (1 << 28), "columns out of range");
   const at::cuda::OptionalCUDAGuard guard(X.device());
   const float* g = opt_columns(weight, X, "weight");
@@ -475,7 +479,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_grad(
     TORCH_CHECK(Y.has_value(), "an activation's gradient needs Y");
     check_rows(*Y, X, "Y");
   }
-  const int type = norm_type(X);
+  const int type = float_type(X);
   TORCH_CHECK(X.size(1) >= 1 && X.size(1) <= (1 << 28), "columns out of range");
   const long long N = X.size(0);
   const int D = (int)X.size(1);
@@ -499,6 +503,77 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_grad(
   return {dX, out[0], out[1]};
 }
 
+// ---- Newton-Schulz and the optimiser step ------------------------------------
+
+static void muon_call(const std::vector<torch::Tensor>& g,
+                      const std::vector<torch::Tensor>& mom,
+                      const std::vector<torch::Tensor>& w,
+                      const std::vector<double>& step, double mu, double keep,
+                      bool nesterov, int64_t steps,
+                      const std::vector<double>& coef, double eps,
+                      double scale_b) {
+  const size_t n = g.size();
+  TORCH_CHECK(n > 0 && w.size() == n && coef.size() == 3 && steps >= 1,
+              "muon: bad arguments");
+  TORCH_CHECK((mom.empty() && step.empty()) ||
+                  (mom.size() == n && step.size() == n),
+              "muon: one buffer and one step per matrix");
+  const at::cuda::OptionalCUDAGuard guard(g[0].device());
+  std::vector<int> rows(n), cols(n);
+  std::vector<const void*> gp(n);
+  std::vector<float*> mp(n);
+  std::vector<void*> wp(n);
+  std::vector<float> sp(n);
+  for (size_t k = 0; k < n; ++k) {
+    TORCH_CHECK(g[k].dim() == 2 && g[k].numel() > 0 && g[k].is_contiguous() &&
+                    g[k].device() == g[0].device() &&
+                    g[k].scalar_type() == g[0].scalar_type(),
+                "gradients: contiguous matrices of one type on one device");
+    TORCH_CHECK(g[k].size(0) < (1 << 24) && g[k].size(1) < (1 << 24),
+                "matrix too large");
+    TORCH_CHECK(w[k].sizes() == g[k].sizes() && w[k].is_contiguous() &&
+                    w[k].device() == g[0].device() &&
+                    w[k].scalar_type() == w[0].scalar_type(),
+                "weights: contiguous, like the gradients");
+    rows[k] = (int)g[k].size(0);
+    cols[k] = (int)g[k].size(1);
+    gp[k] = g[k].data_ptr();
+    wp[k] = w[k].data_ptr();
+    if (!mom.empty()) {
+      TORCH_CHECK(mom[k].sizes() == g[k].sizes() && mom[k].is_contiguous() &&
+                      mom[k].device() == g[0].device() &&
+                      mom[k].scalar_type() == torch::kFloat32,
+                  "momentum buffers: contiguous f32, like the gradients");
+      mp[k] = mom[k].data_ptr<float>();
+      sp[k] = (float)step[k];
+    }
+  }
+  const float cf[3] = {(float)coef[0], (float)coef[1], (float)coef[2]};
+  const int gtype = float_type(g[0]), wtype = float_type(w[0]);
+  auto ws = torch::empty({muon_workspace((int)n, rows.data(), cols.data())},
+                         g[0].options().dtype(torch::kUInt8));
+  // three products everywhere unless the result is rounded to bf16
+  launch_muon((int)n, rows.data(), cols.data(), gp.data(),
+              mom.empty() ? nullptr : mp.data(), wp.data(),
+              mom.empty() ? nullptr : sp.data(), gtype, wtype, (float)mu,
+              (float)keep, (float)eps, nesterov, (int)steps, cf,
+              (float)scale_b, wtype != 1, ws.data_ptr(), cur_stream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+void newton_schulz(std::vector<torch::Tensor> g, std::vector<torch::Tensor> out,
+                   int64_t steps, std::vector<double> coef, double eps,
+                   double scale_b) {
+  muon_call(g, {}, out, {}, 0.0, 1.0, false, steps, coef, eps, scale_b);
+}
+
+void muon_update(std::vector<torch::Tensor> w, std::vector<torch::Tensor> g,
+                 std::vector<torch::Tensor> mom, std::vector<double> step,
+                 double mu, double keep, bool nesterov, int64_t steps,
+                 std::vector<double> coef, double eps, double scale_b) {
+  muon_call(g, mom, w, step, mu, keep, nesterov, steps, coef, eps, scale_b);
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bin_codes", &bin_codes, "K4a quantile binning");
   m.def("tree_hist_cls", &tree_hist_cls, "K2 class histograms (all trees)");
@@ -514,5 +589,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gemm_bias_act", &gemm_bias_act, "K5 fused MFMA GEMM+bias+act");
   m.def("layer_norm", &layer_norm, "layer norm + activation, row statistics");
   m.def("layer_norm_grad", &layer_norm_grad, "dX, dweight, dbias of layer norm");
+  m.def("newton_schulz", &newton_schulz, "orthogonalised matrices");
+  m.def("muon_update", &muon_update, "momentum, orthogonalisation, weights");
   m.def("wgrad_bias", &wgrad_bias, "K7 split-N wgrad + fused bias grad");
 }

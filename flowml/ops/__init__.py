@@ -20,8 +20,10 @@ flagship hot loop touches).
 
 from __future__ import annotations
 
+import functools
+import math
 import os
-from typing import List, Optional, Tuple
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -759,6 +761,205 @@ def layer_norm_grad(
         p - p.mean(dim=1, keepdim=True) - xh * (p * xh).mean(dim=1, keepdim=True)
     )
     return dX.to(X.dtype), (dz * xh).sum(dim=0), dz.sum(dim=0)
+
+
+# ---------------------------------------------------------------------------
+# Newton-Schulz orthogonalisation and the optimiser step around it
+# ---------------------------------------------------------------------------
+
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_scale(steps: int, coefficients: Tuple[float, float, float]) -> float:
+    """Check the polynomial a·s + b·s³ + c·s⁵ and find the power of two that
+    brings b·A + c·A² into fp16.
+
+    Singular values start in [0, 1]. The kernels hold the iterates in fp16
+    pairs scaled by 2^14, so they must stay under 1.9; a polynomial that lets
+    them grow further does not orthogonalise either.
+    """
+    if steps < 1 or int(steps) != steps:
+        raise ValueError(f"steps must be a whole number >= 1, got {steps!r}")
+    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+        raise ValueError(f"coefficients must be three finite numbers, got {coefficients!r}")
+    a, b, c = coefficients
+
+    def crest(f, slope2, top):
+        # |f| on [0, top] peaks at an end or where the slope, a quadratic in
+        # s², is zero
+        p, q, r = slope2
+        at = [top]
+        roots = []
+        if r:
+            disc = q * q - 4 * p * r
+            if disc >= 0:
+                roots = [(-q + sg * math.sqrt(disc)) / (2 * r) for sg in (1, -1)]
+        elif q:
+            roots = [-p / q]
+        at += [math.sqrt(v) for v in roots if 0 < v < top * top]
+        return max(abs(f(s)) for s in at)
+
+    top, widest = 1.0, 1.0
+    for _ in range(steps):
+        widest = max(widest, top)
+        top = crest(lambda s: a * s + b * s**3 + c * s**5, (a, 3 * b, 5 * c), top)
+        if not top <= 1.9:
+            raise ValueError(
+                f"coefficients {coefficients!r} let singular values grow to {top:.3g} "
+                "(at most 1.9)"
+            )
+    most = crest(lambda s: b * s**2 + c * s**4, (b, 2 * c, 0.0), widest)
+    return 2.0 ** min(14, math.floor(math.log2(32768.0 / max(most, 1e-30))))
+
+
+def _ns_matrices(ts: Sequence[torch.Tensor], name: str) -> None:
+    for t in ts:
+        if not isinstance(t, torch.Tensor) or t.dim() != 2:
+            raise ValueError(f"{name} must be matrices")
+        if t.dtype not in _NORM_TYPES:
+            raise ValueError(f"{name} must be f32, bf16 or f16, got {t.dtype}")
+        if t.dtype != ts[0].dtype or t.device != ts[0].device:
+            raise ValueError(f"{name} must have one type and one device")
+
+
+def _ns_torch(u: torch.Tensor, steps: int, coefficients, eps: float) -> torch.Tensor:
+    a, b, c = coefficients
+    x = u.to(torch.float32)
+    norm = float(x.to(torch.float64).square().sum().sqrt())
+    x = x / (eps if norm <= eps else norm)
+    if x.shape[0] > x.shape[1]:
+        x = x.T
+    for _ in range(steps):
+        p = x @ x.T
+        x = a * x + (b * p + c * (p @ p)) @ x
+    return x if u.shape[0] <= u.shape[1] else x.T
+
+
+def newton_schulz(
+    G: Union[torch.Tensor, Sequence[torch.Tensor]],
+    steps: int = 5,
+    coefficients: Tuple[float, float, float] = NS_COEFFICIENTS,
+    eps: float = 1e-7,
+):
+    """Orthogonalise a matrix, a stack of matrices (B×m×n) or a sequence of
+    matrices of any shapes: with G = U·S·Vᵀ, about U·Vᵀ.
+
+    X₀ = G / max(‖G‖_F, eps), then `steps` times, with A = X·Xᵀ on the shorter
+    side, X ← a·X + (b·A + c·A²)·X. The polynomial moves every singular value
+    towards 1 (the default one into [0.7, 1.2], fast for small ones). The
+    result has G's type; f32 and f16 are computed as exactly as in fp32. All
+    matrices of a call share their kernel launches. A matrix that holds a NaN
+    or an infinity comes out as NaN, an empty one as it is.
+    """
+    coefficients = tuple(float(v) for v in coefficients)
+    scale = _ns_scale(steps, coefficients)
+    if not 1e-30 <= eps < math.inf:
+        raise ValueError(f"eps must be finite and at least 1e-30, got {eps!r}")
+    if isinstance(G, torch.Tensor):
+        if G.dim() == 2:
+            return newton_schulz([G], steps, coefficients, eps)[0]
+        if G.dim() != 3:
+            raise ValueError(f"newton_schulz takes m×n or B×m×n, got {tuple(G.shape)}")
+        if G.dtype not in _NORM_TYPES:
+            raise ValueError(f"G must be f32, bf16 or f16, got {G.dtype}")
+        out = torch.empty(G.shape, dtype=G.dtype, device=G.device)
+        G, outs = G.unbind(0), out.unbind(0)
+    else:
+        G = list(G)
+        _ns_matrices(G, "G")
+        out = outs = [torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in G]
+    live = [k for k, g in enumerate(G) if g.numel()]
+    if live and hip_available(G[0]):
+        get_ext().newton_schulz([G[k].contiguous() for k in live], [outs[k] for k in live],
+                                steps, coefficients, eps, scale)
+    else:
+        for k in live:
+            outs[k].copy_(_ns_torch(G[k], steps, coefficients, eps))
+    return out
+
+
+def muon_update(
+    weights: Sequence[torch.Tensor],  # f32, bf16 or f16, updated in place
+    grads: Sequence[torch.Tensor],
+    buffers: Sequence[torch.Tensor],  # f32 momentum, updated in place
+    lr: float,
+    momentum: float = 0.95,
+    weight_decay: float = 0.0,
+    nesterov: bool = True,
+    steps: int = 5,
+    coefficients: Tuple[float, float, float] = NS_COEFFICIENTS,
+    eps: float = 1e-7,
+) -> None:
+    """One optimiser step on a sequence of weight matrices, in place:
+
+        M ← momentum·M + G        U = G + momentum·M (nesterov) or M
+        W ← (1 − lr·weight_decay)·W − lr·0.2·√max(rows, cols)·newton_schulz(U)
+
+    The factor gives every update the same mean square (0.2·lr)², whatever the
+    shape, the same for a matrix and its transpose. Weights and buffers must be
+    contiguous and apart from each other in memory. The numbers are taken at
+    the call: a captured graph repeats the step with the lr it was captured with.
+    """
+    coefficients = tuple(float(v) for v in coefficients)
+    scale = _ns_scale(steps, coefficients)
+    if not 1e-30 <= eps < math.inf:
+        raise ValueError(f"eps must be finite and at least 1e-30, got {eps!r}")
+    if not 0 <= momentum < 1:
+        raise ValueError(f"momentum must be in [0, 1), got {momentum!r}")
+    weights, grads, buffers = list(weights), list(grads), list(buffers)
+    if not len(weights) == len(grads) == len(buffers):
+        raise ValueError("muon_update takes one gradient and one buffer per weight matrix")
+    if not weights:
+        return
+    _ns_matrices(weights, "weights")
+    _ns_matrices(grads, "grads")
+    _ns_matrices(buffers, "buffers")
+    if buffers[0].dtype != torch.float32:
+        raise ValueError("momentum buffers must be f32")
+    if not weights[0].device == grads[0].device == buffers[0].device:
+        raise ValueError("weights, grads and buffers must be on one device")
+    spans = []
+    for w, g, m in zip(weights, grads, buffers):
+        if w.shape != g.shape or w.shape != m.shape:
+            raise ValueError(
+                f"shapes differ: weight {tuple(w.shape)}, gradient {tuple(g.shape)}, "
+                f"buffer {tuple(m.shape)}"
+            )
+        if not (w.is_contiguous() and m.is_contiguous()):
+            raise ValueError("weights and buffers are updated in place: they must be contiguous")
+        for t, written in ((w, True), (m, True), (g, False)):
+            # a gradient that is not contiguous is copied before the step
+            if t.numel() and (written or t.is_contiguous()):
+                lo = t.data_ptr()
+                spans.append((lo, lo + t.numel() * t.element_size(), written))
+    spans.sort()
+    end_written = end_read = 0
+    for lo, hi, written in spans:
+        if lo < end_written or (written and lo < end_read):
+            raise ValueError("weights and buffers must not overlap in memory, nor with gradients")
+        if written:
+            end_written = max(end_written, hi)
+        else:
+            end_read = max(end_read, hi)
+    keep = 1.0 - lr * weight_decay
+    if hip_available(weights[0]):
+        live = [k for k, w in enumerate(weights) if w.numel()]
+        if live:
+            get_ext().muon_update(
+                [weights[k] for k in live], [grads[k].contiguous() for k in live],
+                [buffers[k] for k in live],
+                [lr * 0.2 * math.sqrt(max(weights[k].shape)) for k in live],
+                momentum, keep, nesterov, steps, coefficients, eps, scale,
+            )
+        return
+    for w, g, m in zip(weights, grads, buffers):
+        if not w.numel():
+            continue
+        g = g.to(torch.float32)
+        m.mul_(momentum).add_(g)
+        o = _ns_torch(g + momentum * m if nesterov else m, steps, coefficients, eps)
+        w.copy_(keep * w.to(torch.float32) - lr * 0.2 * math.sqrt(max(w.shape)) * o)
 
 
 def softmax_xent_grad(

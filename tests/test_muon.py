@@ -1,0 +1,269 @@
+"""Newton-Schulz orthogonalisation and the optimiser step against 64 bits."""
+
+import math
+
+import pytest
+import torch
+
+from flowml import ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+COEF = ops.NS_COEFFICIENTS
+
+
+def gradient(kind, m, n, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    rn = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    if kind == "full":
+        return rn(m, n)
+    if kind == "low":  # rank r and a little noise
+        r = max(1, min(m, n) // 16)
+        return rn(m, r) @ rn(r, n) / r ** 0.5 + 0.01 * rn(m, n)
+    if kind == "one":
+        return rn(m, 1) @ rn(1, n)
+    if kind == "offset":  # relu activations: one large singular value
+        return (torch.relu(rn(4 * max(m, n), m)).T @ rn(4 * max(m, n), n)) / max(m, n)
+    raise ValueError(kind)
+
+
+def reference(G, steps=5, coef=COEF, eps=1e-7):
+    """The definition in 64 bits, and the norms of the iterates."""
+    a, b, c = coef
+    x = G.double()
+    x = x / max(float(x.norm()), eps)
+    sizes = []
+    for _ in range(steps):
+        sizes.append(float(x.norm()))
+        if x.shape[0] <= x.shape[1]:
+            k = x @ x.T
+            x = a * x + (b * k + c * k @ k) @ x
+        else:
+            k = x.T @ x
+            x = a * x + x @ (b * k + c * k @ k)
+    return x, sizes
+
+
+def tolerance(G, sizes, dtype, coef=COEF):
+    """Bound of the error's 2-norm.
+
+    A step maps singular values by p; in the 2-norm its derivative is at most
+    L = max |p'| over their range (the largest divided difference). What a step
+    loses: pairs of fp16 hold 22 bits, and A, A^2, B and X are each rounded to
+    them (16 half steps cover the polynomial's factors |b| and 2|c|), sums of K
+    products in fp32 walk sqrt(K) quarters of that. It grows by L in each later
+    step. bf16 results are rounded once (half a step, 2^-8), and their A and B
+    are held in 11 bits: 5 steps of two such roundings, 2^-12 each as they are
+    spread, on values that |p'| <= 1.6 no longer grows: under 2^-8.
+    """
+    a, b, c = coef
+    s = torch.linspace(0, 1.2025, 2000).double()
+    L = float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max())
+    eta = 2.0 ** -22 * (16 + max(G.shape) ** 0.5)
+    tol = sum(L ** (len(sizes) - 1 - k) * eta * v * 1.0 for k, v in enumerate(sizes))
+    return tol
+
+
+def check(G, got, steps=5, coef=COEF, eps=1e-7):
+    ref, sizes = reference(G.cpu(), steps, coef, eps)
+    off = float((got.cpu().double() - ref).norm())
+    tol = tolerance(G, sizes, G.dtype, coef)
+    size = float(ref.norm())
+    if G.dtype == torch.bfloat16:
+        tol += (2.0 ** -8 + 2.0 ** -8) * size
+    elif G.dtype == torch.float16:
+        tol += 2.0 ** -11 * size + 2.0 ** -25 * G.numel() ** 0.5
+    assert got.dtype == G.dtype and got.shape == G.shape and got.is_contiguous()
+    assert off <= tol, (tuple(G.shape), G.dtype, off, tol, size)
+
+
+SHAPES = [(1, 1), (1, 7), (9, 1), (2, 2), (5, 3), (41, 128), (128, 64), (64, 5), (65, 64), (63, 200),
+          (130, 257), (1, 3000), (2000, 3)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["full", "low", "one", "offset"])
+def test_small(kind, dtype, dev):
+    grads = [gradient(kind, m, n, seed=m + n).to(dtype).to(dev) for m, n in SHAPES]
+    together = ops.newton_schulz(grads)
+    for g, o in zip(grads, together):
+        check(g, o)
+    # alone or in company, a matrix gives the same result within the bound
+    for g in grads[::4]:
+        check(g, ops.newton_schulz(g))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,n", [(255, 255), (256, 300), (300, 4000), (777, 1001), (1024, 512),
+                                 (2048, 2050)])
+def test_large(m, n, dtype):
+    for kind in ("full", "low", "one", "offset"):
+        G = gradient(kind, m, n, seed=3).to(dtype).cuda()
+        got = ops.newton_schulz(G)
+        check(G, got)
+        assert torch.equal(got, ops.newton_schulz(G))  # one order of sums
+
+
+@pytest.mark.gpu
+def test_many_matrices():
+    """More than one table of matrices, of one shape and of several."""
+    stack = torch.stack([gradient("full", 70, 33, seed=k) for k in range(53)]).cuda()
+    out = ops.newton_schulz(stack)
+    assert out.shape == stack.shape
+    for g, o in zip(stack, out):
+        check(g, o)
+    mixed = [gradient("full", 1 + 13 * (k % 17), 1 + 29 * (k % 11), seed=k).cuda() for k in range(60)]
+    for g, o in zip(mixed, ops.newton_schulz(mixed)):
+        check(g, o)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("coef,steps", [((1.5, -0.5, 0.0), 12), ((2.0, -1.5, 0.5), 9), (COEF, 1),
+                                        ((0.5, 0.0, 0.0), 2)])
+def test_other_polynomials(coef, steps, dev):
+    for m, n in ((30, 50), (200, 90)):
+        G = gradient("offset", m, n).to(dev)
+        check(G, ops.newton_schulz(G, steps=steps, coefficients=coef), steps, coef)
+    if steps > 8:  # these converge: the result is orthogonal
+        G = torch.eye(20, 30) + 0.1 * gradient("full", 20, 30)
+        o = ops.newton_schulz(G.to(dev), steps=steps, coefficients=coef).cpu()
+        assert (o @ o.T - torch.eye(20)).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_special_values(dev):
+    z = torch.zeros(40, 70, device=dev)
+    assert torch.equal(ops.newton_schulz(z), z)
+    # norms below eps are divided by eps; very small and very large ones keep
+    # their digits
+    G = gradient("full", 40, 70).to(dev)
+    G = G / G.norm()
+    check(G * 1e-9, ops.newton_schulz(G * 1e-9))
+    check(G * 1e-3, ops.newton_schulz(G * 1e-3, eps=1e-2), eps=1e-2)
+    check(G * 1e30, ops.newton_schulz(G * 1e30))
+    check(G * 1e-28, ops.newton_schulz(G * 1e-28, eps=1e-30), eps=1e-30)
+    for bad in (float("nan"), float("inf")):
+        H = G.clone()
+        H[3, 5] = bad
+        other = ops.newton_schulz([H, G])
+        assert other[0].isnan().all()
+        check(G, other[1])
+    # empty matrices, an empty stack, an empty sequence
+    outs = ops.newton_schulz([G, G[:0], G[:, :0]])
+    check(G, outs[0])
+    assert outs[1].shape == (0, 70) and outs[2].shape == (40, 0)
+    assert ops.newton_schulz(G[None][:0]).shape == (0, 40, 70)
+    assert ops.newton_schulz([]) == []
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_strides(dev):
+    base = gradient("full", 90, 140).to(dev)
+    for G in (base.T, base[::2, 3:77], base[:, ::3], base[:1].expand(30, 140)):
+        check(G, ops.newton_schulz(G))
+
+
+def step_reference(w, g, m, lr, mu, wd, nesterov, steps=5):
+    m = mu * m.double() + g.double()
+    u = g.double() + mu * m if nesterov else m
+    o, sizes = reference(u, steps)
+    s = lr * 0.2 * math.sqrt(max(w.shape))
+    return (1 - lr * wd) * w.double() - s * o, m, u, sizes, s
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("wtype,gtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
+                                         (torch.float32, torch.bfloat16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("nesterov", [True, False])
+def test_update(wtype, gtype, nesterov, dev):
+    shapes = [(41, 128), (128, 64), (64, 5), (0, 4), (300, 290), (1, 1)]
+    ws = [gradient("full", *s, seed=1).to(wtype).to(dev) for s in shapes]
+    ms = [gradient("offset", *s, seed=2).to(dev) if s[0] else torch.zeros(s, device=dev) for s in shapes]
+    for turn in range(2):
+        gs = [gradient("full", *s, seed=3 + turn).to(gtype).to(dev) for s in shapes]
+        before = [(w.clone(), m.clone()) for w, m in zip(ws, ms)]
+        ops.muon_update(ws, gs, ms, lr=0.05, momentum=0.9, weight_decay=0.1, nesterov=nesterov)
+        for (w0, m0), w, m, g in zip(before, ws, ms, gs):
+            if not w.numel():
+                continue
+            ref, mref, u, sizes, s = step_reference(w0.cpu(), g.cpu(), m0.cpu(), 0.05, 0.9, 0.1, nesterov)
+            # buffer: two roundings, and mu in fp32
+            e = 2.0 ** -23 * ((0.9 * m0.cpu().double()).abs() + mref.abs())
+            assert ((m.cpu().double() - mref).abs() <= e).all()
+            tol = s * (tolerance(u, sizes, wtype) + 2.0 ** -22 * float(ref.norm()))
+            tol += 2.0 ** -22 * float(ref.norm())
+            if wtype != torch.float32:
+                tol += torch.finfo(wtype).eps / 2 * float(ref.norm())
+            if wtype == torch.bfloat16:
+                tol += s * 2.0 ** -8 * math.sqrt(min(w.shape))
+            assert float((w.cpu().double() - ref).norm()) <= tol
+
+
+@pytest.mark.gpu
+def test_update_twice_the_same_and_in_a_graph():
+    shapes = [(41, 128), (300, 500), (129, 5)]
+    mk = lambda seed: [gradient("offset", *s, seed=seed).cuda() for s in shapes]  # noqa: E731
+    ws, gs, ms = mk(1), mk(2), mk(3)
+
+    def step(w, g, m):
+        ops.muon_update(w, g, m, lr=0.02, weight_decay=0.01)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    we, me = [w.clone() for w in ws], [m.clone() for m in ms]
+    with torch.cuda.stream(s):
+        step([w.clone() for w in ws], gs, [m.clone() for m in ms])
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(ws, gs, ms)
+    for turn in range(4):
+        for g, f in zip(gs, mk(10 + turn)):
+            g.copy_(f)
+        step(we, gs, me)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(ws + ms, we + me))
+
+
+def test_refusals():
+    w, g, m = torch.randn(6, 4), torch.randn(6, 4), torch.zeros(6, 4)
+    step = lambda *a, **k: ops.muon_update(*a, lr=0.1, **k)  # noqa: E731
+    flat = torch.zeros(40)
+    bad = [
+        lambda: ops.newton_schulz(g[0]),
+        lambda: ops.newton_schulz(g.double()),
+        lambda: ops.newton_schulz(g.double()[None]),
+        lambda: ops.newton_schulz([g, g.bfloat16()]),
+        lambda: ops.newton_schulz([g, g[0]]),
+        lambda: ops.newton_schulz([g, 3.0]),
+        lambda: ops.newton_schulz(g, steps=0),
+        lambda: ops.newton_schulz(g, steps=1.5),
+        lambda: ops.newton_schulz(g, eps=0.0),
+        lambda: ops.newton_schulz(g, eps=float("nan")),
+        lambda: ops.newton_schulz(g, eps=1e-35),
+        lambda: ops.newton_schulz(g, coefficients=(3.0, 0.0, 0.0)),
+        lambda: ops.newton_schulz(g, coefficients=(1.0, 2.0)),
+        lambda: ops.newton_schulz(g, coefficients=(float("nan"), 0.0, 0.0)),
+        lambda: step([w], [g], []),
+        lambda: step([w], [g[:5]], [m]),
+        lambda: step([w], [g], [m.bfloat16()]),
+        lambda: step([w.double()], [g], [m]),
+        lambda: step([w.T], [g.T], [m.T]),
+        lambda: step([w, w], [g, g], [m, m.clone()]),
+        lambda: step([w, w.clone()], [g, g], [m, m]),
+        lambda: step([w], [g], [w]),
+        lambda: step([w], [m], [m]),
+        lambda: step([w], [w], [m]),
+        lambda: step([flat[:24].view(6, 4)], [g], [flat[16:40].view(6, 4)]),
+        lambda: step([w], [g], [m], momentum=1.0),
+        lambda: step([w], [g], [m], momentum=-0.1),
+    ]
+    keep = [t.clone() for t in (w, g, m)]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            print("not refused:", i)
+    assert all(torch.equal(p, q) for p, q in zip(keep, (w, g, m)))
+    step([], [], [])
