@@ -37,6 +37,8 @@
 #include <hip/hip_bf16.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
+#include <stdlib.h>  // TUNING
 
 namespace {
 
@@ -60,6 +62,7 @@ struct Mat {
   void* w;         // weights, or the result
   int m, n;        // shorter and longer side
   int mp, np;      // padded to whole tiles
+  int ldm, ldn;    // distance of working rows that run along m, along n
   int rows, cols;  // as the caller has it
   int full;        // 1: three products everywhere
   float step;
@@ -77,17 +80,18 @@ struct Table {
 
 // ---- working planes ---------------------------------------------------------
 
-__host__ __device__ inline size_t plane_x(const Mat& t) { return (size_t)t.mp * t.np; }
-__host__ __device__ inline size_t plane_a(const Mat& t) { return (size_t)t.mp * t.mp; }
+__host__ __device__ inline size_t plane_x(const Mat& t) { return (size_t)t.mp * t.ldn; }
+__host__ __device__ inline size_t plane_xt(const Mat& t) { return (size_t)t.np * t.ldm; }
+__host__ __device__ inline size_t plane_a(const Mat& t) { return (size_t)t.mp * t.ldm; }
 __device__ __forceinline__ f16* ws_x(const Mat& t, int p) { return t.ws + p * plane_x(t); }
 __device__ __forceinline__ f16* ws_xt(const Mat& t, int which, int p) {
-  return t.ws + (2 + 2 * which + p) * plane_x(t);
+  return t.ws + 2 * plane_x(t) + (2 * which + p) * plane_xt(t);
 }
 __device__ __forceinline__ f16* ws_a(const Mat& t, int p) {
-  return t.ws + 6 * plane_x(t) + p * plane_a(t);
+  return t.ws + 2 * plane_x(t) + 4 * plane_xt(t) + p * plane_a(t);
 }
 __device__ __forceinline__ f16* ws_b(const Mat& t, int p) {
-  return t.ws + 6 * plane_x(t) + (2 + p) * plane_a(t);
+  return t.ws + 2 * plane_x(t) + 4 * plane_xt(t) + (2 + p) * plane_a(t);
 }
 
 __device__ __forceinline__ int find(const Table& tab, int block) {
@@ -140,7 +144,8 @@ __global__ __launch_bounds__(256) void flowml_ns_first(Table tab, int norm_block
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   const int b = blockIdx.x - t.first;
   const bool turned = t.rows > t.cols;  // the caller's rows run along n
-  const int prow = turned ? t.np : t.mp, pcol = turned ? t.mp : t.np;
+  const int pcol = turned ? t.mp : t.np;
+  const int ld_straight = turned ? t.ldm : t.ldn, ld_turned = turned ? t.ldn : t.ldm;
   const int r0 = (b / (pcol / 64)) * 64, c0 = (b % (pcol / 64)) * 64;
 
   // |G|: every block adds the same partial sums in the same order
@@ -171,15 +176,15 @@ __global__ __launch_bounds__(256) void flowml_ns_first(Table tab, int norm_block
       u *= scale;
     }
     const f16 hi = (f16)u, lo = (f16)(u - (float)hi);
-    straight[0][(size_t)r * pcol + c] = hi;
-    straight[1][(size_t)r * pcol + c] = lo;
+    straight[0][(size_t)r * ld_straight + c] = hi;
+    straight[1][(size_t)r * ld_straight + c] = lo;
     tile[i][tc] = (uint32_t)__builtin_bit_cast(uint16_t, hi) |
                   ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
   }
   __syncthreads();
   for (int i = tr; i < 64; i += 4) {
     const uint32_t v = tile[tc][i];
-    const size_t at = (size_t)(c0 + i) * prow + r0 + tc;
+    const size_t at = (size_t)(c0 + i) * ld_turned + r0 + tc;
     turned_p[0][at] = __builtin_bit_cast(f16, (uint16_t)(v & 0xffff));
     turned_p[1][at] = __builtin_bit_cast(f16, (uint16_t)(v >> 16));
   }
@@ -189,100 +194,175 @@ __global__ __launch_bounds__(256) void flowml_ns_first(Table tab, int norm_block
 
 enum { TO_A = 0, TO_B = 1, TO_X = 2, TO_END = 3 };
 
+// A block's tile and the WM x WN waves that share it.
+template <int TM_, int TN_, int WM_, int WN_>
+struct Tile {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, WAVES = WM * WN;
+  static constexpr int FM = TM / WM / 32, FN = TN / WN / 32;
+};
+
 template <int BK>
 __device__ __forceinline__ int swizzle(int chunk, int row) {
-  // eight neighbouring rows' pieces of one chunk fall on all 32 banks
-  return BK == 64 ? (chunk ^ (row & 7)) : (chunk ^ ((row >> 1) & 3));
+  // 16 neighbouring rows' pieces of one chunk fall on all 64 banks
+  return BK == 64 ? (chunk ^ ((row >> 1) & 7)) : (chunk ^ ((row >> 2) & 3));
 }
 
-// acc += P Q^T over K: P has TM rows, Q TN rows, BK values of K at a time.
-// PA, PB: planes of each (2: hi and lo).
-template <int TM, int TN, int WM, int WN, int BK, int PA, int PB>
-__device__ __forceinline__ void product(const f16* const (&P)[2], int ldp,
-                                        const f16* const (&Q)[2], int ldq, int K, f16* lds,
-                                        f32x16 (&acc)[TM / WM / 32][TN / WN / 32]) {
-  constexpr int NT = WM * WN * 64;
-  constexpr int CH = BK / 8;                 // 16-byte chunks in a row
-  constexpr int LA = TM * CH / NT, LB = TN * CH / NT;
-  constexpr int FM = TM / WM / 32, FN = TN / WN / 32;
-  constexpr int STAGE = (PA * TM + PB * TN) * BK;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = (wave / WN) * (TM / WM), wn = (wave % WN) * (TN / WN);
+typedef __attribute__((address_space(3))) void lds_void;
 
-  f16x8 ra[PA][LA], rb[PB][LB];
-  auto fetch = [&](int k0) {
-#pragma unroll
-    for (int p = 0; p < PA; ++p)
-#pragma unroll
-      for (int i = 0; i < LA; ++i) {
-        const int c = tid + i * NT;
-        ra[p][i] = *(const f16x8*)(P[p] + (size_t)(c / CH) * ldp + k0 + (c % CH) * 8);
-      }
-#pragma unroll
-    for (int p = 0; p < PB; ++p)
-#pragma unroll
-      for (int i = 0; i < LB; ++i) {
-        const int c = tid + i * NT;
-        rb[p][i] = *(const f16x8*)(Q[p] + (size_t)(c / CH) * ldq + k0 + (c % CH) * 8);
-      }
-  };
-  auto keep = [&](f16* s) {
-#pragma unroll
-    for (int p = 0; p < PA; ++p)
-#pragma unroll
-      for (int i = 0; i < LA; ++i) {
-        const int c = tid + i * NT, r = c / CH;
-        *(f16x8*)(s + p * TM * BK + r * BK + swizzle<BK>(c % CH, r) * 8) = ra[p][i];
-      }
-#pragma unroll
-    for (int p = 0; p < PB; ++p)
-#pragma unroll
-      for (int i = 0; i < LB; ++i) {
-        const int c = tid + i * NT, r = c / CH;
-        *(f16x8*)(s + (PA * TM + p * TN) * BK + r * BK + swizzle<BK>(c % CH, r) * 8) = rb[p][i];
-      }
-  };
+// Where a lane's 16 bytes of 1 KB, piece `piece` of a plane of rows of BK
+// values, come from.  They land in LDS at 16 * lane, so the swizzle is here.
+template <int BK>
+__device__ __forceinline__ int source_of(int ld, int piece, int lane) {
+  constexpr int CH = BK / 8;
+  const int slot = piece * 64 + lane, row = slot / CH;
+  return row * ld * 2 + swizzle<BK>(slot % CH, row) * 16;
+}
 
-  fetch(0);
-  keep(lds);
-  __syncthreads();
-  int turn = 0;
-  for (int k0 = 0; k0 < K; k0 += BK, turn ^= 1) {
-    if (k0 + BK < K) fetch(k0 + BK);
-    const f16* s = lds + turn * STAGE;
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// All waves' LDS reads so far are over and their finished copies can be seen.
+__device__ __forceinline__ void block_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// acc += P Q^T over K: P has TM rows, Q TN rows.  PA, PB: planes of each (2:
+// hi and lo).  S stages of operands in LDS: the copies of S - 1 steps are under
+// way while a step is multiplied, and a step waits for its own copies alone.
+//
+// A step is cut into units of some matrix instructions.  Between them a unit
+// sends its share of the copies and reads the next unit's fragments, across
+// the steps' borders too: a wave issues in order, and a row of reads in front
+// of the multiplications keeps the matrix core idle as long as LDS takes to
+// accept them (64 x 64 tiles: 1040 cycles a step, 400 of them multiplying).
+// The scheduling barriers keep the compiler from gathering them again.
+template <class T, int BK, int S, int PA, int PB>
+__device__ __forceinline__ void product(const f16* const (&P)[2], const f16* const (&Q)[2], int ld,
+                                        int K, f16* lds, f32x16 (&acc)[T::FM][T::FN]) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know buffer resources
+  constexpr int STAGE = (PA * T::TM + PB * T::TN) * BK;
+  constexpr int LA = T::TM * BK / 512 / T::WAVES, LB = T::TN * BK / 512 / T::WAVES;
+  constexpr int LOADS = PA * LA + PB * LB;  // copies per wave and stage
+  constexpr int KU = T::FM == 1 ? 2 : 1;    // slices of K to a unit
+  constexpr int KG = BK / 16 / KU, UNITS = KG * T::FM;
+  // units that send copies: with two stages these are waited for at this
+  // step's end, and leave early
+  constexpr int SPREAD = S == 2 ? (UNITS + 3) / 4 : UNITS;
+  static_assert(KG % 2 == 0, "fragments alternate between two sets");
+  static_assert(T::TM * BK % (512 * T::WAVES) == 0 && T::TN * BK % (512 * T::WAVES) == 0,
+                "every wave copies as much");
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave / T::WN) * (T::TM / T::WM), wn = (wave % T::WN) * (T::TN / T::WN);
+
+  // buffer loads: the lane's part of an address stays, the step's is a scalar
+  __amdgpu_buffer_rsrc_t rp[PA], rq[PB];
 #pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      f16x8 a[PA][FM], b[PB][FN];
-      const int chunk = kk * 2 + (lane >> 5);
+  for (int p = 0; p < PA; ++p)
+    rp[p] = __builtin_amdgcn_make_buffer_rsrc((void*)P[p], 0, T::TM * ld * 2, 0x00020000);
 #pragma unroll
-      for (int p = 0; p < PA; ++p)
+  for (int p = 0; p < PB; ++p)
+    rq[p] = __builtin_amdgcn_make_buffer_rsrc((void*)Q[p], 0, T::TN * ld * 2, 0x00020000);
+  int from_p[LA], from_q[LB];
 #pragma unroll
-        for (int f = 0; f < FM; ++f) {
-          const int r = wm + f * 32 + (lane & 31);
-          a[p][f] = *(const f16x8*)(s + p * TM * BK + r * BK + swizzle<BK>(chunk, r) * 8);
-        }
+  for (int i = 0; i < LA; ++i) from_p[i] = source_of<BK>(ld, wave * LA + i, lane);
 #pragma unroll
-      for (int p = 0; p < PB; ++p)
-#pragma unroll
-        for (int f = 0; f < FN; ++f) {
-          const int r = wn + f * 32 + (lane & 31);
-          b[p][f] =
-              *(const f16x8*)(s + (PA * TM + p * TN) * BK + r * BK + swizzle<BK>(chunk, r) * 8);
-        }
-#pragma unroll
-      for (int f = 0; f < FM; ++f)
-#pragma unroll
-        for (int g = 0; g < FN; ++g) {
-          if constexpr (PA == 2)
-            acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[1][f], b[0][g], acc[f][g], 0, 0, 0);
-          if constexpr (PB == 2)
-            acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][f], b[1][g], acc[f][g], 0, 0, 0);
-          acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[0][f], b[0][g], acc[f][g], 0, 0, 0);
-        }
+  for (int i = 0; i < LB; ++i) from_q[i] = source_of<BK>(ld, wave * LB + i, lane);
+  auto copy = [&](int k0, f16* s, int which) {
+    const bool first = which < PA * LA;
+    const int w = first ? which : which - PA * LA, l = first ? LA : LB;
+    const int p = w / l, i = w % l;
+    f16* to = s + (first ? p * T::TM : PA * T::TM + p * T::TN) * BK + (wave * l + i) * 512;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(first ? rp[p] : rq[p], (lds_void*)to, 16,
+                                             first ? from_p[i] : from_q[i], k0 * 2, 0, 0);
+  };
+  auto read = [&](const f16* plane, int row, int kk) {
+    return *(const f16x8*)(plane + row * BK + swizzle<BK>(kk * 2 + (lane >> 5), row) * 8);
+  };
+  f16x8 a[2][KU][PA], b[2][KU][PB][T::FN];
+  // Reads and multiplications of a unit, in the order in which the fragments
+  // are needed: lo hi, hi lo, hi hi.
+  auto read_one = [&](const f16* s, int u, int which) {
+    const int kg = u / T::FM, f = u % T::FM;
+    const int per = PA + (f == 0 ? PB * T::FN : 0), k = which / per, j = which % per;
+    const bool late = j > T::FN && f == 0;  // the planes of the second product
+    const int pb = PB == 2 && (PA == 2) == late ? 1 : 0;
+    if (j == 0 || (PA == 2 && j == (f == 0 ? T::FN + 1 : 1))) {
+      const int p = j == 0 ? PA - 1 : 0;
+      a[u & 1][k][p] = read(s + p * T::TM * BK, wm + f * 32 + (lane & 31), kg * KU + k);
+    } else {
+      const int g = late ? j - T::FN - PA : j - 1;
+      b[kg & 1][k][pb][g] = read(s + (PA * T::TM + pb * T::TN) * BK,
+                                 wn + g * 32 + (lane & 31), kg * KU + k);
     }
-    if (k0 + BK < K) keep(lds + (turn ^ 1) * STAGE);
-    __syncthreads();
-  }
+  };
+  constexpr int PAIRS = PA == 2 ? 3 : PB, MULS = KU * PAIRS * T::FN;
+  auto multiply_one = [&](int u, int which) {
+    const int kg = u / T::FM, f = u % T::FM;
+    const int k = which / (PAIRS * T::FN), c = which / T::FN % PAIRS, g = which % T::FN;
+    const int pa = PA == 2 && c == 0 ? 1 : 0, pb = PB == 2 && c == PAIRS - 2 ? 1 : 0;
+    acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u & 1][k][pa], b[kg & 1][k][pb][g],
+                                                       acc[f][g], 0, 0, 0);
+  };
+
+  // the last unit's copies that go behind the wait after its first instruction
+  constexpr int LAST = SPREAD < UNITS ? 0 : LOADS - (UNITS - 1) * LOADS / UNITS;
+  constexpr int REST = LAST - LAST / MULS;
+
+  const int steps = K / BK;
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i)
+    if (i < steps) {
+#pragma unroll
+      for (int c = 0; c < LOADS; ++c) copy(i * BK, lds + i * STAGE, c);
+    }
+  if (S - 1 <= steps)
+    wait_loads<LOADS*(S - 2)>();
+  else
+    wait_loads<0>();
+  block_barrier();
+#pragma unroll
+  for (int r = 0; r < KU * (PA + PB * T::FN); ++r) read_one(lds, 0, r);
+  int cur = 0, free = (S - 1) * STAGE;  // the stage read, and the one to fill
+  auto step = [&](auto more, int i) {
+    constexpr bool MORE = decltype(more)::value;
+    const int next = cur + STAGE == S * STAGE ? 0 : cur + STAGE;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const bool last = u + 1 == UNITS;
+      const int reads = KU * (PA + ((u + 1) % T::FM == 0 ? PB * T::FN : 0));
+      const int c0 = u < SPREAD ? u * LOADS / SPREAD : LOADS;
+      const int copies = u < SPREAD ? (u + 1) * LOADS / SPREAD - c0 : 0;
+#pragma unroll
+      for (int m = 0; m < MULS; ++m) {
+        multiply_one(u, m);
+        if (MORE) {
+#pragma unroll
+          for (int c = m * copies / MULS; c < (m + 1) * copies / MULS; ++c)
+            copy((i + S - 1) * BK, lds + free, c0 + c);
+        }
+        if (last && m == 0 && (MORE || i + 1 < steps)) {
+          // of this step's own copies, REST are still to be sent
+          wait_loads<MORE ? LOADS*(S - 2) - REST : 0>();
+          block_barrier();
+        }
+        if (!last || MORE || i + 1 < steps) {
+          // two at a time: what LDS delivers during a matrix instruction
+          const int r1 = m + 1 == MULS || 2 * m + 2 > reads ? reads : 2 * m + 2;
+#pragma unroll
+          for (int r = 2 * m; r < r1; ++r) read_one(lds + (last ? next : cur), (u + 1) % UNITS, r);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    free = cur;
+    cur = next;
+  };
+  int i = 0;
+  for (; i + S - 1 < steps; ++i) step(std::true_type{}, i);
+  for (; i < steps; ++i) step(std::false_type{}, i);
+#endif
 }
 
 __device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
@@ -290,124 +370,286 @@ __device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
   lo = (f16)(v - (float)hi);
 }
 
-// One tile of A, B, X' or the result.  `ka`, `kb`: the tile is
-// ka * (old tile) + kb * (product).
-template <int T, int WM, int WN, int BK, int TO>
-__global__ __launch_bounds__(WM * WN * 64) void flowml_ns_product(Table tab, int turn, float ka,
-                                                                  float kb) {
-  constexpr int FM = T / WM / 32, FN = T / WN / 32;
-  __shared__ __align__(16) f16 lds[2 * 4 * T * BK];
-  const Mat& t = tab.mat[find(tab, blockIdx.x)];
-  const int b = blockIdx.x - t.first;
-  int ti, tj;
-  if (TO == TO_A || TO == TO_B) {
-    // b = tj (tj + 1) / 2 + ti, ti <= tj
-    tj = (int)((sqrtf(8.f * b + 1.f) - 1.f) * 0.5f);
-    while ((tj + 1) * (tj + 2) / 2 <= b) ++tj;
-    while (tj * (tj + 1) / 2 > b) --tj;
-    ti = b - tj * (tj + 1) / 2;
+// 8 values side by side, `left` of them within the matrix.
+__device__ __forceinline__ void load8(const void* p, size_t at, int type, int left, float* v) {
+  if (left >= 8) {
+    if (type == T_F32) {
+      typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+      const f32x4 x = *(const f32x4*)((const float*)p + at), y = *(const f32x4*)((const float*)p + at + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = x[k], v[4 + k] = y[k];
+    } else if (type == T_BF16) {
+      typedef __bf16 b8 __attribute__((ext_vector_type(8), aligned(2)));
+      const b8 x = *(const b8*)((const __bf16*)p + at);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
+    } else {
+      typedef f16 h8 __attribute__((ext_vector_type(8), aligned(2)));
+      const h8 x = *(const h8*)((const f16*)p + at);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
+    }
   } else {
-    ti = b % (t.mp / T);
-    tj = b / (t.mp / T);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < left ? load_as(p, at + k, type) : 0.f;
   }
-  const int i0 = ti * T, j0 = tj * T;
+}
+
+__device__ __forceinline__ void store8(void* p, size_t at, int type, int left, const float* v) {
+  if (left >= 8) {
+    if (type == T_F32) {
+      typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+      *(f32x4*)((float*)p + at) = f32x4{v[0], v[1], v[2], v[3]};
+      *(f32x4*)((float*)p + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else if (type == T_BF16) {
+      typedef __bf16 b8 __attribute__((ext_vector_type(8), aligned(2)));
+      b8 x;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = (__bf16)v[k];
+      *(b8*)((__bf16*)p + at) = x;
+    } else {
+      typedef f16 h8 __attribute__((ext_vector_type(8), aligned(2)));
+      h8 x;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = (f16)v[k];
+      *(h8*)((f16*)p + at) = x;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < left) store_as(p, at + k, type, v[k]);
+  }
+}
+
+// The result, or the weights' update, for 8 values of one row of the caller's.
+__device__ __forceinline__ void deliver(const Table& tab, const Mat& t, int row, int col, float* v) {
+  if (row >= t.rows || col >= t.cols) return;
+  const size_t at = (size_t)row * t.cols + col;
+  if (t.mom) {
+    float w[8];
+    load8(t.w, at, tab.wtype, t.cols - col, w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = tab.keep * w[k] - t.step * v[k];
+  }
+  store8(t.w, at, tab.wtype, t.cols - col, v);
+}
+
+constexpr int kPieceLd = 36;                  // floats from row to row of a piece in LDS
+constexpr int kPieceHalfs = 32 * kPieceLd * 2;
+
+// The 32 x 32 piece at (i0, j0) of A, B, X' or the result: ka * (old value) +
+// kb * (product).  A lane holds 4 neighbouring rows of a column, 4 times; the
+// piece goes through the wave's own LDS so that every global access is 16
+// bytes per lane, 64 bytes in a row.  (Written from the registers, 2 and 8
+// bytes per lane, the tiles' ends took 8 us of 31 at 128 x 128 and 100 us of
+// 360 at 256 x 256.)
+template <int TO>
+__device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn, float ka, float kb,
+                                       int i0, int j0, bool mirror, const f32x16& acc, float* lds) {
+  const int lane = threadIdx.x & 63;
+  const bool turned = t.rows > t.cols;
+  f16* ch = TO == TO_A ? ws_a(t, 0) : TO == TO_B ? ws_b(t, 0) : ws_xt(t, turn ^ 1, 0);
+  f16* cl = TO == TO_A ? ws_a(t, 1) : TO == TO_B ? ws_b(t, 1) : ws_xt(t, turn ^ 1, 1);
+  const int r4 = lane >> 2, c8 = (lane & 3) * 8;
+  // the old values, from the copy in which i runs along rows
+  f16x8 oh[2], ol[2];
+  if (TO != TO_A) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const size_t at = (size_t)(j0 + h * 16 + r4) * t.ldm + i0 + c8;
+      oh[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 0) : ws_xt(t, turn, 0)) + at);
+      ol[h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      if (TO != TO_B || t.full)
+        ol[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 1) : ws_xt(t, turn, 1)) + at);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *(float4*)(lds + (lane & 31) * kPieceLd + q * 8 + (lane >> 5) * 4) =
+        make_float4(kb * acc[q * 4], kb * acc[q * 4 + 1], kb * acc[q * 4 + 2], kb * acc[q * 4 + 3]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int j = h * 16 + r4;
+    float* p = lds + j * kPieceLd + c8;
+    const float4 x = *(const float4*)p, y = *(const float4*)(p + 4);
+    float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    if (TO != TO_A) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += ka * ((float)oh[h][k] + (float)ol[h][k]);
+    }
+    if (TO == TO_END) {
+      if (turned) {
+        deliver(tab, t, j0 + j, i0 + c8, v);
+      } else {
+        *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4*)(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      }
+      continue;
+    }
+    f16x8 hi, lo;
+    uint32_t both[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      f16 a, b;
+      split(v[k], a, b);
+      hi[k] = a;
+      lo[k] = b;
+      both[k] = (uint32_t)__builtin_bit_cast(uint16_t, a) |
+                ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
+    }
+    const size_t at = (size_t)(j0 + j) * t.ldm + i0 + c8;
+    *(f16x8*)(ch + at) = hi;
+    if (TO == TO_X || t.full) *(f16x8*)(cl + at) = lo;
+    *(uint4*)p = make_uint4(both[0], both[1], both[2], both[3]);
+    *(uint4*)(p + 4) = make_uint4(both[4], both[5], both[6], both[7]);
+  }
+  if (!mirror || (TO == TO_END && turned)) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  f16* sh = TO == TO_X ? ws_x(t, 0) : ch;
+  f16* sl = TO == TO_X ? ws_x(t, 1) : cl;
+  const int ldc = TO == TO_X ? t.ldn : t.ldm;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int i = h * 16 + r4;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = lds[(c8 + k) * kPieceLd + i];
+    if (TO == TO_END) {
+      deliver(tab, t, i0 + i, j0 + c8, v);
+      continue;
+    }
+    f16x8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t u = __float_as_uint(v[k]);
+      hi[k] = __builtin_bit_cast(f16, (uint16_t)(u & 0xffff));
+      lo[k] = __builtin_bit_cast(f16, (uint16_t)(u >> 16));
+    }
+    const size_t at = (size_t)(i0 + i) * ldc + j0 + c8;
+    *(f16x8*)(sh + at) = hi;
+    if (t.full) *(f16x8*)(sl + at) = lo;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
+// Blocks go round the 8 XCDs in turn, each with an L2 of its own.  Every XCD
+// takes a run of neighbouring tiles instead, and a run is about square, so
+// that its blocks share operands in their L2.
+__device__ __forceinline__ int xcd_order(int block, int blocks) {
+  const int x = block & 7, each = blocks >> 3, more = blocks & 7;
+  return x * each + (x < more ? x : more) + (block >> 3);
+}
+
+__device__ __forceinline__ int run_height(int tiles, int rows) {
+  const int g = (int)sqrtf((float)(tiles >> 3));
+  return g < 1 ? 1 : g > rows ? rows : g;
+}
+
+// Strips of g tile rows, column by column.
+__device__ __forceinline__ void tile_of_grid(int b, int rows, int cols, int& ti, int& tj) {
+  const int g = run_height(rows * cols, rows), strip = b / (g * cols);
+  const int h = rows - strip * g < g ? rows - strip * g : g;  // of this strip
+  b -= strip * g * cols;
+  ti = strip * g + b % h;
+  tj = b / h;
+}
+
+// The same on the tiles with ti <= tj: a strip begins with a triangle.
+__device__ __forceinline__ void tile_of_triangle(int b, int rows, int& ti, int& tj) {
+  const int g = run_height(rows * (rows + 1) / 2, rows);
+  int top = 0, h = g;
+  for (;; top += g) {
+    h = rows - top < g ? rows - top : g;
+    const int count = h * (h + 1) / 2 + h * (rows - top - h);
+    if (b < count) break;
+    b -= count;
+  }
+  const int corner = h * (h + 1) / 2;
+  if (b >= corner) {
+    ti = top + (b - corner) % h;
+    tj = top + h + (b - corner) / h;
+  } else {
+    int c = 0;
+    while ((c + 1) * (c + 2) / 2 <= b) ++c;
+    ti = top + b - c * (c + 1) / 2;
+    tj = top + c;
+  }
+}
+
+// BK and S for a pair of plane counts.
+template <int BK_, int S_>
+struct Depth {
+  static constexpr int BK = BK_, S = S_;
+};
+
+template <class T, class D, int PA, int PB>
+constexpr int lds_halfs() {
+  return (PA * T::TM + PB * T::TN) * D::BK * D::S;
+}
+constexpr int most(int a, int b) { return a > b ? a : b; }
+
+// One tile of A, B, X' or the result.  D22, D11, D12: LDS depths for full
+// products, hi hi, and hi (hi + lo).
+template <class T, class D22, class D11, class D12, int TO>
+__global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, int turn, float ka,
+                                                                  float kb) {
+  constexpr bool SYM = TO == TO_A || TO == TO_B;
+  constexpr int HALFS = most(most(lds_halfs<T, D22, 2, 2>(), T::WAVES * kPieceHalfs),
+                             SYM ? lds_halfs<T, D11, 1, 1>() : lds_halfs<T, D12, 1, 2>());
+  __shared__ __align__(16) f16 lds[HALFS];
+  const int block = xcd_order(blockIdx.x, gridDim.x);
+  const Mat& t = tab.mat[find(tab, block)];
+  int ti, tj;
+  if (SYM)
+    tile_of_triangle(block - t.first, t.mp / T::TM, ti, tj);
+  else
+    tile_of_grid(block - t.first, t.mp / T::TM, t.np / T::TN, ti, tj);
+  const int i0 = ti * T::TM, j0 = tj * T::TN;
 
   const f16* P[2];
   const f16* Q[2];
-  int ld, K;
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
     if (TO == TO_A) {
-      P[p] = ws_x(t, p) + (size_t)i0 * t.np;
-      Q[p] = ws_x(t, p) + (size_t)j0 * t.np;
+      P[p] = ws_x(t, p) + (size_t)i0 * t.ldn;
+      Q[p] = ws_x(t, p) + (size_t)j0 * t.ldn;
     } else if (TO == TO_B) {
-      P[p] = ws_a(t, p) + (size_t)i0 * t.mp;
-      Q[p] = ws_a(t, p) + (size_t)j0 * t.mp;
+      P[p] = ws_a(t, p) + (size_t)i0 * t.ldm;
+      Q[p] = ws_a(t, p) + (size_t)j0 * t.ldm;
     } else {
-      P[p] = ws_b(t, p) + (size_t)i0 * t.mp;
-      Q[p] = ws_xt(t, turn, p) + (size_t)j0 * t.mp;
+      P[p] = ws_b(t, p) + (size_t)i0 * t.ldm;
+      Q[p] = ws_xt(t, turn, p) + (size_t)j0 * t.ldm;
     }
   }
-  ld = K = TO == TO_A ? t.np : t.mp;
+  const int K = TO == TO_A ? t.np : t.mp, ld = TO == TO_A ? t.ldn : t.ldm;
 
-  f32x16 acc[FM][FN];
+  f32x16 acc[T::FM][T::FN];
 #pragma unroll
-  for (int f = 0; f < FM; ++f)
+  for (int f = 0; f < T::FM; ++f)
 #pragma unroll
-    for (int g = 0; g < FN; ++g)
+    for (int g = 0; g < T::FN; ++g)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[f][g][r] = 0.f;
   if (t.full)
-    product<T, T, WM, WN, BK, 2, 2>(P, ld, Q, ld, K, lds, acc);
-  else if (TO == TO_A || TO == TO_B)
-    product<T, T, WM, WN, BK, 1, 1>(P, ld, Q, ld, K, lds, acc);
+    product<T, D22::BK, D22::S, 2, 2>(P, Q, ld, K, lds, acc);
+  else if (SYM)
+    product<T, D11::BK, D11::S, 1, 1>(P, Q, ld, K, lds, acc);
   else
-    product<T, T, WM, WN, BK, 1, 2>(P, ld, Q, ld, K, lds, acc);
+    product<T, D12::BK, D12::S, 1, 2>(P, Q, ld, K, lds, acc);
 
-  // a lane holds 4 neighbouring rows of a column, 4 times per 32 x 32 piece
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wi = i0 + (wave / WN) * (T / WM), wj = j0 + (wave % WN) * (T / WN);
+  const bool mirror = !SYM || ti != tj;
+  // a tile on the diagonal is its own mirror image: one writer for each value,
+  // since (i, j) and (j, i) may differ in the last bit
+  block_barrier();
+  float* piece = (float*)(lds + wave * kPieceHalfs);
+  const int wi = i0 + (wave / T::WN) * (T::TM / T::WM), wj = j0 + (wave % T::WN) * (T::TN / T::WN);
 #pragma unroll
-  for (int f = 0; f < FM; ++f)
+  for (int f = 0; f < T::FM; ++f)
 #pragma unroll
-    for (int g = 0; g < FN; ++g)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int i = wi + f * 32 + q * 8 + (lane >> 5) * 4;
-        const int j = wj + g * 32 + (lane & 31);
-        float v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = kb * acc[f][g][q * 4 + r];
-        if (TO != TO_A) {
-          // the old tile, from the copy in which its rows lie side by side
-          const size_t at = (size_t)j * t.mp + i;
-          const f16x4 h = *(const f16x4*)((TO == TO_B ? ws_a(t, 0) : ws_xt(t, turn, 0)) + at);
-          f16x4 l = {0, 0, 0, 0};
-          if (TO != TO_B || t.full)
-            l = *(const f16x4*)((TO == TO_B ? ws_a(t, 1) : ws_xt(t, turn, 1)) + at);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] += ka * ((float)h[r] + (float)l[r]);
-        }
-        if (TO == TO_END) {
-          const bool turned = t.rows > t.cols;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if (i + r < t.m && j < t.n) {
-              const size_t at = turned ? (size_t)j * t.cols + i + r : (size_t)(i + r) * t.cols + j;
-              float o = v[r];
-              if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
-              store_as(t.w, at, tab.wtype, o);
-            }
-          }
-          continue;
-        }
-        f16x4 h, l;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          f16 x, y;
-          split(v[r], x, y);
-          h[r] = x;
-          l[r] = y;
-        }
-        const size_t across = (size_t)j * t.mp + i;  // [j][i..i+3]
-        f16* ch = TO == TO_A ? ws_a(t, 0) : TO == TO_B ? ws_b(t, 0) : ws_xt(t, turn ^ 1, 0);
-        f16* cl = TO == TO_A ? ws_a(t, 1) : TO == TO_B ? ws_b(t, 1) : ws_xt(t, turn ^ 1, 1);
-        const bool low = TO == TO_X || t.full;
-        *(f16x4*)(ch + across) = h;
-        if (low) *(f16x4*)(cl + across) = l;
-        // a tile on the diagonal is its own mirror image: one writer for each
-        // value, since (i, j) and (j, i) may differ in the last bit
-        if (TO != TO_X && ti == tj) continue;
-        f16* sh = TO == TO_X ? ws_x(t, 0) : ch;
-        f16* sl = TO == TO_X ? ws_x(t, 1) : cl;
-        const int ldc = TO == TO_X ? t.np : t.mp;
-        const bool low_s = TO == TO_X ? (bool)t.full : low;  // X X^T takes hi alone
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          sh[(size_t)(i + r) * ldc + j] = h[r];
-          if (low_s) sl[(size_t)(i + r) * ldc + j] = l[r];
-        }
-      }
+    for (int g = 0; g < T::FN; ++g)
+      finish<TO>(tab, t, turn, ka, kb, wi + f * 32, wj + g * 32, mirror, acc[f][g], piece);
 }
 
 // ---- launch plan ----------------------------------------------------------------
@@ -418,44 +660,55 @@ int pad(int v, int t) { return (v + t - 1) / t * t; }
 
 // Tile side for a whole call: 128 where B X then has a tile for every CU.
 int tile_for(int count, const int* rows, const int* cols) {
+  if (const char* e = getenv("NS_TILE")) return atoi(e);  // TUNING
   long long tiles = 0;
   for (int k = 0; k < count; ++k)
     tiles += (long long)((rows[k] + 127) / 128) * ((cols[k] + 127) / 128);
   return tiles >= 256 ? 128 : 64;
 }
 
+// Rows lie an odd number of 128-byte lines apart: a step's pieces of 64 to 256
+// rows would all be in one channel of L2 if the distance were a power of two.
+int row_distance(int v) { return v + (v % 128 ? 0 : 64); }
+
 size_t bytes_of(int rows, int cols, int tile) {
   const size_t mp = pad(rows < cols ? rows : cols, tile), np = pad(rows < cols ? cols : rows, tile);
-  return kNormBlocks * sizeof(double) + (6 * mp * np + 4 * mp * mp) * sizeof(f16);
+  const size_t ldm = row_distance(mp), ldn = row_distance(np);
+  return kNormBlocks * sizeof(double) + (2 * mp * ldn + 4 * np * ldm + 4 * mp * ldm) * sizeof(f16);
 }
 
-template <int T, int WM, int WN, int BK>
+// (tile, depth for two planes, for hi hi, for hi (hi + lo))
+typedef Tile<64, 64, 2, 2> T64;
+typedef Tile<128, 128, 2, 2> T128;
+typedef Tile<256, 256, 2, 4> T256;
+
+template <class T, class D22, class D11, class D12>
 void products(Table& tab, int steps, const float* coef, float scale_b, hipStream_t st) {
   const float sa = kScaleA, sx = kScaleX, sb = scale_b;
   int sym = 0, all = 0, first_all[kMats];
   for (int k = 0; k < tab.count; ++k) {
     Mat& t = tab.mat[k];
-    const int mt = t.mp / T;
+    const int mt = t.mp / T::TM;
     t.first = sym;
     first_all[k] = all;
     sym += mt * (mt + 1) / 2;
-    all += mt * (t.np / T);
+    all += mt * (t.np / T::TN);
   }
   Table tall = tab;
   for (int k = 0; k < tab.count; ++k) tall.mat[k].first = first_all[k];
-  const dim3 block(WM * WN * 64);
+  const dim3 block(T::WAVES * 64);
+#define NS_LAUNCH(TO, GRID, TAB, TURN, KA, KB)                                                 \
+  hipLaunchKernelGGL((flowml_ns_product<T, D22, D11, D12, TO>), dim3(GRID), block, 0, st, TAB, \
+                     TURN, KA, KB)
   for (int s = 0; s < steps; ++s) {
-    hipLaunchKernelGGL((flowml_ns_product<T, WM, WN, BK, TO_A>), dim3(sym), block, 0, st, tab, 0,
-                       0.f, sa / (sx * sx));
-    hipLaunchKernelGGL((flowml_ns_product<T, WM, WN, BK, TO_B>), dim3(sym), block, 0, st, tab, 0,
-                       coef[1] * sb / sa, coef[2] * sb / (sa * sa));
+    NS_LAUNCH(TO_A, sym, tab, 0, 0.f, sa / (sx * sx));
+    NS_LAUNCH(TO_B, sym, tab, 0, coef[1] * sb / sa, coef[2] * sb / (sa * sa));
     if (s + 1 < steps)
-      hipLaunchKernelGGL((flowml_ns_product<T, WM, WN, BK, TO_X>), dim3(all), block, 0, st, tall,
-                         s & 1, coef[0], 1.f / sb);
+      NS_LAUNCH(TO_X, all, tall, s & 1, coef[0], 1.f / sb);
     else
-      hipLaunchKernelGGL((flowml_ns_product<T, WM, WN, BK, TO_END>), dim3(all), block, 0, st, tall,
-                         s & 1, coef[0] / sx, 1.f / (sb * sx));
+      NS_LAUNCH(TO_END, all, tall, s & 1, coef[0] / sx, 1.f / (sb * sx));
   }
+#undef NS_LAUNCH
 }
 
 }  // namespace
@@ -499,6 +752,8 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
       t.n = t.rows < t.cols ? t.cols : t.rows;
       t.mp = pad(t.m, tile);
       t.np = pad(t.n, tile);
+      t.ldm = row_distance(t.mp);
+      t.ldn = row_distance(t.np);
       t.part = (double*)at;
       t.ws = (f16*)(at + kNormBlocks * sizeof(double));
       at += bytes_of(t.rows, t.cols, tile);
@@ -520,9 +775,11 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
       tiles += (tab.mat[k].mp / 64) * (tab.mat[k].np / 64);
     }
     hipLaunchKernelGGL(flowml_ns_first, dim3(tiles), dim3(256), 0, st, tab, kPerNormBlock);
-    if (tile == 128)
-      products<128, 2, 2, 32>(tab, steps, coef, scale_b, st);
+    if (tile == 256)
+      products<T256, Depth<32, 2>, Depth<64, 2>, Depth<32, 3>>(tab, steps, coef, scale_b, st);
+    else if (tile == 128)
+      products<T128, Depth<32, 4>, Depth<64, 4>, Depth<32, 4>>(tab, steps, coef, scale_b, st);
     else
-      products<64, 2, 2, 64>(tab, steps, coef, scale_b, st);
+      products<T64, Depth<64, 4>, Depth<64, 4>, Depth<64, 4>>(tab, steps, coef, scale_b, st);
   }
 }
