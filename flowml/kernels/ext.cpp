@@ -529,8 +529,9 @@ static void muon_call(const std::vector<torch::Tensor>& g,
                     g[k].device() == g[0].device() &&
                     g[k].scalar_type() == g[0].scalar_type(),
                 "gradients: contiguous matrices of one type on one device");
-    TORCH_CHECK(g[k].size(0) < (1 << 24) && g[k].size(1) < (1 << 24),
-                "matrix too large");
+    // places in a working plane are 32-bit byte offsets
+    TORCH_CHECK((g[k].size(0) + 255) * (g[k].size(1) + 255) < (1LL << 30),
+                "matrix too large: 2^30 values at most");
     TORCH_CHECK(w[k].sizes() == g[k].sizes() && w[k].is_contiguous() &&
                     w[k].device() == g[0].device() &&
                     w[k].scalar_type() == w[0].scalar_type(),

@@ -38,7 +38,6 @@
 #include <math.h>
 #include <stdint.h>
 #include <type_traits>
-#include <stdlib.h>  // TUNING
 
 namespace {
 
@@ -50,7 +49,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
 
 constexpr int kMats = 24;        // matrices to a launch: the table is an argument
-constexpr int kNormBlocks = 64;  // most blocks that sum one matrix' squares
+constexpr int kNormBlocks = 1024;  // most blocks that sum one matrix' squares
 constexpr float kScaleX = 16384.f;  // |x| <= 1.9: within fp16
 constexpr float kScaleA = 16384.f;  // |x|^2 <= 3.7
 
@@ -61,13 +60,13 @@ struct Mat {
   float* mom;      // momentum buffer, or null
   void* w;         // weights, or the result
   int m, n;        // shorter and longer side
-  int mp, np;      // padded to whole tiles
-  int ldm, ldn;    // distance of working rows that run along m, along n
+  int mp, np;      // padded to whole tiles of B X
+  int ma;          // m padded to whole tiles of A as well
+  int parts;       // sums of squares
   int rows, cols;  // as the caller has it
   int full;        // 1: three products everywhere
   float step;
   int first;       // first block of this matrix in a launch
-  int blocks;      // and their number
 };
 
 struct Table {
@@ -80,9 +79,22 @@ struct Table {
 
 // ---- working planes ---------------------------------------------------------
 
-__host__ __device__ inline size_t plane_x(const Mat& t) { return (size_t)t.mp * t.ldn; }
-__host__ __device__ inline size_t plane_xt(const Mat& t) { return (size_t)t.np * t.ldm; }
-__host__ __device__ inline size_t plane_a(const Mat& t) { return (size_t)t.mp * t.ldm; }
+// A plane holds rows of K values in panels of 32: panel after panel, row after
+// row, 64 bytes each.  A tile's share of a panel is one piece of memory, so
+// copies to LDS and the writes of a 32 x 32 piece run over whole cache lines
+// (in plain rows a step takes 64 or 128 bytes here and there, at distances
+// that fall on few channels of L2 when K is a power of two).
+//
+// X has ma rows of np values (mp of them in use), its transpose np rows of mp,
+// A and B ma rows of ma.  Sums over m run to mp, so what lies behind it in A
+// and B meets nothing.
+__host__ __device__ inline size_t plane_x(const Mat& t) { return (size_t)t.ma * t.np; }
+__host__ __device__ inline size_t plane_xt(const Mat& t) { return (size_t)t.np * t.mp; }
+__host__ __device__ inline size_t plane_a(const Mat& t) { return (size_t)t.ma * t.ma; }
+// place of (row, k) in a plane of `rows` rows
+__device__ __forceinline__ size_t place(int rows, int row, int k) {
+  return ((size_t)(k >> 5) * rows + row) * 32 + (k & 31);
+}
 __device__ __forceinline__ f16* ws_x(const Mat& t, int p) { return t.ws + p * plane_x(t); }
 __device__ __forceinline__ f16* ws_xt(const Mat& t, int which, int p) {
   return t.ws + 2 * plane_x(t) + (2 * which + p) * plane_xt(t);
@@ -115,21 +127,99 @@ __device__ __forceinline__ void store_as(void* p, size_t i, int type, float v) {
     ((f16*)p)[i] = (f16)v;
 }
 
+// 8 values side by side, `left` of them within the matrix.
+__device__ __forceinline__ void load8(const void* p, size_t at, int type, int left, float* v) {
+  if (left >= 8) {
+    if (type == T_F32) {
+      typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+      const f32x4 x = *(const f32x4*)((const float*)p + at), y = *(const f32x4*)((const float*)p + at + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = x[k], v[4 + k] = y[k];
+    } else if (type == T_BF16) {
+      typedef __bf16 b8 __attribute__((ext_vector_type(8), aligned(2)));
+      const b8 x = *(const b8*)((const __bf16*)p + at);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
+    } else {
+      typedef f16 h8 __attribute__((ext_vector_type(8), aligned(2)));
+      const h8 x = *(const h8*)((const f16*)p + at);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = k < left ? load_as(p, at + k, type) : 0.f;
+  }
+}
+
+__device__ __forceinline__ void store8(void* p, size_t at, int type, int left, const float* v) {
+  if (left >= 8) {
+    if (type == T_F32) {
+      typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+      *(f32x4*)((float*)p + at) = f32x4{v[0], v[1], v[2], v[3]};
+      *(f32x4*)((float*)p + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    } else if (type == T_BF16) {
+      typedef __bf16 b8 __attribute__((ext_vector_type(8), aligned(2)));
+      b8 x;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = (__bf16)v[k];
+      *(b8*)((__bf16*)p + at) = x;
+    } else {
+      typedef f16 h8 __attribute__((ext_vector_type(8), aligned(2)));
+      h8 x;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = (f16)v[k];
+      *(h8*)((f16*)p + at) = x;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < left) store_as(p, at + k, type, v[k]);
+  }
+}
+
+__device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
+  hi = (f16)v;
+  lo = (f16)(v - (float)hi);
+}
+
+// U, what is orthogonalised, for 8 values: G, or G with its momentum.
+__device__ __forceinline__ void load_u(const Table& tab, const Mat& t, size_t at, int left, float* u) {
+  load8(t.g, at, tab.gtype, left, u);
+  if (t.mom) {
+    float m[8];
+    load8(t.mom, at, T_F32, left, m);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = tab.nesterov ? u[k] + tab.mu * m[k] : m[k];
+  }
+}
+
 // ---- sums of squares, and the momentum ---------------------------------------
 
+// In 64 bits: a long sum, and squares of values near the ends of fp32.
 __global__ __launch_bounds__(256) void flowml_ns_norm(Table tab) {
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   const int b = blockIdx.x - t.first;
-  const size_t total = (size_t)t.rows * t.cols;
+  const size_t total = (size_t)t.rows * t.cols, stride = (size_t)t.parts * 2048;
   double s = 0.0;
-  for (size_t i = (size_t)b * 256 + threadIdx.x; i < total; i += (size_t)t.blocks * 256) {
-    float u = load_as(t.g, i, tab.gtype);
+  for (size_t at = ((size_t)b * 256 + threadIdx.x) * 8; at < total; at += stride) {
+    const int left = total - at < 8 ? (int)(total - at) : 8;
+    float u[8];
     if (t.mom) {
-      const float v = tab.mu * t.mom[i] + u;
-      t.mom[i] = v;
-      u = tab.nesterov ? u + tab.mu * v : v;
+      float g[8], m[8];
+      load8(t.g, at, tab.gtype, left, g);
+      load8(t.mom, at, T_F32, left, m);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        m[k] = tab.mu * m[k] + g[k];
+        u[k] = tab.nesterov ? g[k] + tab.mu * m[k] : m[k];
+      }
+      store8(t.mom, at, T_F32, left, m);
+    } else {
+      load8(t.g, at, tab.gtype, left, u);
     }
-    s += (double)u * (double)u;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += (double)u[k] * (double)u[k];
   }
   __shared__ double red[4];
   for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
@@ -140,53 +230,65 @@ __global__ __launch_bounds__(256) void flowml_ns_norm(Table tab) {
 
 // ---- the first iterate: 64 x 64 tiles of the caller's matrix -------------------
 
-__global__ __launch_bounds__(256) void flowml_ns_first(Table tab, int norm_blocks_of_one) {
+__global__ __launch_bounds__(256) void flowml_ns_first(Table tab) {
+  __shared__ double red[4];
+  __shared__ uint32_t tile[64][65];
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
-  const int b = blockIdx.x - t.first;
+  const int b = blockIdx.x - t.first, tid = threadIdx.x;
   const bool turned = t.rows > t.cols;  // the caller's rows run along n
-  const int pcol = turned ? t.mp : t.np;
-  const int ld_straight = turned ? t.ldm : t.ldn, ld_turned = turned ? t.ldn : t.ldm;
-  const int r0 = (b / (pcol / 64)) * 64, c0 = (b % (pcol / 64)) * 64;
+  const int rows_straight = turned ? t.np : t.ma, rows_turned = turned ? t.ma : t.np;
+  const int across = (turned ? t.mp : t.np) / 64;
+  const int r0 = b / across * 64, c0 = b % across * 64;
 
   // |G|: every block adds the same partial sums in the same order
-  const size_t total = (size_t)t.rows * t.cols;
-  int parts = (int)((total + norm_blocks_of_one - 1) / norm_blocks_of_one);
-  if (parts > kNormBlocks) parts = kNormBlocks;
   double s = 0.0;
-  for (int k = 0; k < parts; ++k) s += t.part[k];
-  const double norm = sqrt(s);
+  for (int k = tid; k < t.parts; k += 256) s += t.part[k];
+  for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
+  if ((tid & 63) == 0) red[tid >> 6] = s;
+  __syncthreads();
+  const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
   const float scale = norm <= (double)tab.eps ? (float)(kScaleX / (double)tab.eps)
                                               : (float)(kScaleX / norm);  // NaN stays
-
-  __shared__ uint32_t tile[64][65];
+  // hi hi alone takes X X^T from the higher halves
   f16* straight[2];
-  f16* turned_p[2];
+  f16* other[2];
   for (int p = 0; p < 2; ++p) {
     straight[p] = turned ? ws_xt(t, 0, p) : ws_x(t, p);
-    turned_p[p] = turned ? ws_x(t, p) : ws_xt(t, 0, p);
+    other[p] = turned ? ws_x(t, p) : ws_xt(t, 0, p);
   }
-  const int tc = threadIdx.x & 63, tr = threadIdx.x >> 6;
-  for (int i = tr; i < 64; i += 4) {
-    const int r = r0 + i, c = c0 + tc;
-    float u = 0.f;
-    if (r < t.rows && c < t.cols) {
-      const size_t at = (size_t)r * t.cols + c;
-      u = load_as(t.g, at, tab.gtype);
-      if (t.mom) u = tab.nesterov ? u + tab.mu * t.mom[at] : t.mom[at];
-      u *= scale;
+  const int r8 = tid >> 3, c8 = (tid & 7) * 8;
+#pragma unroll
+  for (int h = 0; h < 64; h += 32) {
+    const int r = r0 + r8 + h, c = c0 + c8;
+    float u[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < t.rows && c < t.cols) load_u(tab, t, (size_t)r * t.cols + c, t.cols - c, u);
+    f16x8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      f16 x, y;
+      split(u[k] * scale, x, y);
+      hi[k] = x;
+      lo[k] = y;
+      tile[r8 + h][c8 + k] = (uint32_t)__builtin_bit_cast(uint16_t, x) |
+                             ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
     }
-    const f16 hi = (f16)u, lo = (f16)(u - (float)hi);
-    straight[0][(size_t)r * ld_straight + c] = hi;
-    straight[1][(size_t)r * ld_straight + c] = lo;
-    tile[i][tc] = (uint32_t)__builtin_bit_cast(uint16_t, hi) |
-                  ((uint32_t)__builtin_bit_cast(uint16_t, lo) << 16);
+    const size_t at = place(rows_straight, r, c);
+    *(f16x8*)(straight[0] + at) = hi;
+    if (turned || t.full) *(f16x8*)(straight[1] + at) = lo;
   }
   __syncthreads();
-  for (int i = tr; i < 64; i += 4) {
-    const uint32_t v = tile[tc][i];
-    const size_t at = (size_t)(c0 + i) * ld_turned + r0 + tc;
-    turned_p[0][at] = __builtin_bit_cast(f16, (uint16_t)(v & 0xffff));
-    turned_p[1][at] = __builtin_bit_cast(f16, (uint16_t)(v >> 16));
+#pragma unroll
+  for (int h = 0; h < 64; h += 32) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t v = tile[c8 + k][r8 + h];
+      hi[k] = __builtin_bit_cast(f16, (uint16_t)(v & 0xffff));
+      lo[k] = __builtin_bit_cast(f16, (uint16_t)(v >> 16));
+    }
+    const size_t at = place(rows_turned, c0 + r8 + h, r0 + c8);
+    *(f16x8*)(other[0] + at) = hi;
+    if (!turned || t.full) *(f16x8*)(other[1] + at) = lo;
   }
 }
 
@@ -201,22 +303,11 @@ struct Tile {
   static constexpr int FM = TM / WM / 32, FN = TN / WN / 32;
 };
 
-template <int BK>
-__device__ __forceinline__ int swizzle(int chunk, int row) {
-  // 16 neighbouring rows' pieces of one chunk fall on all 64 banks
-  return BK == 64 ? (chunk ^ ((row >> 1) & 7)) : (chunk ^ ((row >> 2) & 3));
-}
+// Where in its 64 bytes of LDS a row keeps a 16-byte chunk: those of 16
+// neighbouring rows fall on all 64 banks.
+__device__ __forceinline__ int swizzle(int chunk, int row) { return chunk ^ ((row >> 2) & 3); }
 
 typedef __attribute__((address_space(3))) void lds_void;
-
-// Where a lane's 16 bytes of 1 KB, piece `piece` of a plane of rows of BK
-// values, come from.  They land in LDS at 16 * lane, so the swizzle is here.
-template <int BK>
-__device__ __forceinline__ int source_of(int ld, int piece, int lane) {
-  constexpr int CH = BK / 8;
-  const int slot = piece * 64 + lane, row = slot / CH;
-  return row * ld * 2 + swizzle<BK>(slot % CH, row) * 16;
-}
 
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -238,8 +329,8 @@ __device__ __forceinline__ void block_barrier() {
 // accept them (64 x 64 tiles: 1040 cycles a step, 400 of them multiplying).
 // The scheduling barriers keep the compiler from gathering them again.
 template <class T, int BK, int S, int PA, int PB>
-__device__ __forceinline__ void product(const f16* const (&P)[2], const f16* const (&Q)[2], int ld,
-                                        int K, f16* lds, f32x16 (&acc)[T::FM][T::FN]) {
+__device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, const f16* const (&Q)[2],
+                                        int rows_q, int K, f16* lds, f32x16 (&acc)[T::FM][T::FN]) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know buffer resources
   constexpr int STAGE = (PA * T::TM + PB * T::TN) * BK;
   constexpr int LA = T::TM * BK / 512 / T::WAVES, LB = T::TN * BK / 512 / T::WAVES;
@@ -250,35 +341,36 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], const f16* con
   // step's end, and leave early
   constexpr int SPREAD = S == 2 ? (UNITS + 3) / 4 : UNITS;
   static_assert(KG % 2 == 0, "fragments alternate between two sets");
-  static_assert(T::TM * BK % (512 * T::WAVES) == 0 && T::TN * BK % (512 * T::WAVES) == 0,
-                "every wave copies as much");
+  static_assert(T::TM * 32 % (512 * T::WAVES) == 0 && T::TN * 32 % (512 * T::WAVES) == 0,
+                "every wave copies as much of a panel");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = (wave / T::WN) * (T::TM / T::WM), wn = (wave % T::WN) * (T::TN / T::WN);
 
-  // buffer loads: the lane's part of an address stays, the step's is a scalar
+  // 1 KB, 16 rows of a panel, to a copy.  A lane's 16 bytes land at 16 * lane,
+  // so the swizzle is in the place they come from; the rest of it is scalar.
   __amdgpu_buffer_rsrc_t rp[PA], rq[PB];
 #pragma unroll
   for (int p = 0; p < PA; ++p)
-    rp[p] = __builtin_amdgcn_make_buffer_rsrc((void*)P[p], 0, T::TM * ld * 2, 0x00020000);
+    rp[p] = __builtin_amdgcn_make_buffer_rsrc((void*)P[p], 0, -1, 0x00020000);
 #pragma unroll
   for (int p = 0; p < PB; ++p)
-    rq[p] = __builtin_amdgcn_make_buffer_rsrc((void*)Q[p], 0, T::TN * ld * 2, 0x00020000);
-  int from_p[LA], from_q[LB];
-#pragma unroll
-  for (int i = 0; i < LA; ++i) from_p[i] = source_of<BK>(ld, wave * LA + i, lane);
-#pragma unroll
-  for (int i = 0; i < LB; ++i) from_q[i] = source_of<BK>(ld, wave * LB + i, lane);
+    rq[p] = __builtin_amdgcn_make_buffer_rsrc((void*)Q[p], 0, -1, 0x00020000);
+  const int from = (lane >> 2) * 64 + swizzle(lane & 3, lane >> 2) * 16;
   auto copy = [&](int k0, f16* s, int which) {
     const bool first = which < PA * LA;
     const int w = first ? which : which - PA * LA, l = first ? LA : LB;
-    const int p = w / l, i = w % l;
-    f16* to = s + (first ? p * T::TM : PA * T::TM + p * T::TN) * BK + (wave * l + i) * 512;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(first ? rp[p] : rq[p], (lds_void*)to, 16,
-                                             first ? from_p[i] : from_q[i], k0 * 2, 0, 0);
+    const int p = w / l, i = w % l, panel = i / (l / (BK / 32)), j = i % (l / (BK / 32));
+    const int rows = first ? T::TM : T::TN, piece = wave * (l / (BK / 32)) + j;
+    f16* to = s + (first ? p * T::TM : PA * T::TM + p * T::TN) * BK + panel * rows * 32 + piece * 512;
+    const int panels = (k0 >> 5) + panel;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        first ? rp[p] : rq[p], (lds_void*)to, 16, from,
+        panels * (first ? rows_p : rows_q) * 64 + piece * 1024, 0, 0);
   };
-  auto read = [&](const f16* plane, int row, int kk) {
-    return *(const f16x8*)(plane + row * BK + swizzle<BK>(kk * 2 + (lane >> 5), row) * 8);
+  auto read = [&](const f16* plane, int rows, int row, int kk) {
+    return *(const f16x8*)(plane + (kk >> 1) * rows * 32 + row * 32 +
+                           swizzle((kk & 1) * 2 + (lane >> 5), row) * 8);
   };
   f16x8 a[2][KU][PA], b[2][KU][PB][T::FN];
   // Reads and multiplications of a unit, in the order in which the fragments
@@ -290,10 +382,10 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], const f16* con
     const int pb = PB == 2 && (PA == 2) == late ? 1 : 0;
     if (j == 0 || (PA == 2 && j == (f == 0 ? T::FN + 1 : 1))) {
       const int p = j == 0 ? PA - 1 : 0;
-      a[u & 1][k][p] = read(s + p * T::TM * BK, wm + f * 32 + (lane & 31), kg * KU + k);
+      a[u & 1][k][p] = read(s + p * T::TM * BK, T::TM, wm + f * 32 + (lane & 31), kg * KU + k);
     } else {
       const int g = late ? j - T::FN - PA : j - 1;
-      b[kg & 1][k][pb][g] = read(s + (PA * T::TM + pb * T::TN) * BK,
+      b[kg & 1][k][pb][g] = read(s + (PA * T::TM + pb * T::TN) * BK, T::TN,
                                  wn + g * 32 + (lane & 31), kg * KU + k);
     }
   };
@@ -365,62 +457,6 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], const f16* con
 #endif
 }
 
-__device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
-  hi = (f16)v;
-  lo = (f16)(v - (float)hi);
-}
-
-// 8 values side by side, `left` of them within the matrix.
-__device__ __forceinline__ void load8(const void* p, size_t at, int type, int left, float* v) {
-  if (left >= 8) {
-    if (type == T_F32) {
-      typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-      const f32x4 x = *(const f32x4*)((const float*)p + at), y = *(const f32x4*)((const float*)p + at + 4);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = x[k], v[4 + k] = y[k];
-    } else if (type == T_BF16) {
-      typedef __bf16 b8 __attribute__((ext_vector_type(8), aligned(2)));
-      const b8 x = *(const b8*)((const __bf16*)p + at);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
-    } else {
-      typedef f16 h8 __attribute__((ext_vector_type(8), aligned(2)));
-      const h8 x = *(const h8*)((const f16*)p + at);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] = (float)x[k];
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = k < left ? load_as(p, at + k, type) : 0.f;
-  }
-}
-
-__device__ __forceinline__ void store8(void* p, size_t at, int type, int left, const float* v) {
-  if (left >= 8) {
-    if (type == T_F32) {
-      typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
-      *(f32x4*)((float*)p + at) = f32x4{v[0], v[1], v[2], v[3]};
-      *(f32x4*)((float*)p + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
-    } else if (type == T_BF16) {
-      typedef __bf16 b8 __attribute__((ext_vector_type(8), aligned(2)));
-      b8 x;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = (__bf16)v[k];
-      *(b8*)((__bf16*)p + at) = x;
-    } else {
-      typedef f16 h8 __attribute__((ext_vector_type(8), aligned(2)));
-      h8 x;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = (f16)v[k];
-      *(h8*)((f16*)p + at) = x;
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < left) store_as(p, at + k, type, v[k]);
-  }
-}
-
 // The result, or the weights' update, for 8 values of one row of the caller's.
 __device__ __forceinline__ void deliver(const Table& tab, const Mat& t, int row, int col, float* v) {
   if (row >= t.rows || col >= t.cols) return;
@@ -440,7 +476,7 @@ constexpr int kPieceHalfs = 32 * kPieceLd * 2;
 // The 32 x 32 piece at (i0, j0) of A, B, X' or the result: ka * (old value) +
 // kb * (product).  A lane holds 4 neighbouring rows of a column, 4 times; the
 // piece goes through the wave's own LDS so that every global access is 16
-// bytes per lane, 64 bytes in a row.  (Written from the registers, 2 and 8
+// bytes per lane, side by side.  (Written from the registers, 2 and 8
 // bytes per lane, the tiles' ends took 8 us of 31 at 128 x 128 and 100 us of
 // 360 at 256 x 256.)
 template <int TO>
@@ -451,12 +487,13 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
   f16* ch = TO == TO_A ? ws_a(t, 0) : TO == TO_B ? ws_b(t, 0) : ws_xt(t, turn ^ 1, 0);
   f16* cl = TO == TO_A ? ws_a(t, 1) : TO == TO_B ? ws_b(t, 1) : ws_xt(t, turn ^ 1, 1);
   const int r4 = lane >> 2, c8 = (lane & 3) * 8;
+  const int rows_j = TO == TO_A || TO == TO_B ? t.ma : t.np;  // of a plane whose rows are columns j
   // the old values, from the copy in which i runs along rows
   f16x8 oh[2], ol[2];
   if (TO != TO_A) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const size_t at = (size_t)(j0 + h * 16 + r4) * t.ldm + i0 + c8;
+      const size_t at = place(rows_j, j0 + h * 16 + r4, i0 + c8);
       oh[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 0) : ws_xt(t, turn, 0)) + at);
       ol[h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
       if (TO != TO_B || t.full)
@@ -498,7 +535,7 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
       both[k] = (uint32_t)__builtin_bit_cast(uint16_t, a) |
                 ((uint32_t)__builtin_bit_cast(uint16_t, b) << 16);
     }
-    const size_t at = (size_t)(j0 + j) * t.ldm + i0 + c8;
+    const size_t at = place(rows_j, j0 + j, i0 + c8);
     *(f16x8*)(ch + at) = hi;
     if (TO == TO_X || t.full) *(f16x8*)(cl + at) = lo;
     *(uint4*)p = make_uint4(both[0], both[1], both[2], both[3]);
@@ -508,7 +545,6 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   f16* sh = TO == TO_X ? ws_x(t, 0) : ch;
   f16* sl = TO == TO_X ? ws_x(t, 1) : cl;
-  const int ldc = TO == TO_X ? t.ldn : t.ldm;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = h * 16 + r4;
@@ -526,7 +562,7 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
       hi[k] = __builtin_bit_cast(f16, (uint16_t)(u & 0xffff));
       lo[k] = __builtin_bit_cast(f16, (uint16_t)(u >> 16));
     }
-    const size_t at = (size_t)(i0 + i) * ldc + j0 + c8;
+    const size_t at = place(t.ma, i0 + i, j0 + c8);
     *(f16x8*)(sh + at) = hi;
     if (t.full) *(f16x8*)(sl + at) = lo;
   }
@@ -602,7 +638,7 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   const Mat& t = tab.mat[find(tab, block)];
   int ti, tj;
   if (SYM)
-    tile_of_triangle(block - t.first, t.mp / T::TM, ti, tj);
+    tile_of_triangle(block - t.first, t.ma / T::TM, ti, tj);
   else
     tile_of_grid(block - t.first, t.mp / T::TM, t.np / T::TN, ti, tj);
   const int i0 = ti * T::TM, j0 = tj * T::TN;
@@ -611,18 +647,10 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   const f16* Q[2];
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    if (TO == TO_A) {
-      P[p] = ws_x(t, p) + (size_t)i0 * t.ldn;
-      Q[p] = ws_x(t, p) + (size_t)j0 * t.ldn;
-    } else if (TO == TO_B) {
-      P[p] = ws_a(t, p) + (size_t)i0 * t.ldm;
-      Q[p] = ws_a(t, p) + (size_t)j0 * t.ldm;
-    } else {
-      P[p] = ws_b(t, p) + (size_t)i0 * t.ldm;
-      Q[p] = ws_xt(t, turn, p) + (size_t)j0 * t.ldm;
-    }
+    P[p] = (TO == TO_A ? ws_x(t, p) : TO == TO_B ? ws_a(t, p) : ws_b(t, p)) + i0 * 32;
+    Q[p] = (TO == TO_A ? ws_x(t, p) : TO == TO_B ? ws_a(t, p) : ws_xt(t, turn, p)) + j0 * 32;
   }
-  const int K = TO == TO_A ? t.np : t.mp, ld = TO == TO_A ? t.ldn : t.ldm;
+  const int K = TO == TO_A ? t.np : t.mp, rows_q = SYM ? t.ma : t.np;
 
   f32x16 acc[T::FM][T::FN];
 #pragma unroll
@@ -632,11 +660,11 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[f][g][r] = 0.f;
   if (t.full)
-    product<T, D22::BK, D22::S, 2, 2>(P, Q, ld, K, lds, acc);
+    product<T, D22::BK, D22::S, 2, 2>(P, t.ma, Q, rows_q, K, lds, acc);
   else if (SYM)
-    product<T, D11::BK, D11::S, 1, 1>(P, Q, ld, K, lds, acc);
+    product<T, D11::BK, D11::S, 1, 1>(P, t.ma, Q, rows_q, K, lds, acc);
   else
-    product<T, D12::BK, D12::S, 1, 2>(P, Q, ld, K, lds, acc);
+    product<T, D12::BK, D12::S, 1, 2>(P, t.ma, Q, rows_q, K, lds, acc);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool mirror = !SYM || ti != tj;
@@ -654,61 +682,81 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
 
 // ---- launch plan ----------------------------------------------------------------
 
-constexpr int kPerNormBlock = 16384;
+constexpr int kPerNormBlock = 8192;
 
 int pad(int v, int t) { return (v + t - 1) / t * t; }
 
-// Tile side for a whole call: 128 where B X then has a tile for every CU.
-int tile_for(int count, const int* rows, const int* cols) {
-  if (const char* e = getenv("NS_TILE")) return atoi(e);  // TUNING
-  long long tiles = 0;
-  for (int k = 0; k < count; ++k)
-    tiles += (long long)((rows[k] + 127) / 128) * ((cols[k] + 127) / 128);
-  return tiles >= 256 ? 128 : 64;
+// Tile sides of a call's symmetric products (A and B) and of B X.  A tile of
+// 256 runs at 1300 TFLOP/s and one of 64 at 650, but tiles are worth their
+// size only if there are enough for the 256 CUs.  Measured, us a product:
+//   A of 1024 x 4096 x 2, full:  64 (272 tiles) 27      128 (72 tiles) 56
+//   A of 2048 x 4096, hi hi:     64 (528) 38   128 (136) 30   256 (36) 78
+//   A of 4096 x 4096, hi hi:     128 (528) 91  192 (253) 74   256 (136) 94
+//   B X of 1024 x 4096, full:    64 (1024) 36  128 (256) 29   256 (64) 62
+//   B X of 4096 x 4096:          128 (1024) 266               256 (256) 230
+struct Sides {
+  int sym, all;
+};
+
+Sides sides_for(int count, const int* rows, const int* cols) {
+  auto tiles = [&](int t, bool sym) {
+    long long sum = 0;
+    for (int k = 0; k < count; ++k) {
+      const long long a = ((rows[k] < cols[k] ? rows[k] : cols[k]) + t - 1) / t;
+      const long long b = ((rows[k] < cols[k] ? cols[k] : rows[k]) + t - 1) / t;
+      sum += sym ? a * (a + 1) / 2 : a * b;
+    }
+    return sum;
+  };
+  Sides s;
+  s.all = tiles(256, false) >= 200 ? 256 : tiles(128, false) >= 128 ? 128 : 64;
+  s.sym = tiles(256, true) >= 400   ? 256
+          : tiles(192, true) >= 200 ? 192
+          : tiles(128, true) >= 128 ? 128
+                                    : 64;
+  return s;
 }
 
-// Rows lie an odd number of 128-byte lines apart: a step's pieces of 64 to 256
-// rows would all be in one channel of L2 if the distance were a power of two.
-int row_distance(int v) { return v + (v % 128 ? 0 : 64); }
-
-size_t bytes_of(int rows, int cols, int tile) {
-  const size_t mp = pad(rows < cols ? rows : cols, tile), np = pad(rows < cols ? cols : rows, tile);
-  const size_t ldm = row_distance(mp), ldn = row_distance(np);
-  return kNormBlocks * sizeof(double) + (2 * mp * ldn + 4 * np * ldm + 4 * mp * ldm) * sizeof(f16);
+size_t bytes_of(int rows, int cols, Sides s) {
+  const size_t mp = pad(rows < cols ? rows : cols, s.all), np = pad(rows < cols ? cols : rows, s.all);
+  const size_t ma = pad(mp, s.sym);
+  return kNormBlocks * sizeof(double) + (2 * ma * np + 4 * np * mp + 4 * ma * ma) * sizeof(f16);
 }
 
-// (tile, depth for two planes, for hi hi, for hi (hi + lo))
-typedef Tile<64, 64, 2, 2> T64;
-typedef Tile<128, 128, 2, 2> T128;
-typedef Tile<256, 256, 2, 4> T256;
-
-template <class T, class D22, class D11, class D12>
-void products(Table& tab, int steps, const float* coef, float scale_b, hipStream_t st) {
-  const float sa = kScaleA, sx = kScaleX, sb = scale_b;
-  int sym = 0, all = 0, first_all[kMats];
+// one product for all matrices of a table; `first` of each is set here
+template <class T, class D22, class D11, class D12, int TO>
+void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
+  int blocks = 0;
   for (int k = 0; k < tab.count; ++k) {
     Mat& t = tab.mat[k];
-    const int mt = t.mp / T::TM;
-    t.first = sym;
-    first_all[k] = all;
-    sym += mt * (mt + 1) / 2;
-    all += mt * (t.np / T::TN);
+    t.first = blocks;
+    const int mt = t.ma / T::TM;
+    blocks += TO == TO_A || TO == TO_B ? mt * (mt + 1) / 2 : (t.mp / T::TM) * (t.np / T::TN);
   }
-  Table tall = tab;
-  for (int k = 0; k < tab.count; ++k) tall.mat[k].first = first_all[k];
-  const dim3 block(T::WAVES * 64);
-#define NS_LAUNCH(TO, GRID, TAB, TURN, KA, KB)                                                 \
-  hipLaunchKernelGGL((flowml_ns_product<T, D22, D11, D12, TO>), dim3(GRID), block, 0, st, TAB, \
-                     TURN, KA, KB)
-  for (int s = 0; s < steps; ++s) {
-    NS_LAUNCH(TO_A, sym, tab, 0, 0.f, sa / (sx * sx));
-    NS_LAUNCH(TO_B, sym, tab, 0, coef[1] * sb / sa, coef[2] * sb / (sa * sa));
-    if (s + 1 < steps)
-      NS_LAUNCH(TO_X, all, tall, s & 1, coef[0], 1.f / sb);
+  hipLaunchKernelGGL((flowml_ns_product<T, D22, D11, D12, TO>), dim3(blocks), dim3(T::WAVES * 64),
+                     0, st, tab, turn, ka, kb);
+}
+
+template <int TO>
+void product(Sides s, Table& tab, int turn, float ka, float kb, hipStream_t st) {
+  // tile, waves, and the depth of LDS for two planes, hi hi, hi (hi + lo)
+  if constexpr (TO == TO_A || TO == TO_B) {
+    if (s.sym == 256)
+      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+    else if (s.sym == 192)
+      product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+    else if (s.sym == 128)
+      product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
     else
-      NS_LAUNCH(TO_END, all, tall, s & 1, coef[0] / sx, 1.f / (sb * sx));
+      product_of<Tile<64, 64, 2, 2>, Depth<64, 4>, Depth<64, 4>, Depth<64, 2>, TO>(tab, turn, ka, kb, st);
+  } else {
+    if (s.all == 256)
+      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+    else if (s.all == 128)
+      product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+    else
+      product_of<Tile<64, 64, 2, 2>, Depth<64, 4>, Depth<64, 2>, Depth<64, 4>, TO>(tab, turn, ka, kb, st);
   }
-#undef NS_LAUNCH
 }
 
 }  // namespace
@@ -717,9 +765,9 @@ void products(Table& tab, int steps, const float* coef, float scale_b, hipStream
 
 // workspace of a call, in bytes
 extern "C" long long muon_workspace(int count, const int* rows, const int* cols) {
-  const int tile = tile_for(count, rows, cols);
+  const Sides s = sides_for(count, rows, cols);
   size_t sum = 0;
-  for (int k = 0; k < count; ++k) sum += bytes_of(rows[k], cols[k], tile);
+  for (int k = 0; k < count; ++k) sum += bytes_of(rows[k], cols[k], s);
   return (long long)sum;
 }
 
@@ -732,7 +780,8 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
                             int wtype, float mu, float keep, float eps, int nesterov, int steps,
                             const float* coef, float scale_b, int full, void* ws, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const int tile = tile_for(count, rows, cols);
+  const Sides sides = sides_for(count, rows, cols);
+  const float sa = kScaleA, sx = kScaleX, sb = scale_b;
   char* at = (char*)ws;
   for (int k0 = 0; k0 < count; k0 += kMats) {
     Table tab;
@@ -743,43 +792,43 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
     tab.keep = keep;
     tab.eps = eps;
     tab.nesterov = nesterov;
-    int norm_blocks = 0;
+    int blocks = 0;
     for (int k = 0; k < tab.count; ++k) {
       Mat& t = tab.mat[k];
       t.rows = rows[k0 + k];
       t.cols = cols[k0 + k];
       t.m = t.rows < t.cols ? t.rows : t.cols;
       t.n = t.rows < t.cols ? t.cols : t.rows;
-      t.mp = pad(t.m, tile);
-      t.np = pad(t.n, tile);
-      t.ldm = row_distance(t.mp);
-      t.ldn = row_distance(t.np);
+      t.mp = pad(t.m, sides.all);
+      t.np = pad(t.n, sides.all);
+      t.ma = pad(t.mp, sides.sym);
       t.part = (double*)at;
       t.ws = (f16*)(at + kNormBlocks * sizeof(double));
-      at += bytes_of(t.rows, t.cols, tile);
+      at += bytes_of(t.rows, t.cols, sides);
       t.g = g[k0 + k];
       t.mom = mom ? mom[k0 + k] : nullptr;
       t.w = w[k0 + k];
       t.step = step ? step[k0 + k] : 0.f;
       t.full = full || t.m < 256;
-      const size_t total = (size_t)t.rows * t.cols;
-      const size_t want = (total + kPerNormBlock - 1) / kPerNormBlock;
-      t.first = norm_blocks;
-      t.blocks = (int)(want < kNormBlocks ? want : kNormBlocks);
-      norm_blocks += t.blocks;
+      const size_t want = ((size_t)t.rows * t.cols + kPerNormBlock - 1) / kPerNormBlock;
+      t.parts = (int)(want < kNormBlocks ? want : kNormBlocks);
+      t.first = blocks;
+      blocks += t.parts;
     }
-    hipLaunchKernelGGL(flowml_ns_norm, dim3(norm_blocks), dim3(256), 0, st, tab);
-    int tiles = 0;
+    hipLaunchKernelGGL(flowml_ns_norm, dim3(blocks), dim3(256), 0, st, tab);
+    blocks = 0;
     for (int k = 0; k < tab.count; ++k) {
-      tab.mat[k].first = tiles;
-      tiles += (tab.mat[k].mp / 64) * (tab.mat[k].np / 64);
+      tab.mat[k].first = blocks;
+      blocks += (tab.mat[k].mp / 64) * (tab.mat[k].np / 64);
     }
-    hipLaunchKernelGGL(flowml_ns_first, dim3(tiles), dim3(256), 0, st, tab, kPerNormBlock);
-    if (tile == 256)
-      products<T256, Depth<32, 2>, Depth<64, 2>, Depth<32, 3>>(tab, steps, coef, scale_b, st);
-    else if (tile == 128)
-      products<T128, Depth<32, 4>, Depth<64, 4>, Depth<32, 4>>(tab, steps, coef, scale_b, st);
-    else
-      products<T64, Depth<64, 4>, Depth<64, 4>, Depth<64, 4>>(tab, steps, coef, scale_b, st);
+    hipLaunchKernelGGL(flowml_ns_first, dim3(blocks), dim3(256), 0, st, tab);
+    for (int s = 0; s < steps; ++s) {
+      product<TO_A>(sides, tab, 0, 0.f, sa / (sx * sx), st);
+      product<TO_B>(sides, tab, 0, coef[1] * sb / sa, coef[2] * sb / (sa * sa), st);
+      if (s + 1 < steps)
+        product<TO_X>(sides, tab, s & 1, coef[0], 1.f / sb, st);
+      else
+        product<TO_END>(sides, tab, s & 1, coef[0] / sx, 1.f / (sb * sx), st);
+    }
   }
 }
