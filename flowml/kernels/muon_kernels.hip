@@ -178,7 +178,11 @@ __device__ __forceinline__ void store8(void* p, size_t at, int type, int left, c
   }
 }
 
+// The empty statement makes v a number of fp32: without it the compiler may
+// round the product that v comes from straight to fp16 for one use of hi and by
+// way of fp32 for the other, and a tie between them costs lo its meaning.
 __device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
+  asm volatile("" : "+v"(v));
   hi = (f16)v;
   lo = (f16)(v - (float)hi);
 }
@@ -335,8 +339,7 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
   constexpr int STAGE = (PA * T::TM + PB * T::TN) * BK;
   constexpr int LA = T::TM * BK / 512 / T::WAVES, LB = T::TN * BK / 512 / T::WAVES;
   constexpr int LOADS = PA * LA + PB * LB;  // copies per wave and stage
-  constexpr int KU = T::FM == 1 ? 2 : 1;    // slices of K to a unit
-  constexpr int KG = BK / 16 / KU, UNITS = KG * T::FM;
+  constexpr int KG = BK / 16, UNITS = KG * T::FM;
   // units that send copies: with two stages these are waited for at this
   // step's end, and leave early
   constexpr int SPREAD = S == 2 ? (UNITS + 3) / 4 : UNITS;
@@ -372,30 +375,29 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
     return *(const f16x8*)(plane + (kk >> 1) * rows * 32 + row * 32 +
                            swizzle((kk & 1) * 2 + (lane >> 5), row) * 8);
   };
-  f16x8 a[2][KU][PA], b[2][KU][PB][T::FN];
+  f16x8 a[2][PA], b[2][PB][T::FN];
   // Reads and multiplications of a unit, in the order in which the fragments
   // are needed: lo hi, hi lo, hi hi.
   auto read_one = [&](const f16* s, int u, int which) {
     const int kg = u / T::FM, f = u % T::FM;
-    const int per = PA + (f == 0 ? PB * T::FN : 0), k = which / per, j = which % per;
-    const bool late = j > T::FN && f == 0;  // the planes of the second product
+    const bool late = which > T::FN && f == 0;  // the planes of the second product
     const int pb = PB == 2 && (PA == 2) == late ? 1 : 0;
-    if (j == 0 || (PA == 2 && j == (f == 0 ? T::FN + 1 : 1))) {
-      const int p = j == 0 ? PA - 1 : 0;
-      a[u & 1][k][p] = read(s + p * T::TM * BK, T::TM, wm + f * 32 + (lane & 31), kg * KU + k);
+    if (which == 0 || (PA == 2 && which == (f == 0 ? T::FN + 1 : 1))) {
+      const int p = which == 0 ? PA - 1 : 0;
+      a[u & 1][p] = read(s + p * T::TM * BK, T::TM, wm + f * 32 + (lane & 31), kg);
     } else {
-      const int g = late ? j - T::FN - PA : j - 1;
-      b[kg & 1][k][pb][g] = read(s + (PA * T::TM + pb * T::TN) * BK, T::TN,
-                                 wn + g * 32 + (lane & 31), kg * KU + k);
+      const int g = late ? which - T::FN - PA : which - 1;
+      b[kg & 1][pb][g] = read(s + (PA * T::TM + pb * T::TN) * BK, T::TN,
+                              wn + g * 32 + (lane & 31), kg);
     }
   };
-  constexpr int PAIRS = PA == 2 ? 3 : PB, MULS = KU * PAIRS * T::FN;
+  constexpr int PAIRS = PA == 2 ? 3 : PB, MULS = PAIRS * T::FN;
   auto multiply_one = [&](int u, int which) {
     const int kg = u / T::FM, f = u % T::FM;
-    const int k = which / (PAIRS * T::FN), c = which / T::FN % PAIRS, g = which % T::FN;
+    const int c = which / T::FN, g = which % T::FN;
     const int pa = PA == 2 && c == 0 ? 1 : 0, pb = PB == 2 && c == PAIRS - 2 ? 1 : 0;
-    acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u & 1][k][pa], b[kg & 1][k][pb][g],
-                                                       acc[f][g], 0, 0, 0);
+    acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u & 1][pa], b[kg & 1][pb][g], acc[f][g],
+                                                       0, 0, 0);
   };
 
   // the last unit's copies that go behind the wait after its first instruction
@@ -415,7 +417,7 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
     wait_loads<0>();
   block_barrier();
 #pragma unroll
-  for (int r = 0; r < KU * (PA + PB * T::FN); ++r) read_one(lds, 0, r);
+  for (int r = 0; r < PA + PB * T::FN; ++r) read_one(lds, 0, r);
   int cur = 0, free = (S - 1) * STAGE;  // the stage read, and the one to fill
   auto step = [&](auto more, int i) {
     constexpr bool MORE = decltype(more)::value;
@@ -423,7 +425,7 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const bool last = u + 1 == UNITS;
-      const int reads = KU * (PA + ((u + 1) % T::FM == 0 ? PB * T::FN : 0));
+      const int reads = PA + ((u + 1) % T::FM == 0 ? PB * T::FN : 0);
       const int c0 = u < SPREAD ? u * LOADS / SPREAD : LOADS;
       const int copies = u < SPREAD ? (u + 1) * LOADS / SPREAD - c0 : 0;
 #pragma unroll
@@ -680,6 +682,397 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
       finish<TO>(tab, t, turn, ka, kb, wi + f * 32, wj + g * 32, mirror, acc[f][g], piece);
 }
 
+// ---- matrices that one block holds ----------------------------------------------
+
+// Sides up to 64 x 256 (a small network's layers): the whole iteration in one
+// launch, iterates in LDS, as pairs of fp16 and with the lo lo products too.
+// What bounds it is latency: five barriers and some 64 matrix instructions a
+// step, 1.5 us.
+//
+// Rows of an LDS plane lie 16 bytes more than a multiple of 64 apart, so that
+// 16 neighbouring rows' chunks fall on all 64 banks.
+
+constexpr int kSmallM = 64, kSmallN = 256, kSmallThreads = 512;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+size_t small_lds(int m, int n) {
+  const size_t mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
+  return 2 * (mp * (np + 8) + np * (mp + 8) + mp * (mp + 8)) * sizeof(f16);
+}
+
+// 16 x 16 pieces of P Q^T, K values at a time from row `p` of P, row `q` of Q
+__device__ __forceinline__ f32x4 small_product(const f16* P, int ldp, size_t lo_p, int p,
+                                               const f16* Q, int ldq, size_t lo_q, int q, int K,
+                                               int lane) {
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const f16* x = P + (p + (lane & 15)) * ldp + (lane >> 4) * 8;
+  const f16* y = Q + (q + (lane & 15)) * ldq + (lane >> 4) * 8;
+#pragma unroll 2
+  for (int k = 0; k < K; k += 32) {
+    const f16x8 xh = *(const f16x8*)(x + k), xl = *(const f16x8*)(x + lo_p + k);
+    const f16x8 yh = *(const f16x8*)(y + k), yl = *(const f16x8*)(y + lo_q + k);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yh, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yl, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yh, acc, 0, 0, 0);
+  }
+  return acc;
+}
+
+struct Poly {
+  float a, b, c, scale_b;
+  int steps;
+};
+
+__device__ void small_matrix(const Table& tab, const Mat& t, const Poly& poly, f16* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int WAVES = kSmallThreads / 64;
+  const int mp = (t.m + 31) / 32 * 32, np = (t.n + 31) / 32 * 32;
+  const int ldx = np + 8, ldt = mp + 8;
+  const size_t lo_x = (size_t)mp * ldx, lo_t = (size_t)np * ldt, lo_a = (size_t)mp * ldt;
+  f16* X = lds;              // mp rows
+  f16* XT = X + 2 * lo_x;    // np rows
+  f16* A = XT + 2 * lo_t;    // mp rows: A, then B
+  const bool turned = t.rows > t.cols;
+
+  // the caller's matrix, 8 values at a time, in registers until |U| is known
+  constexpr int MOST = kSmallM * kSmallN / 8 / kSmallThreads;  // 4
+  const int per_row = (t.cols + 7) / 8, pieces = t.rows * per_row;
+  float u[MOST][8];
+  double sum = 0.0;
+#pragma unroll
+  for (int q = 0; q < MOST; ++q) {
+    const int i = tid + q * kSmallThreads;
+    if (i < pieces) {
+      const int r = i / per_row, c = (i - r * per_row) * 8;
+      const size_t at = (size_t)r * t.cols + c;
+      load8(t.g, at, tab.gtype, t.cols - c, u[q]);
+      if (t.mom) {
+        float m[8];
+        load8(t.mom, at, T_F32, t.cols - c, m);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          m[k] = tab.mu * m[k] + u[q][k];
+          u[q][k] = tab.nesterov ? u[q][k] + tab.mu * m[k] : m[k];
+        }
+        store8(t.mom, at, T_F32, t.cols - c, m);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) sum += (double)u[q][k] * (double)u[q][k];
+    }
+  }
+  // the planes are not in use yet: clear them, and add the sums at their end
+  uint4* clear = (uint4*)lds;
+  const int words = (int)((2 * (lo_x + lo_t + lo_a)) / 8);
+  for (int i = tid; i < words; i += kSmallThreads) clear[i] = make_uint4(0, 0, 0, 0);
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  __shared__ double red[WAVES];
+  if (lane == 0) red[wave] = sum;
+  __syncthreads();
+  double total = 0.0;
+#pragma unroll
+  for (int k = 0; k < WAVES; ++k) total += red[k];
+  const double norm = sqrt(total);
+  const float scale = norm <= (double)tab.eps ? (float)(kScaleX / (double)tab.eps)
+                                              : (float)(kScaleX / norm);
+#pragma unroll
+  for (int q = 0; q < MOST; ++q) {
+    const int i = tid + q * kSmallThreads;
+    if (i < pieces) {
+      const int r = i / per_row, c = (i - r * per_row) * 8;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (c + k < t.cols) {
+          f16 hi, lo;
+          split(u[q][k] * scale, hi, lo);
+          const int x = turned ? c + k : r, y = turned ? r : c + k;
+          X[x * ldx + y] = hi;
+          X[lo_x + x * ldx + y] = lo;
+          XT[y * ldt + x] = hi;
+          XT[lo_t + y * ldt + x] = lo;
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  const float sx = kScaleX, sa = kScaleA, sb = poly.scale_b;
+  const int mt = mp / 16, nt = np / 16;
+  const int row = (lane >> 4) * 4, col = lane & 15;  // 4 rows of a column to a lane
+  auto put = [&](f16* plane, size_t low, size_t at, const f32x4& v) {
+    f16x4 h, l;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      f16 x, y;
+      split(v[r], x, y);
+      h[r] = x;
+      l[r] = y;
+    }
+    *(f16x4*)(plane + at) = h;
+    *(f16x4*)(plane + low + at) = l;
+  };
+  for (int s = 0; s < poly.steps; ++s) {
+    // A and B are kept as their transposes, one bit apart at most
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int b = wave + q * WAVES, i = b / mt * 16, j = b % mt * 16;
+      if (b < mt * mt) {
+        f32x4 v = small_product(X, ldx, lo_x, i, X, ldx, lo_x, j, np, lane);
+        v *= sa / (sx * sx);
+        put(A, lo_a, (j + col) * ldt + i + row, v);
+      }
+    }
+    __syncthreads();
+    f32x4 keep[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int b = wave + q * WAVES, i = b / mt * 16, j = b % mt * 16;
+      if (b < mt * mt) {
+        keep[q] = small_product(A, ldt, lo_a, i, A, ldt, lo_a, j, mp, lane);
+        const size_t at = (j + col) * ldt + i + row;
+        const f16x4 h = *(const f16x4*)(A + at), l = *(const f16x4*)(A + lo_a + at);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          keep[q][r] = poly.c * sb / (sa * sa) * keep[q][r] +
+                       poly.b * sb / sa * ((float)h[r] + (float)l[r]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int b = wave + q * WAVES, i = b / mt * 16, j = b % mt * 16;
+      if (b < mt * mt) put(A, lo_a, (j + col) * ldt + i + row, keep[q]);
+    }
+    __syncthreads();
+    // X' = a X + B X; pieces of a column of X to a wave
+    f32x4 x[2][4];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int j = (wave + q * WAVES) * 16;
+      if (j < np) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int i = p * 16;
+          if (i < mp) {
+            x[q][p] = small_product(A, ldt, lo_a, i, XT, ldt, lo_t, j, mp, lane);
+            const size_t at = (j + col) * ldt + i + row;
+            const f16x4 h = *(const f16x4*)(XT + at), l = *(const f16x4*)(XT + lo_t + at);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              x[q][p][r] = poly.a * ((float)h[r] + (float)l[r]) + x[q][p][r] / sb;
+          }
+        }
+      }
+    }
+    if (s + 1 == poly.steps) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = p * 16 + row + r, j = (wave + q * WAVES) * 16 + col;
+            if (i < t.m && j < t.n) {
+              const size_t at = turned ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
+              float o = x[q][p][r] / sx;
+              if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
+              store_as(t.w, at, tab.wtype, o);
+            }
+          }
+      break;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int j = (wave + q * WAVES) * 16;
+      if (j < np) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int i = p * 16;
+          if (i < mp) {
+            put(XT, lo_t, (j + col) * ldt + i + row, x[q][p]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              f16 hi, lo;
+              split(x[q][p][r], hi, lo);
+              X[(i + row + r) * ldx + j + col] = hi;
+              X[lo_x + (i + row + r) * ldx + j + col] = lo;
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Shorter sides up to 16, longer ones of any length.  The polynomials of A
+// commute, so the iteration needs X only at its ends: with A_0 = U U^T / |U|^2,
+//
+//   Q = a I + b A + c A^2     P <- Q P     A <- Q A Q      O = P U / |U|
+//
+// on 16 x 16 matrices.  A squares the condition of U, which 64 bits bear (in
+// fp32 this form is 10 to 100 times less exact than the other).  Matrices of
+// more than kThinChunk columns take a block for every kThinChunk; the sums of
+// A_0 are then made by a launch of their own, and every block iterates for
+// itself.
+
+constexpr int kThinM = 16, kThinChunk = 1024, kThinLd = 17;
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// U(i, j) for four columns, on the shorter side's rows
+__device__ __forceinline__ void thin_u(const Table& tab, const Mat& t, bool update, int i, int j,
+                                       float* u) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    u[e] = 0.f;
+    if (i < t.m && j + e < t.n) {
+      const size_t at =
+          t.rows > t.cols ? (size_t)(j + e) * t.cols + i : (size_t)i * t.cols + j + e;
+      u[e] = load_as(t.g, at, tab.gtype);
+      if (t.mom) {
+        float m = t.mom[at];
+        if (update) {
+          m = tab.mu * m + u[e];
+          t.mom[at] = m;
+        }
+        u[e] = tab.nesterov ? u[e] + tab.mu * m : m;
+      }
+    }
+  }
+}
+
+// this block's share of U U^T into 256 doubles of LDS
+__device__ void thin_gram(const Table& tab, const Mat& t, int chunk, double* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int WAVES = kSmallThreads / 64;
+  f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+  const int end = t.n - chunk * kThinChunk < kThinChunk ? t.n : (chunk + 1) * kThinChunk;
+  for (int j = chunk * kThinChunk + wave * 16; j < end; j += WAVES * 16) {
+    float u[4];
+    thin_u(tab, t, true, lane & 15, j + (lane >> 4) * 4, u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[e], (double)u[e], acc, 0, 0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) lds[wave * 256 + (r * 4 + (lane >> 4)) * 16 + (lane & 15)] = acc[r];
+  __syncthreads();
+  double s = 0.0;
+  if (tid < 256)
+    for (int k = 0; k < WAVES; ++k) s += lds[k * 256 + tid];
+  __syncthreads();
+  if (tid < 256) lds[tid] = s;
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(kSmallThreads) void flowml_ns_thin_gram(Table tab) {
+  __shared__ double lds[kSmallThreads / 64 * 256];
+  const Mat& t = tab.mat[find(tab, blockIdx.x)];
+  const int chunk = blockIdx.x - t.first;
+  if (t.parts == 1) return;  // one block does it all
+  thin_gram(tab, t, chunk, lds);
+  if (threadIdx.x < 256) t.part[(size_t)chunk * 256 + threadIdx.x] = lds[threadIdx.x];
+}
+
+__device__ void thin_matrix(const Table& tab, const Mat& t, const Poly& poly, int chunk,
+                            double* lds) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  constexpr int WAVES = kSmallThreads / 64;
+  if (t.parts == 1) {
+    thin_gram(tab, t, 0, lds);
+  } else {
+    double s = 0.0;
+    if (tid < 256) {
+      for (int k = 0; k < t.parts; ++k) s += t.part[(size_t)k * 256 + tid];
+      lds[tid] = s;
+    }
+    __syncthreads();
+  }
+  double total = 0.0;
+  for (int k = 0; k < 16; ++k) total += lds[k * 17];
+  const double norm = sqrt(total);
+  const double inv = norm <= (double)tab.eps ? 1.0 / (double)tab.eps : 1.0 / norm;
+
+  // Wave 0 iterates.  A lane's operands of a product of symmetric matrices are
+  // the values (lane & 15, 4 s + lane / 16); it is given (4 r + lane / 16, lane & 15).
+  double* buf = lds + 256;  // 16 rows of kThinLd
+  const int c = lane & 15, q = lane >> 4;
+  if (wave == 0) {
+    f64x4 A, P;  // operands
+#pragma unroll
+    for (int r = 0; r < 4; ++r) A[r] = lds[c * 16 + 4 * r + q] * inv * inv;
+    auto times = [&](const f64x4& x, const f64x4& y) {
+      f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64(x[r], y[r], acc, 0, 0, 0);
+      return acc;
+    };
+    auto operand = [&](const f64x4& v) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) buf[(4 * r + q) * kThinLd + c] = v[r];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      f64x4 o;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = buf[c * kThinLd + 4 * r + q];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      return o;
+    };
+    for (int s = 0; s < poly.steps; ++s) {
+      f64x4 Q = operand(times(A, A));
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        Q[r] = (double)poly.c * Q[r] + (double)poly.b * A[r] + (c == 4 * r + q ? (double)poly.a : 0.0);
+      P = s ? operand(times(Q, P)) : Q;
+      if (s + 1 < poly.steps) A = operand(times(operand(times(Q, A)), Q));
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) buf[c * kThinLd + 4 * r + q] = P[r] * inv;
+  }
+  __syncthreads();
+  f64x4 P;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) P[r] = buf[c * kThinLd + 4 * r + q];
+  const int end = t.n - chunk * kThinChunk < kThinChunk ? t.n : (chunk + 1) * kThinChunk;
+  for (int j0 = chunk * kThinChunk + wave * 16; j0 < end; j0 += WAVES * 16) {
+    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+    const int j = j0 + c;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int k = 4 * r + q;
+      float u = 0.f;
+      if (k < t.m && j < t.n) {
+        const size_t at = t.rows > t.cols ? (size_t)j * t.cols + k : (size_t)k * t.cols + j;
+        u = load_as(t.g, at, tab.gtype);
+        if (t.mom) u = tab.nesterov ? u + tab.mu * t.mom[at] : t.mom[at];
+      }
+      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(P[r], (double)u, acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 4 * r + q;
+      if (i < t.m && j < t.n) {
+        const size_t at = t.rows > t.cols ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
+        float o = (float)acc[r];
+        if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
+        store_as(t.w, at, tab.wtype, o);
+      }
+    }
+  }
+}
+
+extern __shared__ __align__(16) char flowml_ns_lds[];
+
+__global__ __launch_bounds__(kSmallThreads) void flowml_ns_small(Table tab, Poly poly) {
+  const Mat& t = tab.mat[find(tab, blockIdx.x)];
+  if (t.m <= kThinM)
+    thin_matrix(tab, t, poly, blockIdx.x - t.first, (double*)flowml_ns_lds);
+  else
+    small_matrix(tab, t, poly, (f16*)flowml_ns_lds);
+}
+
 // ---- launch plan ----------------------------------------------------------------
 
 constexpr int kPerNormBlock = 8192;
@@ -748,67 +1141,162 @@ void product(Sides s, Table& tab, int turn, float ka, float kb, hipStream_t st) 
     else if (s.sym == 128)
       product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<64, 4>, Depth<64, 4>, Depth<64, 2>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
   } else {
     if (s.all == 256)
       product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
     else if (s.all == 128)
       product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<64, 4>, Depth<64, 2>, Depth<64, 4>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 2>, Depth<32, 5>, TO>(tab, turn, ka, kb, st);
   }
+}
+
+// The way a matrix goes: one block holds it, or 2 + 3 * steps launches.  A
+// short side of 16 or less goes the first way in any company (in 64 bits, where
+// few values leave fp16 pairs' roundings nothing to cancel against); other
+// small ones do if all are small, for a long launch hides them.
+enum { THIN = 0, SMALL = 1, LARGE = 2 };
+
+void ways(int count, const int* rows, const int* cols, int* way) {
+  bool large = false;
+  for (int k = 0; k < count; ++k) {
+    const int m = rows[k] < cols[k] ? rows[k] : cols[k], n = rows[k] < cols[k] ? cols[k] : rows[k];
+    way[k] = m <= kThinM ? THIN : m <= kSmallM && n <= kSmallN ? SMALL : LARGE;
+    large |= way[k] == LARGE;
+  }
+  if (large)
+    for (int k = 0; k < count; ++k)
+      if (way[k] == SMALL) way[k] = LARGE;
+}
+
+size_t thin_bytes(int rows, int cols) {
+  const int n = rows < cols ? cols : rows, chunks = (n + kThinChunk - 1) / kThinChunk;
+  return chunks > 1 ? (size_t)chunks * 256 * sizeof(double) : 0;
+}
+
+struct Call {
+  int count;
+  const int *rows, *cols;
+  const void* const* g;
+  float* const* mom;
+  void* const* w;
+  const float* step;
+};
+
+// up to kMats matrices of the way `way` (or, for SMALL, both that one block
+// holds), from index k0 on; returns the index behind them
+int gather(Table& tab, const Call& c, const int* way, bool large, int k0) {
+  tab.count = 0;
+  int k = k0;
+  for (; k < c.count && tab.count < kMats; ++k) {
+    if ((way[k] == LARGE) != large) continue;
+    Mat& t = tab.mat[tab.count++];
+    t.rows = c.rows[k];
+    t.cols = c.cols[k];
+    t.m = t.rows < t.cols ? t.rows : t.cols;
+    t.n = t.rows < t.cols ? t.cols : t.rows;
+    t.g = c.g[k];
+    t.mom = c.mom ? c.mom[k] : nullptr;
+    t.w = c.w[k];
+    t.step = c.step ? c.step[k] : 0.f;
+  }
+  return k;
+}
+
+// the large ones' shapes alone, for the tiles' sides
+int large_shapes(int count, const int* rows, const int* cols, const int* way, int* r, int* c) {
+  int n = 0;
+  for (int k = 0; k < count; ++k)
+    if (way[k] == LARGE) {
+      r[n] = rows[k];
+      c[n++] = cols[k];
+    }
+  return n;
 }
 
 }  // namespace
 
 // ---- host entry points ------------------------------------------------------------
 
-// workspace of a call, in bytes
-extern "C" long long muon_workspace(int count, const int* rows, const int* cols) {
-  const Sides s = sides_for(count, rows, cols);
+// workspace of a call, in bytes; `scratch`: 3 * count integers
+extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int* scratch) {
+  int *way = scratch, *r = scratch + count, *c = scratch + 2 * count;
+  ways(count, rows, cols, way);
+  const int n = large_shapes(count, rows, cols, way, r, c);
+  const Sides s = sides_for(n, r, c);
   size_t sum = 0;
-  for (int k = 0; k < count; ++k) sum += bytes_of(rows[k], cols[k], s);
+  for (int k = 0; k < count; ++k) {
+    if (way[k] == LARGE) sum += bytes_of(rows[k], cols[k], s);
+    if (way[k] == THIN) sum += thin_bytes(rows[k], cols[k]);
+  }
   return (long long)sum;
 }
 
 // g: gradients; mom: momentum buffers, or null for the orthogonalisation
 // alone; w: weights, or results.  coef: a, b, c; scale_b: a power of two that
 // brings B into fp16.  full: three products for every matrix, whatever its
-// size.
+// size.  ws: muon_workspace() bytes; scratch: as there.
 extern "C" void launch_muon(int count, const int* rows, const int* cols, const void* const* g,
                             float* const* mom, void* const* w, const float* step, int gtype,
                             int wtype, float mu, float keep, float eps, int nesterov, int steps,
-                            const float* coef, float scale_b, int full, void* ws, void* stream) {
+                            const float* coef, float scale_b, int full, void* ws, int* scratch,
+                            void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const Sides sides = sides_for(count, rows, cols);
+  int* way = scratch;
+  ways(count, rows, cols, way);
+  const int n = large_shapes(count, rows, cols, way, scratch + count, scratch + 2 * count);
+  const Sides sides = sides_for(n, scratch + count, scratch + 2 * count);
+  const Call call = {count, rows, cols, g, mom, w, step};
   const float sa = kScaleA, sx = kScaleX, sb = scale_b;
+  Table tab;
+  tab.gtype = gtype;
+  tab.wtype = wtype;
+  tab.mu = mu;
+  tab.keep = keep;
+  tab.eps = eps;
+  tab.nesterov = nesterov;
   char* at = (char*)ws;
-  for (int k0 = 0; k0 < count; k0 += kMats) {
-    Table tab;
-    tab.count = count - k0 < kMats ? count - k0 : kMats;
-    tab.gtype = gtype;
-    tab.wtype = wtype;
-    tab.mu = mu;
-    tab.keep = keep;
-    tab.eps = eps;
-    tab.nesterov = nesterov;
+
+  for (int k0 = 0; k0 < count;) {
+    k0 = gather(tab, call, way, false, k0);
+    if (!tab.count) break;
+    int blocks = 0;
+    bool chunks = false;
+    size_t lds = (256 + 16 * kThinLd + kSmallThreads / 64 * 256) * sizeof(double);
+    for (int k = 0; k < tab.count; ++k) {
+      Mat& t = tab.mat[k];
+      t.part = (double*)at;
+      t.first = blocks;
+      t.parts = 1;
+      if (t.m <= kThinM) {
+        t.parts = (t.n + kThinChunk - 1) / kThinChunk;
+        at += thin_bytes(t.rows, t.cols);
+        chunks |= t.parts > 1;
+      } else {
+        const size_t b = small_lds(t.m, t.n);
+        lds = lds > b ? lds : b;
+      }
+      blocks += t.parts;
+    }
+    if (chunks)
+      hipLaunchKernelGGL(flowml_ns_thin_gram, dim3(blocks), dim3(kSmallThreads), 0, st, tab);
+    const Poly poly = {coef[0], coef[1], coef[2], sb, steps};
+    hipLaunchKernelGGL(flowml_ns_small, dim3(blocks), dim3(kSmallThreads), lds, st, tab, poly);
+  }
+
+  for (int k0 = 0; k0 < count;) {
+    k0 = gather(tab, call, way, true, k0);
+    if (!tab.count) break;
     int blocks = 0;
     for (int k = 0; k < tab.count; ++k) {
       Mat& t = tab.mat[k];
-      t.rows = rows[k0 + k];
-      t.cols = cols[k0 + k];
-      t.m = t.rows < t.cols ? t.rows : t.cols;
-      t.n = t.rows < t.cols ? t.cols : t.rows;
       t.mp = pad(t.m, sides.all);
       t.np = pad(t.n, sides.all);
       t.ma = pad(t.mp, sides.sym);
       t.part = (double*)at;
       t.ws = (f16*)(at + kNormBlocks * sizeof(double));
       at += bytes_of(t.rows, t.cols, sides);
-      t.g = g[k0 + k];
-      t.mom = mom ? mom[k0 + k] : nullptr;
-      t.w = w[k0 + k];
-      t.step = step ? step[k0 + k] : 0.f;
       t.full = full || t.m < 256;
       const size_t want = ((size_t)t.rows * t.cols + kPerNormBlock - 1) / kPerNormBlock;
       t.parts = (int)(want < kNormBlocks ? want : kNormBlocks);

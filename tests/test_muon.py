@@ -132,12 +132,13 @@ def test_other_polynomials(coef, steps, dev):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-def test_special_values(dev):
-    z = torch.zeros(40, 70, device=dev)
+@pytest.mark.parametrize("m,n", [(40, 70), (70, 7), (9, 3000), (130, 90), (300, 300)])
+def test_special_values(m, n, dev):
+    z = torch.zeros(m, n, device=dev)
     assert torch.equal(ops.newton_schulz(z), z)
     # norms below eps are divided by eps; very small and very large ones keep
     # their digits
-    G = gradient("full", 40, 70).to(dev)
+    G = gradient("full", m, n).to(dev)
     G = G / G.norm()
     check(G * 1e-9, ops.newton_schulz(G * 1e-9))
     check(G * 1e-3, ops.newton_schulz(G * 1e-3, eps=1e-2), eps=1e-2)
@@ -152,8 +153,8 @@ def test_special_values(dev):
     # empty matrices, an empty stack, an empty sequence
     outs = ops.newton_schulz([G, G[:0], G[:, :0]])
     check(G, outs[0])
-    assert outs[1].shape == (0, 70) and outs[2].shape == (40, 0)
-    assert ops.newton_schulz(G[None][:0]).shape == (0, 40, 70)
+    assert outs[1].shape == (0, n) and outs[2].shape == (m, 0)
+    assert ops.newton_schulz(G[None][:0]).shape == (0, m, n)
     assert ops.newton_schulz([]) == []
 
 
@@ -172,12 +173,17 @@ def step_reference(w, g, m, lr, mu, wd, nesterov, steps=5):
     return (1 - lr * wd) * w.double() - s * o, m, u, sizes, s
 
 
+SETS = {"small": [(41, 128), (128, 64), (64, 5), (0, 4), (1, 1)],
+        "mixed": [(41, 128), (64, 5), (300, 290), (3, 2100), (129, 70)]}
+
+
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("which", SETS)
 @pytest.mark.parametrize("wtype,gtype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16),
                                          (torch.float32, torch.bfloat16), (torch.float16, torch.float32)])
 @pytest.mark.parametrize("nesterov", [True, False])
-def test_update(wtype, gtype, nesterov, dev):
-    shapes = [(41, 128), (128, 64), (64, 5), (0, 4), (300, 290), (1, 1)]
+def test_update(wtype, gtype, nesterov, which, dev):
+    shapes = SETS[which]
     ws = [gradient("full", *s, seed=1).to(wtype).to(dev) for s in shapes]
     ms = [gradient("offset", *s, seed=2).to(dev) if s[0] else torch.zeros(s, device=dev) for s in shapes]
     for turn in range(2):
@@ -201,8 +207,8 @@ def test_update(wtype, gtype, nesterov, dev):
 
 
 @pytest.mark.gpu
-def test_update_twice_the_same_and_in_a_graph():
-    shapes = [(41, 128), (300, 500), (129, 5)]
+@pytest.mark.parametrize("shapes", [[(41, 128), (64, 5)], [(41, 128), (300, 500), (5, 1300)]])
+def test_update_twice_the_same_and_in_a_graph(shapes):
     mk = lambda seed: [gradient("offset", *s, seed=seed).cuda() for s in shapes]  # noqa: E731
     ws, gs, ms = mk(1), mk(2), mk(3)
 
