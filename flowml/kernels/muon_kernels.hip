@@ -106,6 +106,8 @@ __device__ __forceinline__ f16* ws_b(const Mat& t, int p) {
   return t.ws + 2 * plane_x(t) + 4 * plane_xt(t) + (2 + p) * plane_a(t);
 }
 
+// (Every function that takes the table is inlined: it stays in the arguments'
+// memory, and is copied to each lane's stack as soon as one is not.)
 __device__ __forceinline__ int find(const Table& tab, int block) {
   int k = 0;
   while (k + 1 < tab.count && block >= tab.mat[k + 1].first) ++k;
@@ -684,40 +686,68 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
 
 // ---- matrices that one block holds ----------------------------------------------
 
-// Sides up to 64 x 256 (a small network's layers): the whole iteration in one
-// launch, iterates in LDS, as pairs of fp16 and with the lo lo products too.
-// What bounds it is latency: five barriers and some 64 matrix instructions a
-// step, 1.5 us.
+// What fits 160 KB of LDS (a small network's layers; 64 x 416, 128 x 160): the
+// whole iteration in one launch, with iterates as pairs of fp16.  Latency
+// bounds it: three or four barriers a step, chains of matrix instructions
+// between them.
 //
-// Rows of an LDS plane lie 16 bytes more than a multiple of 64 apart, so that
-// 16 neighbouring rows' chunks fall on all 64 banks.
+// Only the transpose of X is kept.  B X reads its rows; X X^T takes columns,
+// through LDS reads that transpose: 16 lanes load 4 rows of 16 values, and
+// each gets a column.  Rows lie 16 bytes more than a multiple of 64 apart, so
+// that 16 neighbouring rows' chunks fall on all 64 banks.
 
-constexpr int kSmallM = 64, kSmallN = 256, kSmallThreads = 512;
+constexpr int kSmallM = 128, kSmallThreads = 512, kSmallWaves = kSmallThreads / 64;
+constexpr size_t kSmallLds = 160 * 1024 - 256;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// pieces of 16 on the shorter side: 2, 4 or 8
+__host__ __device__ inline int small_pieces(int m) { return m <= 32 ? 2 : m <= 64 ? 4 : 8; }
+
 size_t small_lds(int m, int n) {
-  const size_t mp = (m + 31) / 32 * 32, np = (n + 31) / 32 * 32;
-  return 2 * (mp * (np + 8) + np * (mp + 8) + mp * (mp + 8)) * sizeof(f16);
+  const size_t mt = small_pieces(m), mp = mt * 16, np = (n + 31) / 32 * 32;
+  return 2 * (np + (mt == 8 ? 1 : 2) * mp) * (mp + 8) * sizeof(f16);
 }
 
-// 16 x 16 pieces of P Q^T, K values at a time from row `p` of P, row `q` of Q
-__device__ __forceinline__ f32x4 small_product(const f16* P, int ldp, size_t lo_p, int p,
-                                               const f16* Q, int ldq, size_t lo_q, int q, int K,
-                                               int lane) {
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  const f16* x = P + (p + (lane & 15)) * ldp + (lane >> 4) * 8;
-  const f16* y = Q + (q + (lane & 15)) * ldq + (lane >> 4) * 8;
-#pragma unroll 2
-  for (int k = 0; k < K; k += 32) {
-    const f16x8 xh = *(const f16x8*)(x + k), xl = *(const f16x8*)(x + lo_p + k);
-    const f16x8 yh = *(const f16x8*)(y + k), yl = *(const f16x8*)(y + lo_q + k);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yl, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xl, yh, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yl, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(xh, yh, acc, 0, 0, 0);
-  }
-  return acc;
+bool small_fits(int m, int n) { return m <= kSmallM && n < 4096 && small_lds(m, n) <= kSmallLds; }
+
+// A lane's 8 values of a chunk of 32 in a row of 16 rows' operand, both planes.
+struct Halves {
+  f16x8 hi, lo;
+};
+
+__device__ __forceinline__ Halves small_read(const f16* plane, int low, int at) {
+  return {*(const f16x8*)(plane + at), *(const f16x8*)(plane + low + at)};
+}
+
+// the same of 32 rows from `k` on, columns i to i + 15
+__device__ __forceinline__ f16x8 read_columns(const f16* plane, int ld, int k, int i, int lane) {
+#ifdef __HIP_DEVICE_COMPILE__
+  typedef __fp16 h4 __attribute__((vector_size(8)));
+  typedef __attribute__((address_space(3))) h4 lds_h4;
+  const f16* at = plane + (k + (lane >> 4) * 8 + ((lane & 15) >> 2)) * ld + i + (lane & 3) * 4;
+  const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4*)at));
+  const f16x4 b =
+      __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4*)(at + 4 * ld)));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+#else
+  return f16x8{};
+#endif
+}
+
+__device__ __forceinline__ Halves small_columns(const f16* plane, int low, int ld, int k, int i,
+                                                int lane) {
+  return {read_columns(plane, ld, k, i, lane), read_columns(plane + low, ld, k, i, lane)};
+}
+
+// acc += x y; ALL: the product of the lower halves too, which counts where few
+// values are summed (17 columns: 1.5 times fp32's error without, 1.2 with)
+template <bool ALL>
+__device__ __forceinline__ void small_multiply(const Halves& x, const Halves& y, f32x4& acc) {
+  if (ALL) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.lo, y.lo, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.lo, y.hi, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.hi, y.lo, acc, 0, 0, 0);
+  acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(x.hi, y.hi, acc, 0, 0, 0);
 }
 
 struct Poly {
@@ -725,82 +755,107 @@ struct Poly {
   int steps;
 };
 
-__device__ void small_matrix(const Table& tab, const Mat& t, const Poly& poly, f16* lds) {
+// U for 8 values side by side; `update`: the momentum is moved on, too
+__device__ __forceinline__ void small_u(const Table& tab, const Mat& t, bool update, size_t at,
+                                        int left, float* u) {
+  load8(t.g, at, tab.gtype, left, u);
+  if (t.mom) {
+    float m[8];
+    load8(t.mom, at, T_F32, left, m);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (update) m[k] = tab.mu * m[k] + u[k];
+      u[k] = tab.nesterov ? u[k] + tab.mu * m[k] : m[k];
+    }
+    if (update) store8(t.mom, at, T_F32, left, m);
+  }
+}
+
+template <int MT>
+__device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, const Poly& poly,
+                                             f16* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int WAVES = kSmallThreads / 64;
-  const int mp = (t.m + 31) / 32 * 32, np = (t.n + 31) / 32 * 32;
-  const int ldx = np + 8, ldt = mp + 8;
-  const size_t lo_x = (size_t)mp * ldx, lo_t = (size_t)np * ldt, lo_a = (size_t)mp * ldt;
-  f16* X = lds;              // mp rows
-  f16* XT = X + 2 * lo_x;    // np rows
-  f16* A = XT + 2 * lo_t;    // mp rows: A, then B
+  constexpr int mp = MT * 16, ld = mp + 8, KC = MT / 2;  // KC: chunks of 32 in m
+  constexpr bool ALL = MT == 2, APART = MT < 8;          // B apart from A
+  const int np = (t.n + 31) / 32 * 32;
+  const int lo_x = np * ld;
+  constexpr int lo_a = mp * ld;
+  f16* XT = lds;            // np rows
+  f16* A = XT + 2 * lo_x;   // mp rows
+  f16* B = APART ? A + 2 * lo_a : A;
   const bool turned = t.rows > t.cols;
 
-  // the caller's matrix, 8 values at a time, in registers until |U| is known
-  constexpr int MOST = kSmallM * kSmallN / 8 / kSmallThreads;  // 4
+  // Pieces of 8 values of the caller's rows.  Neighbouring lanes take
+  // neighbouring m: so their 2-byte writes do not meet in a bank.
   const int per_row = (t.cols + 7) / 8, pieces = t.rows * per_row;
-  float u[MOST][8];
-  double sum = 0.0;
-#pragma unroll
-  for (int q = 0; q < MOST; ++q) {
-    const int i = tid + q * kSmallThreads;
-    if (i < pieces) {
-      const int r = i / per_row, c = (i - r * per_row) * 8;
-      const size_t at = (size_t)r * t.cols + c;
-      load8(t.g, at, tab.gtype, t.cols - c, u[q]);
-      if (t.mom) {
-        float m[8];
-        load8(t.mom, at, T_F32, t.cols - c, m);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          m[k] = tab.mu * m[k] + u[q][k];
-          u[q][k] = tab.nesterov ? u[q][k] + tab.mu * m[k] : m[k];
-        }
-        store8(t.mom, at, T_F32, t.cols - c, m);
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum += (double)u[q][k] * (double)u[q][k];
+  auto piece = [&](int p, int& r, int& c) {
+    if (turned) {
+      r = p / per_row;
+      c = (p - r * per_row) * 8;
+    } else {
+      c = p / t.rows;
+      r = p - c * t.rows;
+      c *= 8;
     }
+  };
+  double sum = 0.0;
+  for (int p = tid; p < pieces; p += kSmallThreads) {
+    int r, c;
+    piece(p, r, c);
+    float u[8];
+    small_u(tab, t, true, (size_t)r * t.cols + c, t.cols - c, u);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += (double)u[k] * (double)u[k];
   }
-  // the planes are not in use yet: clear them, and add the sums at their end
-  uint4* clear = (uint4*)lds;
-  const int words = (int)((2 * (lo_x + lo_t + lo_a)) / 8);
-  for (int i = tid; i < words; i += kSmallThreads) clear[i] = make_uint4(0, 0, 0, 0);
+  uint4* clear = (uint4*)XT;
+  for (int i = tid; i < lo_x / 4; i += kSmallThreads) clear[i] = make_uint4(0, 0, 0, 0);
   for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-  __shared__ double red[WAVES];
+  __shared__ double red[kSmallWaves];
   if (lane == 0) red[wave] = sum;
   __syncthreads();
   double total = 0.0;
 #pragma unroll
-  for (int k = 0; k < WAVES; ++k) total += red[k];
+  for (int k = 0; k < kSmallWaves; ++k) total += red[k];
   const double norm = sqrt(total);
   const float scale = norm <= (double)tab.eps ? (float)(kScaleX / (double)tab.eps)
                                               : (float)(kScaleX / norm);
+  for (int p = tid; p < pieces; p += kSmallThreads) {
+    int r, c;
+    piece(p, r, c);
+    float u[8];
+    small_u(tab, t, false, (size_t)r * t.cols + c, t.cols - c, u);
+    f16x8 hi, lo;
 #pragma unroll
-  for (int q = 0; q < MOST; ++q) {
-    const int i = tid + q * kSmallThreads;
-    if (i < pieces) {
-      const int r = i / per_row, c = (i - r * per_row) * 8;
+    for (int k = 0; k < 8; ++k) {
+      f16 x, y;
+      split(u[k] * scale, x, y);
+      hi[k] = x;
+      lo[k] = y;
+    }
+    if (turned) {  // what load8 puts behind the row's end is 0
+      *(f16x8*)(XT + r * ld + c) = hi;
+      *(f16x8*)(XT + lo_x + r * ld + c) = lo;
+    } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < 8; ++k)
         if (c + k < t.cols) {
-          f16 hi, lo;
-          split(u[q][k] * scale, hi, lo);
-          const int x = turned ? c + k : r, y = turned ? r : c + k;
-          X[x * ldx + y] = hi;
-          X[lo_x + x * ldx + y] = lo;
-          XT[y * ldt + x] = hi;
-          XT[lo_t + y * ldt + x] = lo;
+          XT[(c + k) * ld + r] = hi[k];
+          XT[lo_x + (c + k) * ld + r] = lo[k];
         }
-      }
     }
   }
   __syncthreads();
 
   const float sx = kScaleX, sa = kScaleA, sb = poly.scale_b;
-  const int mt = mp / 16, nt = np / 16;
+  const float to_a = sa / (sx * sx), b_old = poly.b * sb / sa, b_new = poly.c * sb / (sa * sa);
+  const float to_x = 1.f / sb, to_end = 1.f / sx;
   const int row = (lane >> 4) * 4, col = lane & 15;  // 4 rows of a column to a lane
-  auto put = [&](f16* plane, size_t low, size_t at, const f32x4& v) {
+  const int from = (lane >> 4) * 8;                  // of an operand's chunk of 32
+  // A and B: AW pieces of a row of pieces to a wave
+  constexpr int AW = MT * MT / kSmallWaves < 1 ? 1 : MT * MT / kSmallWaves;
+  const int ai = wave * AW / MT * 16, aj = wave * AW % MT * 16;
+  const bool has_a = wave * AW < MT * MT;
+  auto put = [&](f16* plane, int low, int at, const f32x4& v) {
     f16x4 h, l;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -812,95 +867,84 @@ __device__ void small_matrix(const Table& tab, const Mat& t, const Poly& poly, f
     *(f16x4*)(plane + at) = h;
     *(f16x4*)(plane + low + at) = l;
   };
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < poly.steps; ++s) {
     // A and B are kept as their transposes, one bit apart at most
+    f32x4 v[AW];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int b = wave + q * WAVES, i = b / mt * 16, j = b % mt * 16;
-      if (b < mt * mt) {
-        f32x4 v = small_product(X, ldx, lo_x, i, X, ldx, lo_x, j, np, lane);
-        v *= sa / (sx * sx);
-        put(A, lo_a, (j + col) * ldt + i + row, v);
+    for (int q = 0; q < AW; ++q) v[q] = zero;
+    if (has_a) {
+#pragma unroll 2
+      for (int k = 0; k < np; k += 32) {
+        const Halves x = small_columns(XT, lo_x, ld, k, ai, lane);
+#pragma unroll
+        for (int q = 0; q < AW; ++q)
+          small_multiply<ALL>(x, small_columns(XT, lo_x, ld, k, aj + q * 16, lane), v[q]);
       }
+#pragma unroll
+      for (int q = 0; q < AW; ++q)
+        put(A, lo_a, (aj + q * 16 + col) * ld + ai + row, v[q] * to_a);
     }
     __syncthreads();
-    f32x4 keep[2];
+    if (has_a) {
+      Halves x[KC];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int b = wave + q * WAVES, i = b / mt * 16, j = b % mt * 16;
-      if (b < mt * mt) {
-        keep[q] = small_product(A, ldt, lo_a, i, A, ldt, lo_a, j, mp, lane);
-        const size_t at = (j + col) * ldt + i + row;
+      for (int k = 0; k < KC; ++k) x[k] = small_read(A, lo_a, (ai + col) * ld + from + k * 32);
+#pragma unroll
+      for (int q = 0; q < AW; ++q) {
+        const int at = (aj + q * 16 + col) * ld + ai + row;
         const f16x4 h = *(const f16x4*)(A + at), l = *(const f16x4*)(A + lo_a + at);
+        f32x4 w = zero;
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+          small_multiply<ALL>(
+              x[k], small_read(A, lo_a, (aj + q * 16 + col) * ld + from + k * 32), w);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[q][r] = b_new * w[r] + b_old * ((float)h[r] + (float)l[r]);
+      }
+    }
+    if (!APART) __syncthreads();
+    if (has_a) {
+#pragma unroll
+      for (int q = 0; q < AW; ++q)
+        put(B, lo_a, (aj + q * 16 + col) * ld + ai + row, v[q]);
+    }
+    __syncthreads();
+    // X' = a X + B X; a wave takes whole rows of X^T, which nobody else reads here
+    for (int j = wave * 16; j < np; j += kSmallWaves * 16) {
+      Halves y[KC];
+#pragma unroll
+      for (int k = 0; k < KC; ++k) y[k] = small_read(XT, lo_x, (j + col) * ld + from + k * 32);
+      f32x4 x[MT];
+#pragma unroll
+      for (int p = 0; p < MT; ++p) {
+        x[p] = zero;
+#pragma unroll
+        for (int k = 0; k < KC; ++k)
+          small_multiply<ALL>(small_read(B, lo_a, (p * 16 + col) * ld + from + k * 32), y[k], x[p]);
+        const int at = (j + col) * ld + p * 16 + row;
+        const f16x4 h = *(const f16x4*)(XT + at), l = *(const f16x4*)(XT + lo_x + at);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          keep[q][r] = poly.c * sb / (sa * sa) * keep[q][r] +
-                       poly.b * sb / sa * ((float)h[r] + (float)l[r]);
+          x[p][r] = poly.a * ((float)h[r] + (float)l[r]) + to_x * x[p][r];
       }
-    }
-    __syncthreads();
+      if (s + 1 < poly.steps) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int b = wave + q * WAVES, i = b / mt * 16, j = b % mt * 16;
-      if (b < mt * mt) put(A, lo_a, (j + col) * ldt + i + row, keep[q]);
-    }
-    __syncthreads();
-    // X' = a X + B X; pieces of a column of X to a wave
-    f32x4 x[2][4];
+        for (int p = 0; p < MT; ++p) put(XT, lo_x, (j + col) * ld + p * 16 + row, x[p]);
+      } else {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int j = (wave + q * WAVES) * 16;
-      if (j < np) {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const int i = p * 16;
-          if (i < mp) {
-            x[q][p] = small_product(A, ldt, lo_a, i, XT, ldt, lo_t, j, mp, lane);
-            const size_t at = (j + col) * ldt + i + row;
-            const f16x4 h = *(const f16x4*)(XT + at), l = *(const f16x4*)(XT + lo_t + at);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              x[q][p][r] = poly.a * ((float)h[r] + (float)l[r]) + x[q][p][r] / sb;
-          }
-        }
-      }
-    }
-    if (s + 1 == poly.steps) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q)
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
+        for (int p = 0; p < MT; ++p)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int i = p * 16 + row + r, j = (wave + q * WAVES) * 16 + col;
-            if (i < t.m && j < t.n) {
-              const size_t at = turned ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
-              float o = x[q][p][r] / sx;
+            const int i = p * 16 + row + r;
+            if (i < t.m && j + col < t.n) {
+              const size_t at =
+                  turned ? (size_t)(j + col) * t.cols + i : (size_t)i * t.cols + j + col;
+              float o = to_end * x[p][r];
               if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
               store_as(t.w, at, tab.wtype, o);
             }
           }
-      break;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const int j = (wave + q * WAVES) * 16;
-      if (j < np) {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const int i = p * 16;
-          if (i < mp) {
-            put(XT, lo_t, (j + col) * ldt + i + row, x[q][p]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              f16 hi, lo;
-              split(x[q][p][r], hi, lo);
-              X[(i + row + r) * ldx + j + col] = hi;
-              X[lo_x + (i + row + r) * ldx + j + col] = lo;
-            }
-          }
-        }
       }
     }
     __syncthreads();
@@ -921,13 +965,13 @@ __device__ void small_matrix(const Table& tab, const Mat& t, const Poly& poly, f
 constexpr int kThinM = 16, kThinChunk = 1024, kThinLd = 17;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
-// U(i, j) for four columns, on the shorter side's rows
+// U(i, j) for four columns before `end`, on the shorter side's rows
 __device__ __forceinline__ void thin_u(const Table& tab, const Mat& t, bool update, int i, int j,
-                                       float* u) {
+                                       int end, float* u) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     u[e] = 0.f;
-    if (i < t.m && j + e < t.n) {
+    if (i < t.m && j + e < end) {
       const size_t at =
           t.rows > t.cols ? (size_t)(j + e) * t.cols + i : (size_t)i * t.cols + j + e;
       u[e] = load_as(t.g, at, tab.gtype);
@@ -944,17 +988,21 @@ __device__ __forceinline__ void thin_u(const Table& tab, const Mat& t, bool upda
 }
 
 // this block's share of U U^T into 256 doubles of LDS
-__device__ void thin_gram(const Table& tab, const Mat& t, int chunk, double* lds) {
+__device__ __forceinline__ void thin_gram(const Table& tab, const Mat& t, int chunk, double* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int WAVES = kSmallThreads / 64;
+  constexpr int WAVES = kSmallWaves;
   f64x4 acc = {0.0, 0.0, 0.0, 0.0};
   const int end = t.n - chunk * kThinChunk < kThinChunk ? t.n : (chunk + 1) * kThinChunk;
-  for (int j = chunk * kThinChunk + wave * 16; j < end; j += WAVES * 16) {
-    float u[4];
-    thin_u(tab, t, true, lane & 15, j + (lane >> 4) * 4, u);
+  for (int j = chunk * kThinChunk + wave * 16; j < end; j += 4 * WAVES * 16) {
+    float u[4][4];  // four groups' loads under way together
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[e], (double)u[e], acc, 0, 0, 0);
+    for (int h = 0; h < 4; ++h)
+      thin_u(tab, t, true, lane & 15, j + h * WAVES * 16 + (lane >> 4) * 4, end, u[h]);
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[h][e], (double)u[h][e], acc, 0, 0, 0);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) lds[wave * 256 + (r * 4 + (lane >> 4)) * 16 + (lane & 15)] = acc[r];
@@ -976,10 +1024,10 @@ __global__ __launch_bounds__(kSmallThreads) void flowml_ns_thin_gram(Table tab) 
   if (threadIdx.x < 256) t.part[(size_t)chunk * 256 + threadIdx.x] = lds[threadIdx.x];
 }
 
-__device__ void thin_matrix(const Table& tab, const Mat& t, const Poly& poly, int chunk,
+__device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, const Poly& poly, int chunk,
                             double* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  constexpr int WAVES = kSmallThreads / 64;
+  constexpr int WAVES = kSmallWaves;
   if (t.parts == 1) {
     thin_gram(tab, t, 0, lds);
   } else {
@@ -1069,8 +1117,12 @@ __global__ __launch_bounds__(kSmallThreads) void flowml_ns_small(Table tab, Poly
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   if (t.m <= kThinM)
     thin_matrix(tab, t, poly, blockIdx.x - t.first, (double*)flowml_ns_lds);
+  else if (small_pieces(t.m) == 2)
+    small_matrix<2>(tab, t, poly, (f16*)flowml_ns_lds);
+  else if (small_pieces(t.m) == 4)
+    small_matrix<4>(tab, t, poly, (f16*)flowml_ns_lds);
   else
-    small_matrix(tab, t, poly, (f16*)flowml_ns_lds);
+    small_matrix<8>(tab, t, poly, (f16*)flowml_ns_lds);
 }
 
 // ---- launch plan ----------------------------------------------------------------
@@ -1162,7 +1214,7 @@ void ways(int count, const int* rows, const int* cols, int* way) {
   bool large = false;
   for (int k = 0; k < count; ++k) {
     const int m = rows[k] < cols[k] ? rows[k] : cols[k], n = rows[k] < cols[k] ? cols[k] : rows[k];
-    way[k] = m <= kThinM ? THIN : m <= kSmallM && n <= kSmallN ? SMALL : LARGE;
+    way[k] = m <= kThinM ? THIN : small_fits(m, n) ? SMALL : LARGE;
     large |= way[k] == LARGE;
   }
   if (large)
