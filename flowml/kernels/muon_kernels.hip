@@ -965,26 +965,40 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
 constexpr int kThinM = 16, kThinChunk = 1024, kThinLd = 17;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
-// U(i, j) for four columns before `end`, on the shorter side's rows
-__device__ __forceinline__ void thin_u(const Table& tab, const Mat& t, bool update, int i, int j,
-                                       int end, float* u) {
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    u[e] = 0.f;
-    if (i < t.m && j + e < end) {
-      const size_t at =
-          t.rows > t.cols ? (size_t)(j + e) * t.cols + i : (size_t)i * t.cols + j + e;
-      u[e] = load_as(t.g, at, tab.gtype);
-      if (t.mom) {
-        float m = t.mom[at];
-        if (update) {
-          m = tab.mu * m + u[e];
-          t.mom[at] = m;
-        }
-        u[e] = tab.nesterov ? u[e] + tab.mu * m : m;
-      }
+// Place of (i, j) in the caller's matrix, i on its shorter side.
+__device__ __forceinline__ size_t thin_place(const Mat& t, int i, int j) {
+  return t.rows > t.cols ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
+}
+
+// U(i, j).  Places outside are read at the nearest one inside and dropped: no
+// branch, so that many loads are under way.
+template <typename G>
+__device__ __forceinline__ float thin_u(const Table& tab, const Mat& t, bool update, int i, int j,
+                                        int end) {
+  const bool in = i < t.m && j < end;
+  const size_t at = thin_place(t, i < t.m ? i : t.m - 1, j < end ? j : end - 1);
+  float u = (float)((const G*)t.g)[at];
+  if (t.mom) {
+    float m = t.mom[at];
+    if (update) {
+      m = tab.mu * m + u;
+      if (in) t.mom[at] = m;
     }
+    u = tab.nesterov ? u + tab.mu * m : m;
   }
+  return in ? u : 0.f;
+}
+
+// f(a value of the gradients' type): the type is asked for once, not at every
+// load, where the branches would let one load follow the other.
+template <typename F>
+__device__ __forceinline__ void by_type(int type, F f) {
+  if (type == T_F32)
+    f(0.f);
+  else if (type == T_BF16)
+    f((__bf16)0.f);
+  else
+    f((f16)0.f);
 }
 
 // this block's share of U U^T into 256 doubles of LDS
@@ -993,17 +1007,24 @@ __device__ __forceinline__ void thin_gram(const Table& tab, const Mat& t, int ch
   constexpr int WAVES = kSmallWaves;
   f64x4 acc = {0.0, 0.0, 0.0, 0.0};
   const int end = t.n - chunk * kThinChunk < kThinChunk ? t.n : (chunk + 1) * kThinChunk;
-  for (int j = chunk * kThinChunk + wave * 16; j < end; j += 4 * WAVES * 16) {
-    float u[4][4];  // four groups' loads under way together
+  by_type(tab.gtype, [&](auto like) {
+    for (int j = chunk * kThinChunk + wave * 16; j < end; j += 4 * WAVES * 16) {
+      float u[4][4];
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
-      thin_u(tab, t, true, lane & 15, j + h * WAVES * 16 + (lane >> 4) * 4, end, u[h]);
+      for (int h = 0; h < 4; ++h)
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
+        for (int e = 0; e < 4; ++e)
+          u[h][e] = thin_u<decltype(like)>(tab, t, true, lane & 15,
+                                           j + h * WAVES * 16 + (lane >> 4) * 4 + e, end);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[h][e], (double)u[h][e], acc, 0, 0, 0);
-  }
+      for (int h = 0; h < 4; ++h)
+        if (j + h * WAVES * 16 < end) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc = __builtin_amdgcn_mfma_f64_16x16x4f64((double)u[h][e], (double)u[h][e], acc, 0, 0, 0);
+        }
+    }
+  });
 #pragma unroll
   for (int r = 0; r < 4; ++r) lds[wave * 256 + (r * 4 + (lane >> 4)) * 16 + (lane & 15)] = acc[r];
   __syncthreads();
@@ -1084,31 +1105,35 @@ __device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, cons
 #pragma unroll
   for (int r = 0; r < 4; ++r) P[r] = buf[c * kThinLd + 4 * r + q];
   const int end = t.n - chunk * kThinChunk < kThinChunk ? t.n : (chunk + 1) * kThinChunk;
-  for (int j0 = chunk * kThinChunk + wave * 16; j0 < end; j0 += WAVES * 16) {
-    f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-    const int j = j0 + c;
+  by_type(tab.gtype, [&](auto like) {
+    for (int j0 = chunk * kThinChunk + wave * 16; j0 < end; j0 += 4 * WAVES * 16) {
+      float u[4][4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int k = 4 * r + q;
-      float u = 0.f;
-      if (k < t.m && j < t.n) {
-        const size_t at = t.rows > t.cols ? (size_t)j * t.cols + k : (size_t)k * t.cols + j;
-        u = load_as(t.g, at, tab.gtype);
-        if (t.mom) u = tab.nesterov ? u + tab.mu * t.mom[at] : t.mom[at];
-      }
-      acc = __builtin_amdgcn_mfma_f64_16x16x4f64(P[r], (double)u, acc, 0, 0, 0);
-    }
+      for (int h = 0; h < 4; ++h)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 4 * r + q;
-      if (i < t.m && j < t.n) {
-        const size_t at = t.rows > t.cols ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
-        float o = (float)acc[r];
-        if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
-        store_as(t.w, at, tab.wtype, o);
+        for (int r = 0; r < 4; ++r)
+          u[h][r] = thin_u<decltype(like)>(tab, t, false, 4 * r + q, j0 + h * WAVES * 16 + c, end);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const int j = j0 + h * WAVES * 16 + c;
+        if (j - c >= end) break;
+        f64x4 acc = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc = __builtin_amdgcn_mfma_f64_16x16x4f64(P[r], (double)u[h][r], acc, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 4 * r + q;
+          if (i < t.m && j < end) {
+            const size_t at = thin_place(t, i, j);
+            float o = (float)acc[r];
+            if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
+            store_as(t.w, at, tab.wtype, o);
+          }
+        }
       }
     }
-  }
+  });
 }
 
 extern __shared__ __align__(16) char flowml_ns_lds[];
