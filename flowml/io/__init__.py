@@ -828,7 +828,10 @@ def _construct(cls, simple: str, rows, path: str, meta):
         ).get("layers")
         w = torch.from_numpy(vector_from_struct(rows[0]["weights"])).to(torch.float32)
         activation = meta.get("paramMap", {}).get("activation", "relu")
-        return cls(layers=[int(x) for x in layers], weights=w, activation=activation)
+        return cls(
+            layers=[int(x) for x in layers], weights=w, activation=activation,
+            layerNorm=bool(meta.get("paramMap", {}).get("layerNorm", False)),
+        )
     if simple == "RandomForestClassificationModel":
         trees = _trees_from_node_rows(rows, regression=False)
         n_classes = max(len(t.stats[0]) for t in trees)

@@ -570,14 +570,29 @@ def mlp_forward(
     bs: List[torch.Tensor],
     activation: str = "relu",
     out_dtype: torch.dtype = torch.float32,
+    norms: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None,
 ) -> torch.Tensor:
     """Forward pass: N×K logits (no softmax). Reference site: BLAS.gemm in
-    spark ml/ann AffineLayer."""
+    spark ml/ann AffineLayer.
+
+    ``norms``: (weight, bias) of a layer norm between each hidden layer's
+    product and its activation.
+    """
     h = X
     L = len(Ws)
+    _check_norms(norms, L)
     for i, (W, b) in enumerate(zip(Ws, bs)):
-        h = gemm_bias_act(h, W, b, "none" if i == L - 1 else activation)
+        if norms is None or i == L - 1:
+            h = gemm_bias_act(h, W, b, "none" if i == L - 1 else activation)
+        else:
+            h = gemm_bias_act(h, W, b, "none")
+            h = layer_norm(h, *norms[i], activation=activation)[0]
     return h.to(out_dtype)
+
+
+def _check_norms(norms, L: int) -> None:
+    if norms is not None and len(norms) != L - 1:
+        raise ValueError(f"norms must have one pair per hidden layer ({L - 1}), got {len(norms)}")
 
 
 def mlp_grad(
@@ -588,24 +603,38 @@ def mlp_grad(
     activation: str = "relu",
     w: Optional[torch.Tensor] = None,
     in_features: Optional[int] = None,
+    norms: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None,
 ):
     """Fused forward+backward for the softmax/cross-entropy MLP.
 
     Returns (loss_sum fp32, [gradW...], [gradB...]) — unnormalized partial
     sums over the local shard (caller all-reduces: SURVEY.md §2.5 C3).
     Reference sites: ANNGradient.compute / BreezeUtil.dgemm (K5-K7).
+
+    ``norms``: (weight, bias) of a layer norm between each hidden layer's
+    product and its activation; a fourth result then has the pairs' gradients.
     """
     L = len(Ws)
+    _check_norms(norms, L)
     acts = [X]
+    stats = []  # per hidden layer: the norm's input, mean and rstd
     h = X
     for i in range(L):
-        h = gemm_bias_act(h, Ws[i], bs[i], "none" if i == L - 1 else activation)
+        if norms is None or i == L - 1:
+            h = gemm_bias_act(h, Ws[i], bs[i], "none" if i == L - 1 else activation)
+        else:
+            z = gemm_bias_act(h, Ws[i], bs[i], "none")
+            h, mean, rstd = layer_norm(z, *norms[i], activation=activation)
+            stats.append((z, mean, rstd))
         acts.append(h)
     logits = acts[-1].to(torch.float32)
     loss, delta = softmax_xent_grad(logits, y, w)
     delta = delta.to(X.dtype)
     gWs: List[Optional[torch.Tensor]] = [None] * L
     gBs: List[Optional[torch.Tensor]] = [None] * L
+    gNs: List[Optional[Tuple[torch.Tensor, torch.Tensor]]] = [None] * (L - 1)
+    # with a norm the activation's derivative is its backward pass's
+    dgrad_act = activation if norms is None else "none"
     use_wgrad_kernel = (
         X.is_cuda and X.dtype == torch.bfloat16 and hip_available(X)
     )
@@ -639,14 +668,21 @@ def mlp_grad(
                     Wt = torch.nn.functional.pad(Wt, (0, Kp - out_i))
                 delta = get_ext().gemm_dgrad_act(
                     d_in.contiguous(), Wt.contiguous(), h_i.contiguous(),
-                    _act_code(activation))
+                    _act_code(dgrad_act))
             else:
                 dx = delta @ Ws[i]            # K7 dgrad (plain GEMM)
-                if activation == "relu":
-                    dact = (h_i > 0).to(dx.dtype)
+                if dgrad_act == "none":
+                    delta = dx
+                elif activation == "relu":
+                    delta = dx * (h_i > 0).to(dx.dtype)
                 else:
-                    dact = h_i * (1 - h_i)
-                delta = dx * dact
+                    delta = dx * (h_i * (1 - h_i))
+            if norms is not None:
+                delta, dgamma, dbeta = layer_norm_grad(
+                    delta, *stats[i - 1], norms[i - 1][0], y=h_i, activation=activation)
+                gNs[i - 1] = (dgamma, dbeta)
+    if norms is not None:
+        return loss, gWs, gBs, gNs
     return loss, gWs, gBs
 
 

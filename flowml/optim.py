@@ -1,4 +1,4 @@
-"""L-BFGS and OWL-QN batch optimizers.
+"""L-BFGS, OWL-QN and Muon batch optimizers.
 
 The reference stack drives training through breeze's LBFGS/OWLQN on the JVM
 driver (SURVEY.md §2.6 "breeze LBFGS/OWLQN"): LogisticRegression and the MLP
@@ -12,13 +12,20 @@ all-reduces the gradient, after which every rank takes the identical step
 ``owlqn``:  LBFGS on the smooth part + pseudo-gradient / orthant projection
 for the L1 term (only indices >= ``l1_start`` are penalized — Spark never
 regularizes intercepts).
+``Muon`` / ``muon``: momentum steps whose updates of weight matrices are
+orthogonalised (``ops.muon_update``): every direction of a matrix moves as far,
+not only the few that dominate its gradient. ``Muon`` steps a list of matrices
+in place; ``muon`` minimizes an objective of a flat vector, with Adam on what
+is no matrix (biases, norm weights).
 """
 
 from __future__ import annotations
 
-from typing import Callable, List, Tuple
+from typing import Callable, List, Sequence, Tuple
 
 import torch
+
+from flowml import ops
 
 FnGrad = Callable[[torch.Tensor], Tuple[float, torch.Tensor]]
 
@@ -247,3 +254,87 @@ def _pseudo_gradient(x: torch.Tensor, g: torch.Tensor, l1: torch.Tensor) -> torc
         ),
     )
     return pg
+
+
+# ---------------------------------------------------------------------------
+# Muon
+# ---------------------------------------------------------------------------
+
+
+class Muon:
+    """Orthogonalised momentum steps on a list of weight matrices, in place.
+
+    ``step(grads)`` is one ``ops.muon_update`` on all of them; the fp32 momentum
+    lives in ``buffers`` (assign or copy them to resume). The matrices may be
+    views into one flat vector, as long as each is contiguous.
+    """
+
+    def __init__(
+        self,
+        weights: Sequence[torch.Tensor],
+        lr: float = 0.02,
+        momentum: float = 0.95,
+        weight_decay: float = 0.0,
+        nesterov: bool = True,
+        steps: int = 5,
+    ):
+        self.weights = list(weights)
+        self.buffers = [
+            torch.zeros(w.shape, dtype=torch.float32, device=w.device) for w in self.weights
+        ]
+        self.lr = lr
+        self.momentum = momentum
+        self.weight_decay = weight_decay
+        self.nesterov = nesterov
+        self.steps = steps
+
+    def step(self, grads: Sequence[torch.Tensor]) -> None:
+        ops.muon_update(
+            self.weights, grads, self.buffers, lr=self.lr, momentum=self.momentum,
+            weight_decay=self.weight_decay, nesterov=self.nesterov, steps=self.steps,
+        )
+
+
+def muon(
+    f_grad: FnGrad,
+    x0: torch.Tensor,
+    matrices: Sequence[Tuple[int, int, int]],
+    max_iter: int = 100,
+    lr: float = 0.02,
+    momentum: float = 0.95,
+    tol: float = 1e-6,
+) -> Tuple[torch.Tensor, List[float]]:
+    """Minimize f with Muon on parts of x, Adam on the others.
+
+    ``matrices``: (offset, rows, cols) of each weight matrix in the flat x,
+    apart from each other. Both kinds take steps of about 0.2·lr (Muon) and lr
+    (Adam) per value. Returns (x, objective_history) like ``lbfgs``; ends early
+    when f changes by less than ``tol``, relatively.
+    """
+    x = x0.clone()
+    rest = torch.ones(x.numel(), dtype=torch.bool)
+    for off, r, c in matrices:
+        if off < 0 or off + r * c > x.numel() or not bool(rest[off : off + r * c].all()):
+            raise ValueError(f"matrix {r}x{c} at {off} lies outside x or over another")
+        rest[off : off + r * c] = False
+    rest = rest.nonzero().flatten().to(x.device)
+
+    def parts(v: torch.Tensor) -> List[torch.Tensor]:
+        return [v[off : off + r * c].view(r, c) for off, r, c in matrices]
+
+    opt = Muon(parts(x), lr=lr, momentum=momentum)
+    m1 = torch.zeros(rest.numel(), dtype=x.dtype, device=x.device)
+    m2 = torch.zeros_like(m1)
+    b1, b2, eps = 0.9, 0.999, 1e-8
+    history: List[float] = []
+    for t in range(1, max_iter + 1):
+        f, g = f_grad(x)
+        history.append(f)
+        if t > 1 and abs(history[-2] - f) / max(abs(history[-2]), abs(f), 1e-12) < tol:
+            break
+        opt.step(parts(g))
+        gr = g[rest]
+        m1.mul_(b1).add_(gr, alpha=1 - b1)
+        m2.mul_(b2).addcmul_(gr, gr, value=1 - b2)
+        x[rest] -= lr * (m1 / (1 - b1**t)) / ((m2 / (1 - b2**t)).sqrt() + eps)
+    return x, history
