@@ -43,31 +43,53 @@ struct Piece {
   typedef raw vec __attribute__((aligned(sizeof(T))));
 };
 
+// 0 behind the row's end
 template <typename T>
-__device__ __forceinline__ void load_piece(const T* p, int left, float* v) {
+__device__ __forceinline__ typename Piece<T>::raw load_raw(const T* p, int left) {
   constexpr int VEC = Piece<T>::VEC;
-  if (left >= VEC) {
-    const typename Piece<T>::raw r = *reinterpret_cast<const typename Piece<T>::vec*>(p);
+  if (left >= VEC) return *reinterpret_cast<const typename Piece<T>::vec*>(p);
+  typename Piece<T>::raw r;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = (float)r[k];
-  } else {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) v[k] = k < left ? (float)p[k] : 0.f;
-  }
+  for (int k = 0; k < VEC; ++k) r[k] = k < left ? p[k] : (T)0.f;
+  return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void store_piece(T* p, int left, const float* v) {
+__device__ __forceinline__ void load_piece(const T* p, int left, float* v) {
+  const typename Piece<T>::raw r = load_raw<T>(p, left);
+#pragma unroll
+  for (int k = 0; k < Piece<T>::VEC; ++k) v[k] = (float)r[k];
+}
+
+// stream: past the caches, for results that do not fit them (1M x 128 bf16:
+// 95 us instead of 113; loads past the caches lose as much).
+template <typename T>
+__device__ __forceinline__ void store_piece(T* p, int left, const float* v, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
   if (left >= VEC) {
     typename Piece<T>::raw r;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) r[k] = (T)v[k];
-    *reinterpret_cast<typename Piece<T>::vec*>(p) = r;
+    if (stream)
+      __builtin_nontemporal_store(r, reinterpret_cast<typename Piece<T>::vec*>(p));
+    else
+      *reinterpret_cast<typename Piece<T>::vec*>(p) = r;
   } else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
       if (k < left) p[k] = (T)v[k];
+  }
+}
+
+// VEC weights of neighbouring columns; `none` for a missing vector or column
+template <int VEC>
+__device__ __forceinline__ void load_columns(const float* p, int c, int D, float none, float* v) {
+  if (p && c + VEC <= D) {
+#pragma unroll
+    for (int k = 0; k < VEC; k += 4) load_piece<float>(p + c + k, 4, v + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = (p && c + k < D) ? p[c + k] : none;
   }
 }
 
@@ -149,11 +171,13 @@ __device__ __forceinline__ float activate_grad(float dy, float y, int act) {
 // forward: LANES lanes x NV pieces hold a row
 // ---------------------------------------------------------------------------
 
+// The next row of a group is under way while this one is worked on: 32 waves
+// a CU with 16 bytes a lane are not quite enough to keep HBM busy.
 template <typename T, int LANES, int NV>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm(
     const T* __restrict__ X, long long ldx, const float* __restrict__ gamma,
     const float* __restrict__ beta, T* __restrict__ Y, float* __restrict__ mean,
-    float* __restrict__ rstd, long long N, int D, float eps, int act) {
+    float* __restrict__ rstd, long long N, int D, float eps, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
   constexpr int BLOCK = LANES > 256 ? LANES : 256;
   constexpr int GROUPS = BLOCK / LANES;
@@ -165,30 +189,35 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm(
   float g[NV][VEC], b[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * LANES + lane) * VEC;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      g[i][k] = (gamma && c + k < D) ? gamma[c + k] : 1.f;
-      b[i][k] = (beta && c + k < D) ? beta[c + k] : 0.f;
-    }
+    load_columns<VEC>(gamma, (i * LANES + lane) * VEC, D, 1.f, g[i]);
+    load_columns<VEC>(beta, (i * LANES + lane) * VEC, D, 0.f, b[i]);
   }
 
-  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < N;
-       row0 += (long long)gridDim.x * GROUPS) {
-    // lanes without a row of their own repeat the last one: the sums below
-    // need every lane of the wave
-    const bool live = row0 + group < N;
-    const long long row = live ? row0 + group : N - 1;
-    const T* x = X + row * ldx;
-    float v[NV][VEC];
-    float s = 0.f;
+  const long long stride = (long long)gridDim.x * GROUPS;
+  typename Piece<T>::raw raw[NV];
+  // lanes without a row of their own repeat the last one: the sums below need
+  // every lane of the wave
+  auto fetch = [&](long long row) {
+    const T* x = X + (row < N ? row : N - 1) * ldx;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * VEC;
-      load_piece<T>(x + c, D - c, v[i]);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) s += v[i][k];
+      raw[i] = load_raw<T>(x + c, D - c);
     }
+  };
+  fetch((long long)blockIdx.x * GROUPS + group);
+  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < N; row0 += stride) {
+    const long long row = row0 + group;
+    float v[NV][VEC];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        v[i][k] = (float)raw[i][k];
+        s += v[i][k];
+      }
+    if (row0 + stride < N) fetch(row + stride);
     const float mu = row_sum<LANES>(s, s_red[0]) / d;
     float q = 0.f;
 #pragma unroll
@@ -201,7 +230,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm(
       }
     }
     const float r = 1.f / sqrtf(row_sum<LANES>(q, s_red[1]) / d + eps);
-    if (live) {
+    if (row < N) {
       T* y = Y + row * D;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -210,7 +239,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm(
 #pragma unroll
           for (int k = 0; k < VEC; ++k)
             v[i][k] = activate(v[i][k] * r * g[i][k] + b[i][k], act);
-          store_piece<T>(y + c, D - c, v[i]);
+          store_piece<T>(y + c, D - c, v[i], stream);
         }
       }
       if (lane == 0) {
@@ -226,7 +255,7 @@ template <typename T>
 __global__ __launch_bounds__(1024) void flowml_layer_norm_long(
     const T* __restrict__ X, long long ldx, const float* __restrict__ gamma,
     const float* __restrict__ beta, T* __restrict__ Y, float* __restrict__ mean,
-    float* __restrict__ rstd, long long N, int D, float eps, int act) {
+    float* __restrict__ rstd, long long N, int D, float eps, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
   __shared__ float s_red[2][16];
   const float d = (float)D;
@@ -249,15 +278,13 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_long(
     const float r = 1.f / sqrtf(row_sum<1024>(q, s_red[1]) / d + eps);
     T* y = Y + row * D;
     for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
+      float g[VEC], b[VEC];
       load_piece<T>(x + c, D - c, v);
+      load_columns<VEC>(gamma, c, D, 1.f, g);
+      load_columns<VEC>(beta, c, D, 0.f, b);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const bool in = c + k < D;
-        const float g = (gamma && in) ? gamma[c + k] : 1.f;
-        const float b = (beta && in) ? beta[c + k] : 0.f;
-        v[k] = activate((v[k] - mu) * r * g + b, act);
-      }
-      store_piece<T>(y + c, D - c, v);
+      for (int k = 0; k < VEC; ++k) v[k] = activate((v[k] - mu) * r * g[k] + b[k], act);
+      store_piece<T>(y + c, D - c, v, stream);
     }
     if (threadIdx.x == 0) {
       mean[row] = mu;
@@ -275,7 +302,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm_g
     const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
     const T* __restrict__ Y, long long ldy, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ gamma,
-    T* __restrict__ dX, float* __restrict__ part, long long N, int D, int act) {
+    T* __restrict__ dX, float* __restrict__ part, long long N, int D, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
   constexpr int BLOCK = LANES > 256 ? LANES : 256;
   constexpr int GROUPS = BLOCK / LANES;
@@ -289,36 +316,45 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm_g
   float g[NV][VEC], dg[NV][VEC], db[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int c = (i * LANES + lane) * VEC;
+    load_columns<VEC>(gamma, (i * LANES + lane) * VEC, D, 1.f, g[i]);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      g[i][k] = (gamma && c + k < D) ? gamma[c + k] : 1.f;
-      dg[i][k] = db[i][k] = 0.f;
-    }
+    for (int k = 0; k < VEC; ++k) dg[i][k] = db[i][k] = 0.f;
   }
 
+  const long long stride = (long long)gridDim.x * GROUPS;
+  typename Piece<T>::raw rx[NV], rd[NV], ry[ACT ? NV : 1];
+  float next_mu, next_r;
+  auto fetch = [&](long long row) {
+    if (row >= N) row = N - 1;
+    next_mu = mean[row];
+    next_r = rstd[row];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * LANES + lane) * VEC;
+      rx[i] = load_raw<T>(X + row * ldx + c, D - c);
+      rd[i] = load_raw<T>(dY + row * lddy + c, D - c);
+      if constexpr (ACT) ry[i] = load_raw<T>(Y + row * ldy + c, D - c);
+    }
+  };
+  // with 16 values of four arrays to a lane, 128 registers do not hold two rows
+  constexpr bool AHEAD = LANES < 1024 || NV * VEC < 16;
+  if (AHEAD) fetch((long long)blockIdx.x * GROUPS + group);
   int turn = 0;  // the block-wide sums of two neighbouring rows use other words
-  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < N;
-       row0 += (long long)gridDim.x * GROUPS, turn ^= 1) {
-    const bool live = row0 + group < N;
-    const long long row = live ? row0 + group : N - 1;
-    const float mu = mean[row], r = rstd[row];
+  for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < N; row0 += stride, turn ^= 1) {
+    const long long row = row0 + group;
+    const bool live = row < N;
+    if (!AHEAD) fetch(row);
+    const float mu = next_mu, r = next_r;
     float xh[NV][VEC], dz[NV][VEC];
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * LANES + lane) * VEC;
-      load_piece<T>(X + row * ldx + c, D - c, xh[i]);
-      load_piece<T>(dY + row * lddy + c, D - c, dz[i]);
-      if constexpr (ACT) {
-        float y[VEC];
-        load_piece<T>(Y + row * ldy + c, D - c, y);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) dz[i][k] = activate_grad(dz[i][k], y[k], act);
-      }
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
-        xh[i][k] = (xh[i][k] - mu) * r;
+        dz[i][k] = (float)rd[i][k];
+        if constexpr (ACT) dz[i][k] = activate_grad(dz[i][k], (float)ry[i][k], act);
+        xh[i][k] = ((float)rx[i][k] - mu) * r;
         // past the row's end dz is 0, and with it p and both sums
         const float p = dz[i][k] * g[i][k];
         s += p;
@@ -329,6 +365,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm_g
         }
       }
     }
+    if (AHEAD && row0 + stride < N) fetch(row + stride);
     row_sum2<LANES>(s, q, s_red[turn]);
     s /= d;
     q /= d;
@@ -341,7 +378,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm_g
 #pragma unroll
           for (int k = 0; k < VEC; ++k)
             o[k] = r * (dz[i][k] * g[i][k] - s - xh[i][k] * q);
-          store_piece<T>(dX + row * D + c, D - c, o);
+          store_piece<T>(dX + row * D + c, D - c, o, stream);
         }
       }
     }
@@ -384,7 +421,7 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
     const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
     const T* __restrict__ Y, long long ldy, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ gamma,
-    T* __restrict__ dX, long long N, int D, int act) {
+    T* __restrict__ dX, long long N, int D, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
   __shared__ float s_red[2][32];
   const float d = (float)D;
@@ -394,15 +431,15 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
     float s = 0.f, q = 0.f;
     for (int look = 0; look < 2; ++look) {
       for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
-        float x[VEC], dz[VEC], y[VEC];
+        float x[VEC], dz[VEC], y[VEC], g[VEC];
+        load_columns<VEC>(gamma, c, D, 1.f, g);
         load_piece<T>(X + row * ldx + c, D - c, x);
         load_piece<T>(dY + row * lddy + c, D - c, dz);
         if (act) load_piece<T>(Y + row * ldy + c, D - c, y);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
           const bool in = c + k < D;
-          const float p = (act ? activate_grad(dz[k], y[k], act) : dz[k]) *
-                          ((gamma && in) ? gamma[c + k] : 1.f);
+          const float p = (act ? activate_grad(dz[k], y[k], act) : dz[k]) * g[k];
           const float xh = (x[k] - mu) * r;
           if (look == 0) {
             s += p;
@@ -411,7 +448,7 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
             x[k] = r * (p - s - xh * q);
           }
         }
-        if (look) store_piece<T>(dX + row * D + c, D - c, x);
+        if (look) store_piece<T>(dX + row * D + c, D - c, x, stream);
       }
       if (look == 0) {
         row_sum2<1024>(s, q, s_red[turn]);
@@ -454,8 +491,17 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_slabs(
   const int c = blockIdx.x * 32 + (threadIdx.x & 31);
   const int run = threadIdx.x >> 5;
   float t = 0.f;
-  if (c < W)
-    for (int k = run; k < G; k += 32) t += part[(long long)k * W + c];
+  if (c < W) {
+    int k = run;
+    for (; k + 7 * 32 < G; k += 8 * 32) {  // eight loads under way
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = part[(long long)(k + e * 32) * W + c];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t += v[e];
+    }
+    for (; k < G; k += 32) t += part[(long long)k * W + c];
+  }
   s[run][threadIdx.x & 31] = t;
   __syncthreads();
   if (run == 0 && c < W) {
@@ -472,13 +518,31 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_slabs(
 
 constexpr int kCUs = 256;
 
-// lanes and pieces for a row of D values of VEC to the piece: one piece per
+// whether a result is too large for the 256 MB of last-level cache to be found
+// there by whoever reads it next
+bool streams(long long N, int D, size_t size) { return N * D * (long long)size > (128LL << 20); }
+
+// Lanes and pieces for a row of D values of VEC to the piece: one piece per
 // lane up to a wave, then more pieces, then more waves.
 struct Shape {
   int lanes, nv;
 };
 
-Shape shape_for(int D, int vec) {
+// Forward: the smallest block whose lanes hold the row in 16 values each (with
+// as many weights and biases), for a CU then works on several rows and their
+// barriers do not meet.
+Shape forward_shape(int D, int vec) {
+  const int pieces = (D + vec - 1) / vec;
+  for (int l = 1; l <= 64; l *= 2)
+    if (pieces <= l) return {l, 1};
+  if (pieces <= 128) return {64, 2};
+  for (int l = 256; l <= 1024; l *= 2)
+    for (int v = 1; v <= 16 / vec; ++v)
+      if (pieces <= l * v) return {l, v};
+  return {0, 0};
+}
+
+Shape backward_shape(int D, int vec) {
   const int pieces = (D + vec - 1) / vec;
   for (int l = 1; l <= 64; l *= 2)
     if (pieces <= l) return {l, 1};
@@ -496,21 +560,22 @@ int rows_per_block(Shape s) { return s.lanes > 256 ? 1 : 256 / s.lanes; }
 template <typename T>
 void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, float* mean,
              float* rstd, long long N, int D, float eps, int act, hipStream_t st) {
-  const Shape s = shape_for(D, Piece<T>::VEC);
+  const Shape s = forward_shape(D, Piece<T>::VEC);
+  const bool stream = streams(N, D, sizeof(T));
   if (!s.lanes) {
     const int grid = (int)(N < 2 * kCUs ? N : 2 * kCUs);
     hipLaunchKernelGGL((flowml_layer_norm_long<T>), dim3(grid), dim3(1024), 0, st, X, ldx, g, b, Y,
-                       mean, rstd, N, D, eps, act);
+                       mean, rstd, N, D, eps, act, stream);
     return;
   }
   const int rpb = rows_per_block(s);
   const long long want = (N + rpb - 1) / rpb;
-  const long long most = (long long)kCUs * 8;
+  const long long most = (long long)kCUs * (s.lanes > 64 ? 8 : 16);
   const int grid = (int)(want < most ? want : most);
 #define LN_CASE(L, V)                                                              \
   if (s.lanes == L && s.nv == V)                                                   \
     hipLaunchKernelGGL((flowml_layer_norm<T, L, V>), dim3(grid),                   \
-                       dim3(L > 256 ? L : 256), 0, st, X, ldx, g, b, Y, mean, rstd, N, D, eps, act)
+                       dim3(L > 256 ? L : 256), 0, st, X, ldx, g, b, Y, mean, rstd, N, D, eps, act, stream)
   LN_CASE(1, 1);
   LN_CASE(2, 1);
   LN_CASE(4, 1);
@@ -521,15 +586,22 @@ void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, fl
   LN_CASE(64, 2);
   LN_CASE(256, 1);
   LN_CASE(256, 2);
-  LN_CASE(1024, 1);
+  LN_CASE(512, 2);
   LN_CASE(1024, 2);
-  if constexpr (Piece<T>::VEC == 4) LN_CASE(1024, 4);
+  if constexpr (Piece<T>::VEC == 4) {
+    LN_CASE(256, 3);
+    LN_CASE(256, 4);
+    LN_CASE(512, 3);
+    LN_CASE(512, 4);
+    LN_CASE(1024, 3);
+    LN_CASE(1024, 4);
+  }
 #undef LN_CASE
 }
 
 // slabs (and blocks) of the backward pass
 int grad_slabs(long long N, int D, int vec) {
-  const Shape s = shape_for(D, vec);
+  const Shape s = backward_shape(D, vec);
   long long want, most;
   if (!s.lanes) {
     // columns kernel: 256 columns to a block, chunks of rows to fill the chip
@@ -548,19 +620,20 @@ template <typename T>
 void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y, long long ldy,
               const float* mean, const float* rstd, const float* g, T* dX, float* part,
               float* out, long long N, int D, int act, hipStream_t st) {
-  const Shape s = shape_for(D, Piece<T>::VEC);
+  const Shape s = backward_shape(D, Piece<T>::VEC);
+  const bool stream = streams(N, D, sizeof(T));
   const int slabs = N ? grad_slabs(N, D, Piece<T>::VEC) : 0;
   if (slabs && !s.lanes) {
     const int grid = (int)(N < 2 * kCUs ? N : 2 * kCUs);
     hipLaunchKernelGGL((flowml_layer_norm_grad_long<T>), dim3(grid), dim3(1024), 0, st, dY, lddy, X,
-                       ldx, Y, ldy, mean, rstd, g, dX, N, D, act);
+                       ldx, Y, ldy, mean, rstd, g, dX, N, D, act, stream);
     const long long chunk = (N + slabs - 1) / slabs;
     hipLaunchKernelGGL((flowml_layer_norm_grad_cols<T>), dim3((D + 255) / 256, slabs),
                        dim3(256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, part, N, D, chunk, act);
   } else if (slabs) {
 #define LN_CASE1(L, V, A)                                                               \
   hipLaunchKernelGGL((flowml_layer_norm_grad<T, L, V, A>), dim3(slabs),                 \
-                     dim3(L > 256 ? L : 256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act)
+                     dim3(L > 256 ? L : 256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act, stream)
 #define LN_CASE(L, V)                \
   if (s.lanes == L && s.nv == V) {   \
     if (act)                         \
