@@ -60,7 +60,7 @@ int layer_norm_grad_slabs(int, long long, int);
 void launch_layer_norm_grad(int, const void*, long long, const void*,
                             long long, const void*, long long, const float*,
                             const float*, const float*, void*, float*, float*,
-                            long long, int, int, void*);
+                            float*, long long, int, int, void*);
 long long muon_workspace(int, const int*, const int*, int*);
 void launch_muon(int, const int*, const int*, const void* const*, float* const*,
                  void* const*, const float*, int, int, float, float, float, int,
@@ -491,16 +491,17 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_grad(
   const float* g = opt_columns(weight, X, "weight");
   const auto f32 = X.options().dtype(torch::kFloat32);
   auto dX = torch::empty({N, D}, X.options());
-  auto out = torch::empty({2, D}, f32);
+  auto dW = torch::empty({D}, f32);
+  auto dB = torch::empty({D}, f32);
   auto part = torch::empty({layer_norm_grad_slabs(type, N, D), 2, D}, f32);
   launch_layer_norm_grad(type, dY.data_ptr(), dY.stride(0), X.data_ptr(),
                          X.stride(0), act ? Y->data_ptr() : nullptr,
                          act ? Y->stride(0) : 0, mean.data_ptr<float>(),
                          rstd.data_ptr<float>(), g, dX.data_ptr(),
-                         part.data_ptr<float>(), out.data_ptr<float>(), N, D,
-                         (int)act, cur_stream());
+                         part.data_ptr<float>(), dW.data_ptr<float>(),
+                         dB.data_ptr<float>(), N, D, (int)act, cur_stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {dX, out[0], out[1]};
+  return {dX, dW, dB};
 }
 
 // ---- Newton-Schulz and the optimiser step ------------------------------------

@@ -117,6 +117,10 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
+// Threads of a block whose rows take `lanes` lanes: one row, or what four waves
+// hold.
+constexpr int block_of(int lanes) { return lanes > 64 ? lanes : 256; }
+
 // Sum over the lanes that share a row: part of a wave, or the whole block.
 // `lds`: LANES / 64 floats that no wave still reads (callers alternate).
 template <int LANES>
@@ -174,12 +178,12 @@ __device__ __forceinline__ float activate_grad(float dy, float y, int act) {
 // The next row of a group is under way while this one is worked on: 32 waves
 // a CU with 16 bytes a lane are not quite enough to keep HBM busy.
 template <typename T, int LANES, int NV>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm(
+__global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm(
     const T* __restrict__ X, long long ldx, const float* __restrict__ gamma,
     const float* __restrict__ beta, T* __restrict__ Y, float* __restrict__ mean,
     float* __restrict__ rstd, long long N, int D, float eps, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
-  constexpr int BLOCK = LANES > 256 ? LANES : 256;
+  constexpr int BLOCK = block_of(LANES);
   constexpr int GROUPS = BLOCK / LANES;
   __shared__ float s_red[2][LANES > 64 ? LANES / 64 : 1];
   const int lane = threadIdx.x % LANES;
@@ -298,13 +302,13 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_long(
 // ---------------------------------------------------------------------------
 
 template <typename T, int LANES, int NV, bool ACT>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void flowml_layer_norm_grad(
+__global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
     const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
     const T* __restrict__ Y, long long ldy, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ gamma,
     T* __restrict__ dX, float* __restrict__ part, long long N, int D, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
-  constexpr int BLOCK = LANES > 256 ? LANES : 256;
+  constexpr int BLOCK = block_of(LANES);
   constexpr int GROUPS = BLOCK / LANES;
   constexpr int WIDTH = LANES * NV * VEC;
   __shared__ float s_red[2][LANES > 64 ? LANES / 32 : 1];
@@ -483,11 +487,12 @@ __global__ __launch_bounds__(256) void flowml_layer_norm_grad_cols(
   slab[D + c] = db;
 }
 
-// out[c] = sum of part[s][c] over the slabs, in an order that G alone sets:
+// dg[c], db[c]: sums of part[s][0][c] and part[s][1][c] over the slabs, in an order that G alone sets:
 // 32 columns x 32 runs of slabs per block.
 __global__ __launch_bounds__(1024) void flowml_layer_norm_slabs(
-    const float* __restrict__ part, float* __restrict__ out, int G, int W) {
+    const float* __restrict__ part, float* __restrict__ dg, float* __restrict__ db, int G, int D) {
   __shared__ float s[32][33];
+  const int W = 2 * D;
   const int c = blockIdx.x * 32 + (threadIdx.x & 31);
   const int run = threadIdx.x >> 5;
   float t = 0.f;
@@ -508,7 +513,10 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_slabs(
     float u = 0.f;
 #pragma unroll
     for (int k = 0; k < 32; ++k) u += s[k][threadIdx.x];
-    out[c] = u;
+    if (c < D)
+      dg[c] = u;
+    else
+      db[c - D] = u;
   }
 }
 
@@ -542,20 +550,23 @@ Shape forward_shape(int D, int vec) {
   return {0, 0};
 }
 
+// Backward: one piece to a lane as far as a block goes, for four arrays and two
+// sums of columns live in registers (16384 x 4096 bf16: 105 us with two pieces
+// to 256 lanes, 92 with one to 512) -- but two to a wave before two waves share
+// a row (100000 x 1000 bf16: 213 us, with 128 lanes 269).
 Shape backward_shape(int D, int vec) {
   const int pieces = (D + vec - 1) / vec;
   for (int l = 1; l <= 64; l *= 2)
     if (pieces <= l) return {l, 1};
   if (pieces <= 128) return {64, 2};
-  if (pieces <= 256) return {256, 1};
-  if (pieces <= 512) return {256, 2};
-  if (pieces <= 1024) return {1024, 1};
-  if (pieces <= 2048) return {1024, 2};
-  if (vec == 4 && pieces <= 4096) return {1024, 4};
+  for (int l = 256; l <= 1024; l *= 2)
+    if (pieces <= l) return {l, 1};
+  for (int v = 2; v <= 16 / vec; v *= 2)
+    if (pieces <= 1024 * v) return {1024, v};
   return {0, 0};
 }
 
-int rows_per_block(Shape s) { return s.lanes > 256 ? 1 : 256 / s.lanes; }
+int rows_per_block(Shape s) { return block_of(s.lanes) / s.lanes; }
 
 template <typename T>
 void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, float* mean,
@@ -575,7 +586,7 @@ void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, fl
 #define LN_CASE(L, V)                                                              \
   if (s.lanes == L && s.nv == V)                                                   \
     hipLaunchKernelGGL((flowml_layer_norm<T, L, V>), dim3(grid),                   \
-                       dim3(L > 256 ? L : 256), 0, st, X, ldx, g, b, Y, mean, rstd, N, D, eps, act, stream)
+                       dim3(block_of(L)), 0, st, X, ldx, g, b, Y, mean, rstd, N, D, eps, act, stream)
   LN_CASE(1, 1);
   LN_CASE(2, 1);
   LN_CASE(4, 1);
@@ -611,7 +622,7 @@ int grad_slabs(long long N, int D, int vec) {
   } else {
     const int rpb = rows_per_block(s);
     want = (N + rpb - 1) / rpb;
-    most = s.lanes > 256 ? kCUs : 4 * kCUs;
+    most = kCUs * (s.lanes == 1024 ? 1 : s.lanes == 512 ? 2 : 4);
   }
   return (int)(want < most ? want : most);
 }
@@ -619,7 +630,7 @@ int grad_slabs(long long N, int D, int vec) {
 template <typename T>
 void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y, long long ldy,
               const float* mean, const float* rstd, const float* g, T* dX, float* part,
-              float* out, long long N, int D, int act, hipStream_t st) {
+              float* dg, float* db, long long N, int D, int act, hipStream_t st) {
   const Shape s = backward_shape(D, Piece<T>::VEC);
   const bool stream = streams(N, D, sizeof(T));
   const int slabs = N ? grad_slabs(N, D, Piece<T>::VEC) : 0;
@@ -633,7 +644,7 @@ void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y
   } else if (slabs) {
 #define LN_CASE1(L, V, A)                                                               \
   hipLaunchKernelGGL((flowml_layer_norm_grad<T, L, V, A>), dim3(slabs),                 \
-                     dim3(L > 256 ? L : 256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act, stream)
+                     dim3(block_of(L)), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act, stream)
 #define LN_CASE(L, V)                \
   if (s.lanes == L && s.nv == V) {   \
     if (act)                         \
@@ -650,7 +661,7 @@ void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y
     LN_CASE(64, 1);
     LN_CASE(64, 2);
     LN_CASE(256, 1);
-    LN_CASE(256, 2);
+    LN_CASE(512, 1);
     LN_CASE(1024, 1);
     LN_CASE(1024, 2);
     if constexpr (Piece<T>::VEC == 4) LN_CASE(1024, 4);
@@ -658,7 +669,7 @@ void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y
 #undef LN_CASE1
   }
   hipLaunchKernelGGL(flowml_layer_norm_slabs, dim3((2 * D + 31) / 32), dim3(1024), 0, st,
-                     part, out, slabs, 2 * D);
+                     part, dg, db, slabs, D);
 }
 
 }  // namespace
@@ -687,16 +698,16 @@ extern "C" int layer_norm_grad_slabs(int type, long long N, int D) {
 extern "C" void launch_layer_norm_grad(int type, const void* dY, long long lddy, const void* X,
                                        long long ldx, const void* Y, long long ldy,
                                        const float* mean, const float* rstd, const float* g,
-                                       void* dX, float* part, float* out, long long N, int D,
-                                       int act, void* stream) {
+                                       void* dX, float* part, float* dg, float* db, long long N,
+                                       int D, int act, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   if (type == T_F32)
     backward((const float*)dY, lddy, (const float*)X, ldx, (const float*)Y, ldy, mean, rstd, g,
-             (float*)dX, part, out, N, D, act, st);
+             (float*)dX, part, dg, db, N, D, act, st);
   else if (type == T_BF16)
     backward((const __bf16*)dY, lddy, (const __bf16*)X, ldx, (const __bf16*)Y, ldy, mean, rstd, g,
-             (__bf16*)dX, part, out, N, D, act, st);
+             (__bf16*)dX, part, dg, db, N, D, act, st);
   else
     backward((const _Float16*)dY, lddy, (const _Float16*)X, ldx, (const _Float16*)Y, ldy, mean,
-             rstd, g, (_Float16*)dX, part, out, N, D, act, st);
+             rstd, g, (_Float16*)dX, part, dg, db, N, D, act, st);
 }

@@ -561,7 +561,7 @@ def _act(h: torch.Tensor, activation: str) -> torch.Tensor:
 
 
 def _act_code(activation: str) -> int:
-    return {"none": 0, "relu": 1, "sigmoid": 2}[activation]
+    return _ACT_CODES[activation]
 
 
 def mlp_forward(
@@ -690,7 +690,13 @@ def mlp_grad(
 # Layer norm with a fused activation
 # ---------------------------------------------------------------------------
 
+_ACT_CODES = {"none": 0, "relu": 1, "sigmoid": 2}
 _NORM_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _unit_columns(t: torch.Tensor) -> torch.Tensor:
+    # any distance between rows is taken as it is, an expanded row (0) too
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
 def _norm_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
@@ -699,27 +705,29 @@ def _norm_rows(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
         raise ValueError(f"{name} must be N×D like X, got {tuple(t.shape)}")
     if t.dtype != like.dtype or t.device != like.device:
         raise ValueError(f"{name} must have X's type and device")
-    # any distance between rows is taken as it is, an expanded row (0) too
-    return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+    return _unit_columns(t)
 
 
 def _norm_columns(t: Optional[torch.Tensor], X: torch.Tensor, name: str):
     if t is None:
         return None
-    if t.shape != (X.shape[1],):
+    if t.dim() != 1 or t.shape[0] != X.shape[1]:
         raise ValueError(f"{name} must have one value per column, got {tuple(t.shape)}")
     if t.device != X.device:
         raise ValueError(f"{name} must be on X's device")
-    return t.to(torch.float32).contiguous()
+    if t.dtype is not torch.float32:
+        t = t.to(torch.float32)
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _check_norm(X: torch.Tensor, activation: str) -> None:
+def _check_norm(X: torch.Tensor, activation: str) -> int:
     if X.dim() != 2 or X.shape[1] < 1:
         raise ValueError(f"layer norm takes N×D with D >= 1, got {tuple(X.shape)}")
     if X.dtype not in _NORM_TYPES:
         raise ValueError(f"layer norm takes f32, bf16 or f16, got {X.dtype}")
-    if activation not in ("none", "relu", "sigmoid"):
+    if activation not in _ACT_CODES:
         raise ValueError(f"Unsupported activation {activation!r}")
+    return _ACT_CODES[activation]
 
 
 def layer_norm(
@@ -734,12 +742,12 @@ def layer_norm(
     are what ``layer_norm_grad`` takes. rstd = 1/√(var + eps), var over D.
     Rows may lie any distance apart; N = 0 gives empty results.
     """
-    _check_norm(X, activation)
-    X = _norm_rows(X, X, "X")
+    act = _check_norm(X, activation)
+    X = _unit_columns(X)
     weight = _norm_columns(weight, X, "weight")
     bias = _norm_columns(bias, X, "bias")
     if hip_available(X):
-        return get_ext().layer_norm(X, weight, bias, float(eps), _act_code(activation))
+        return get_ext().layer_norm(X, weight, bias, eps, act)
     x = X.to(torch.float32)
     mean = x.mean(dim=1)
     x = x - mean.unsqueeze(1)
@@ -768,8 +776,8 @@ def layer_norm_grad(
     are sums over the local rows in a fixed order (two runs agree bit for bit);
     they are given for a missing weight or bias too. N = 0 gives zeros.
     """
-    _check_norm(X, activation)
-    X = _norm_rows(X, X, "X")
+    act = _check_norm(X, activation)
+    X = _unit_columns(X)
     dY = _norm_rows(dY, X, "dY")
     if activation == "none":
         y = None
@@ -779,11 +787,11 @@ def layer_norm_grad(
         y = _norm_rows(y, X, "y")
     weight = _norm_columns(weight, X, "weight")
     for name, t in (("mean", mean), ("rstd", rstd)):
-        if t.shape != (X.shape[0],) or t.dtype != torch.float32 or t.device != X.device:
+        if t.dim() != 1 or len(t) != len(X) or t.dtype != torch.float32 or t.device != X.device:
             raise ValueError(f"{name} must be one f32 per row on X's device")
     if hip_available(X):
         return get_ext().layer_norm_grad(
-            dY, X, mean.contiguous(), rstd.contiguous(), weight, y, _act_code(activation)
+            dY, X, mean.contiguous(), rstd.contiguous(), weight, y, act
         )
     xh = (X.to(torch.float32) - mean.unsqueeze(1)) * rstd.unsqueeze(1)
     dz = dY.to(torch.float32)
