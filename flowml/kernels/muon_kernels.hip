@@ -62,7 +62,8 @@ struct Mat {
   int m, n;        // shorter and longer side
   int mp, np;      // padded to whole tiles of B X
   int ma;          // m padded to whole tiles of A as well
-  int parts;       // sums of squares
+  int parts;       // sums of squares, or chunks of a thin matrix
+  int chunk;       // its columns to a block
   int rows, cols;  // as the caller has it
   int full;        // 1: three products everywhere
   float step;
@@ -477,6 +478,27 @@ __device__ __forceinline__ void deliver(const Table& tab, const Mat& t, int row,
 constexpr int kPieceLd = 36;                  // floats from row to row of a piece in LDS
 constexpr int kPieceHalfs = 32 * kPieceLd * 2;
 
+// The old values of a piece, 8 to a lane, twice, from the copy in which i runs
+// along rows.
+struct Old {
+  f16x8 hi[2], lo[2];
+};
+
+template <int TO>
+__device__ __forceinline__ Old load_old(const Mat& t, int turn, int i0, int j0) {
+  const int lane = threadIdx.x & 63, r4 = lane >> 2, c8 = (lane & 3) * 8;
+  Old o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const size_t at = place(TO == TO_B ? t.ma : t.np, j0 + h * 16 + r4, i0 + c8);
+    o.hi[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 0) : ws_xt(t, turn, 0)) + at);
+    o.lo[h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    if (TO != TO_B || t.full)
+      o.lo[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 1) : ws_xt(t, turn, 1)) + at);
+  }
+  return o;
+}
+
 // The 32 x 32 piece at (i0, j0) of A, B, X' or the result: ka * (old value) +
 // kb * (product).  A lane holds 4 neighbouring rows of a column, 4 times; the
 // piece goes through the wave's own LDS so that every global access is 16
@@ -485,25 +507,14 @@ constexpr int kPieceHalfs = 32 * kPieceLd * 2;
 // 360 at 256 x 256.)
 template <int TO>
 __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn, float ka, float kb,
-                                       int i0, int j0, bool mirror, const f32x16& acc, float* lds) {
+                                       int i0, int j0, bool mirror, const f32x16& acc,
+                                       const Old& old, float* lds) {
   const int lane = threadIdx.x & 63;
   const bool turned = t.rows > t.cols;
   f16* ch = TO == TO_A ? ws_a(t, 0) : TO == TO_B ? ws_b(t, 0) : ws_xt(t, turn ^ 1, 0);
   f16* cl = TO == TO_A ? ws_a(t, 1) : TO == TO_B ? ws_b(t, 1) : ws_xt(t, turn ^ 1, 1);
   const int r4 = lane >> 2, c8 = (lane & 3) * 8;
   const int rows_j = TO == TO_A || TO == TO_B ? t.ma : t.np;  // of a plane whose rows are columns j
-  // the old values, from the copy in which i runs along rows
-  f16x8 oh[2], ol[2];
-  if (TO != TO_A) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const size_t at = place(rows_j, j0 + h * 16 + r4, i0 + c8);
-      oh[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 0) : ws_xt(t, turn, 0)) + at);
-      ol[h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      if (TO != TO_B || t.full)
-        ol[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 1) : ws_xt(t, turn, 1)) + at);
-    }
-  }
 #pragma unroll
   for (int q = 0; q < 4; ++q)
     *(float4*)(lds + (lane & 31) * kPieceLd + q * 8 + (lane >> 5) * 4) =
@@ -517,7 +528,7 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
     float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     if (TO != TO_A) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += ka * ((float)oh[h][k] + (float)ol[h][k]);
+      for (int k = 0; k < 8; ++k) v[k] += ka * ((float)old.hi[h][k] + (float)old.lo[h][k]);
     }
     if (TO == TO_END) {
       if (turned) {
@@ -677,11 +688,20 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   block_barrier();
   float* piece = (float*)(lds + wave * kPieceHalfs);
   const int wi = i0 + (wave / T::WN) * (T::TM / T::WM), wj = j0 + (wave % T::WN) * (T::TN / T::WN);
+  // a piece's old values are under way while the piece before it is finished
+  Old old = {}, next = {};
+  if (TO != TO_A) old = load_old<TO>(t, turn, wi, wj);
 #pragma unroll
   for (int f = 0; f < T::FM; ++f)
 #pragma unroll
-    for (int g = 0; g < T::FN; ++g)
-      finish<TO>(tab, t, turn, ka, kb, wi + f * 32, wj + g * 32, mirror, acc[f][g], piece);
+    for (int g = 0; g < T::FN; ++g) {
+      const int p = f * T::FN + g + 1;
+      if (TO != TO_A && p < T::FM * T::FN)
+        next = load_old<TO>(t, turn, wi + p / T::FN * 32, wj + p % T::FN * 32);
+      finish<TO>(tab, t, turn, ka, kb, wi + f * 32, wj + g * 32, mirror, acc[f][g], old, piece);
+      old = next;
+      __builtin_amdgcn_sched_barrier(0);
+    }
 }
 
 // ---- matrices that one block holds ----------------------------------------------
@@ -957,12 +977,12 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
 //   Q = a I + b A + c A^2     P <- Q P     A <- Q A Q      O = P U / |U|
 //
 // on 16 x 16 matrices.  A squares the condition of U, which 64 bits bear (in
-// fp32 this form is 10 to 100 times less exact than the other).  Matrices of
-// more than kThinChunk columns take a block for every kThinChunk; the sums of
-// A_0 are then made by a launch of their own, and every block iterates for
-// itself.
+// fp32 this form is 10 to 100 times less exact than the other).  Longer ones
+// take a block for every 256 columns or more, 64 blocks at most; the sums of
+// A_0 are then made by a launch of their own, and every block adds them and
+// iterates for itself.  (5 x 1024: one block 15 us, four CCC.)
 
-constexpr int kThinM = 16, kThinChunk = 1024, kThinLd = 17;
+constexpr int kThinM = 16, kThinLd = 17;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // Place of (i, j) in the caller's matrix, i on its shorter side.
@@ -1006,9 +1026,9 @@ __device__ __forceinline__ void thin_gram(const Table& tab, const Mat& t, int ch
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int WAVES = kSmallWaves;
   f64x4 acc = {0.0, 0.0, 0.0, 0.0};
-  const int end = t.n - chunk * kThinChunk < kThinChunk ? t.n : (chunk + 1) * kThinChunk;
+  const int end = t.n - chunk * t.chunk < t.chunk ? t.n : (chunk + 1) * t.chunk;
   by_type(tab.gtype, [&](auto like) {
-    for (int j = chunk * kThinChunk + wave * 16; j < end; j += 4 * WAVES * 16) {
+    for (int j = chunk * t.chunk + wave * 16; j < end; j += 4 * WAVES * 16) {
       float u[4][4];
 #pragma unroll
       for (int h = 0; h < 4; ++h)
@@ -1104,9 +1124,9 @@ __device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, cons
   f64x4 P;
 #pragma unroll
   for (int r = 0; r < 4; ++r) P[r] = buf[c * kThinLd + 4 * r + q];
-  const int end = t.n - chunk * kThinChunk < kThinChunk ? t.n : (chunk + 1) * kThinChunk;
+  const int end = t.n - chunk * t.chunk < t.chunk ? t.n : (chunk + 1) * t.chunk;
   by_type(tab.gtype, [&](auto like) {
-    for (int j0 = chunk * kThinChunk + wave * 16; j0 < end; j0 += 4 * WAVES * 16) {
+    for (int j0 = chunk * t.chunk + wave * 16; j0 < end; j0 += 4 * WAVES * 16) {
       float u[4][4];
 #pragma unroll
       for (int h = 0; h < 4; ++h)
@@ -1247,8 +1267,14 @@ void ways(int count, const int* rows, const int* cols, int* way) {
       if (way[k] == SMALL) way[k] = LARGE;
 }
 
+// columns of a thin matrix to a block
+int thin_chunk(int n) {
+  const int c = (n + 63) / 64;
+  return c < 256 ? 256 : c;
+}
+
 size_t thin_bytes(int rows, int cols) {
-  const int n = rows < cols ? cols : rows, chunks = (n + kThinChunk - 1) / kThinChunk;
+  const int n = rows < cols ? cols : rows, c = thin_chunk(n), chunks = (n + c - 1) / c;
   return chunks > 1 ? (size_t)chunks * 256 * sizeof(double) : 0;
 }
 
@@ -1347,7 +1373,8 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
       t.first = blocks;
       t.parts = 1;
       if (t.m <= kThinM) {
-        t.parts = (t.n + kThinChunk - 1) / kThinChunk;
+        t.chunk = thin_chunk(t.n);
+        t.parts = (t.n + t.chunk - 1) / t.chunk;
         at += thin_bytes(t.rows, t.cols);
         chunks |= t.parts > 1;
       } else {
