@@ -61,7 +61,7 @@ void launch_layer_norm_grad(int, const void*, long long, const void*,
                             long long, const void*, long long, const float*,
                             const float*, const float*, void*, float*, float*,
                             float*, long long, int, int, void*);
-long long muon_workspace(int, const int*, const int*, int*);
+long long muon_workspace(int, const int*, const int*, int, int*);
 void launch_muon(int, const int*, const int*, const void* const*, float* const*,
                  void* const*, const float*, int, int, float, float, float, int,
                  int, const float*, float, int, void*, int*, void*);
@@ -552,16 +552,17 @@ static void muon_call(const std::vector<torch::Tensor>& g,
   }
   const float cf[3] = {(float)coef[0], (float)coef[1], (float)coef[2]};
   const int gtype = float_type(g[0]), wtype = float_type(w[0]);
+  // three products everywhere unless the result is rounded to bf16
+  const int full = wtype != 1;
   std::vector<int> scratch(3 * n);
   auto ws = torch::empty(
-      {muon_workspace((int)n, rows.data(), cols.data(), scratch.data())},
+      {muon_workspace((int)n, rows.data(), cols.data(), full, scratch.data())},
       g[0].options().dtype(torch::kUInt8));
-  // three products everywhere unless the result is rounded to bf16
   launch_muon((int)n, rows.data(), cols.data(), gp.data(),
               mom.empty() ? nullptr : mp.data(), wp.data(),
               mom.empty() ? nullptr : sp.data(), gtype, wtype, (float)mu,
               (float)keep, (float)eps, nesterov, (int)steps, cf,
-              (float)scale_b, wtype != 1, ws.data_ptr(), scratch.data(),
+              (float)scale_b, full, ws.data_ptr(), scratch.data(),
               cur_stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }

@@ -36,6 +36,8 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
 #include <math.h>
+
+#include <algorithm>
 #include <stdint.h>
 #include <type_traits>
 
@@ -68,6 +70,9 @@ struct Mat {
   int full;        // 1: three products everywhere
   float step;
   int first;       // first block of this matrix in a launch
+  int split;       // blocks to a tile of A, each with kpart of K
+  int kpart;
+  float* sums;     // their sums, tile by tile, if there are several
 };
 
 struct Table {
@@ -585,8 +590,8 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
 }
 
 // Blocks go round the 8 XCDs in turn, each with an L2 of its own.  Every XCD
-// takes a run of neighbouring tiles instead, and a run is about square, so
-// that its blocks share operands in their L2.
+// takes a run of neighbouring tiles of a matrix instead, and a run is about
+// square, so that its blocks share operands in their L2.
 __device__ __forceinline__ int xcd_order(int block, int blocks) {
   const int x = block & 7, each = blocks >> 3, more = blocks & 7;
   return x * each + (x < more ? x : more) + (block >> 3);
@@ -649,13 +654,21 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   constexpr int HALFS = most(most(lds_halfs<T, D22, 2, 2>(), T::WAVES * kPieceHalfs),
                              SYM ? lds_halfs<T, D11, 1, 1>() : lds_halfs<T, D12, 1, 2>());
   __shared__ __align__(16) f16 lds[HALFS];
-  const int block = xcd_order(blockIdx.x, gridDim.x);
-  const Mat& t = tab.mat[find(tab, block)];
-  int ti, tj;
-  if (SYM)
-    tile_of_triangle(block - t.first, t.ma / T::TM, ti, tj);
-  else
-    tile_of_grid(block - t.first, t.mp / T::TM, t.np / T::TN, ti, tj);
+  const Mat& t = tab.mat[find(tab, blockIdx.x)];
+  int ti, tj, tile, part = 0;
+  if (SYM) {
+    const int mt = t.ma / T::TM, tiles = mt * (mt + 1) / 2;
+    tile = xcd_order(blockIdx.x - t.first, tiles * (TO == TO_A ? t.split : 1));
+    if (TO == TO_A) {
+      part = tile / tiles;
+      tile -= part * tiles;
+    }
+    tile_of_triangle(tile, mt, ti, tj);
+  } else {
+    const int mt = t.mp / T::TM, nt = t.np / T::TN;
+    tile = xcd_order(blockIdx.x - t.first, mt * nt);
+    tile_of_grid(tile, mt, nt, ti, tj);
+  }
   const int i0 = ti * T::TM, j0 = tj * T::TN;
 
   const f16* P[2];
@@ -665,7 +678,17 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
     P[p] = (TO == TO_A ? ws_x(t, p) : TO == TO_B ? ws_a(t, p) : ws_b(t, p)) + i0 * 32;
     Q[p] = (TO == TO_A ? ws_x(t, p) : TO == TO_B ? ws_a(t, p) : ws_xt(t, turn, p)) + j0 * 32;
   }
-  const int K = TO == TO_A ? t.np : t.mp, rows_q = SYM ? t.ma : t.np;
+  int K = TO == TO_A ? t.np : t.mp;
+  const int rows_q = SYM ? t.ma : t.np;
+  if (TO == TO_A && t.split > 1) {
+    const int k0 = part * t.kpart;
+    K = K - k0 < t.kpart ? K - k0 : t.kpart;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      P[p] += (size_t)k0 * t.ma;
+      Q[p] += (size_t)k0 * t.ma;
+    }
+  }
 
   f32x16 acc[T::FM][T::FN];
 #pragma unroll
@@ -688,6 +711,22 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   block_barrier();
   float* piece = (float*)(lds + wave * kPieceHalfs);
   const int wi = i0 + (wave / T::WN) * (T::TM / T::WM), wj = j0 + (wave % T::WN) * (T::TN / T::WN);
+  if (TO == TO_A && t.split > 1) {
+    float* to = t.sums + ((size_t)part * ((t.ma / T::TM) * (t.ma / T::TM + 1) / 2) + tile) *
+                            (T::TM * T::TN);
+#pragma unroll
+    for (int f = 0; f < T::FM; ++f)
+#pragma unroll
+      for (int g = 0; g < T::FN; ++g) {
+        const int pi = (wi - i0) / 32 + f, pj = (wj - j0) / 32 + g;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *(float4*)(to + (pi * (T::TN / 32) + pj) * 1024 + q * 256 + lane * 4) =
+              make_float4(acc[f][g][q * 4], acc[f][g][q * 4 + 1], acc[f][g][q * 4 + 2],
+                          acc[f][g][q * 4 + 3]);
+      }
+    return;
+  }
   // a piece's old values are under way while the piece before it is finished
   Old old = {}, next = {};
   if (TO != TO_A) old = load_old<TO>(t, turn, wi, wj);
@@ -702,6 +741,36 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
       old = next;
       __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+// A from the sums of its parts of K, one 32 x 32 piece to a wave, parts in order.
+template <int T>
+__global__ __launch_bounds__(256) void flowml_ns_join(Table tab, float kb) {
+  __shared__ __align__(16) float lds[4 * 32 * kPieceLd];
+  constexpr int EACH = (T / 32) * (T / 32) / 4;  // blocks to a tile
+  const Mat& t = tab.mat[find(tab, blockIdx.x)];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int b = blockIdx.x - t.first, tile = b / EACH, piece = b % EACH * 4 + wave;
+  const int mt = t.ma / T, tiles = mt * (mt + 1) / 2;
+  int ti, tj;
+  tile_of_triangle(tile, mt, ti, tj);
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < t.split; ++s) {
+    const float* from = t.sums + ((size_t)s * tiles + tile) * (T * T) + piece * 1024 + lane * 4;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 v = *(const float4*)(from + q * 256);
+      acc[q * 4] += v.x;
+      acc[q * 4 + 1] += v.y;
+      acc[q * 4 + 2] += v.z;
+      acc[q * 4 + 3] += v.w;
+    }
+  }
+  finish<TO_A>(tab, t, 0, 0.f, kb, ti * T + piece / (T / 32) * 32, tj * T + piece % (T / 32) * 32,
+               ti != tj, acc, Old{}, lds + wave * 32 * kPieceLd);
 }
 
 // ---- matrices that one block holds ----------------------------------------------
@@ -980,7 +1049,7 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
 // fp32 this form is 10 to 100 times less exact than the other).  Longer ones
 // take a block for every 256 columns or more, 64 blocks at most; the sums of
 // A_0 are then made by a launch of their own, and every block adds them and
-// iterates for itself.  (5 x 1024: one block 15 us, four CCC.)
+// iterates for itself.  (5 x 1024: one block 15 us, four 14.)
 
 constexpr int kThinM = 16, kThinLd = 17;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -1176,41 +1245,103 @@ constexpr int kPerNormBlock = 8192;
 
 int pad(int v, int t) { return (v + t - 1) / t * t; }
 
-// Tile sides of a call's symmetric products (A and B) and of B X.  A tile of
-// 256 runs at 1300 TFLOP/s and one of 64 at 650, but tiles are worth their
-// size only if there are enough for the 256 CUs.  Measured, us a product:
-//   A of 1024 x 4096 x 2, full:  64 (272 tiles) 27      128 (72 tiles) 56
-//   A of 2048 x 4096, hi hi:     64 (528) 38   128 (136) 30   256 (36) 78
+// Tile sides of a call's products, and the parts of K of A.  A tile of 256 runs
+// at 1300 TFLOP/s and one of 64 at 650, but tiles are worth their size only if
+// there are enough for the 256 CUs.  Measured, us a product:
+//   A of 2048 x 4096, hi hi:     64 (528 tiles) 38   128 (136) 30   256 (36) 78
 //   A of 4096 x 4096, hi hi:     128 (528) 91  192 (253) 74   256 (136) 94
 //   B X of 1024 x 4096, full:    64 (1024) 36  128 (256) 29   256 (64) 62
+//   two of these:                128 (512) 75   128 x 256 (256) 66
 //   B X of 4096 x 4096:          128 (1024) 266               256 (256) 230
+// Where A has few tiles and a long K, blocks take parts of K and a launch more
+// joins them: two of 1024 x 4096, full, take 50 us as 272 tiles of 64, and
+// 32 + 6 us as 72 of 128 in 3 parts; all steps of 100 x 100000, 2800 and 377 us.
 struct Sides {
-  int sym, all;
+  int a, b, m, n;  // A, B, and B X along m and n
+  int kpart;       // K of A to a block
 };
 
-Sides sides_for(int count, const int* rows, const int* cols) {
-  auto tiles = [&](int t, bool sym) {
+int shorter(int r, int c) { return std::min(r, c); }
+int longer(int r, int c) { return std::max(r, c); }
+
+Sides sides_for(int count, const int* rows, const int* cols, bool full) {
+  auto tiles = [&](int ti, int tj) {
     long long sum = 0;
-    for (int k = 0; k < count; ++k) {
-      const long long a = ((rows[k] < cols[k] ? rows[k] : cols[k]) + t - 1) / t;
-      const long long b = ((rows[k] < cols[k] ? cols[k] : rows[k]) + t - 1) / t;
-      sum += sym ? a * (a + 1) / 2 : a * b;
-    }
+    for (int k = 0; k < count; ++k)
+      sum += (long long)(pad(shorter(rows[k], cols[k]), ti) / ti) *
+             (pad(longer(rows[k], cols[k]), tj) / tj);
     return sum;
   };
+  constexpr int ALL = 1 << 30;
   Sides s;
-  s.all = tiles(256, false) >= 200 ? 256 : tiles(128, false) >= 128 ? 128 : 64;
-  s.sym = tiles(256, true) >= 400   ? 256
-          : tiles(192, true) >= 200 ? 192
-          : tiles(128, true) >= 128 ? 128
+  // a larger side has to make good the padding of matrices that are low
+  const long long t64 = tiles(64, 64), t128 = tiles(128, 128), t256 = tiles(256, 256);
+  s.m = t256 >= 200 && 3 * t256 <= t128 ? 256 : t128 >= 128 && 8 * t128 <= 3 * t64 ? 128 : 64;
+  s.n = s.m == 128 && tiles(128, 256) >= 200 ? 256 : s.m;
+  // blocks of a symmetric product, and how many of them leave their sums
+  auto triangle = [&](int t, int kpart, long long* parts = nullptr) {
+    long long sum = 0, several = 0;
+    for (int k = 0; k < count; ++k) {
+      const long long a = pad(shorter(rows[k], cols[k]), t) / t;
+      const int n = pad(longer(rows[k], cols[k]), s.n), split = (n - 1) / kpart + 1;
+      sum += a * (a + 1) / 2 * split;
+      if (split > 1) several += a * (a + 1) / 2 * split;
+    }
+    if (parts) *parts = several;
+    return sum;
+  };
+  s.b = triangle(256, ALL) >= 400   ? 256
+        : triangle(192, ALL) >= 200 ? 192
+        : triangle(128, ALL) >= 128 ? 128
                                     : 64;
+  s.a = s.b;
+  s.kpart = ALL;
+  if (s.b == 64) {
+    int most = 0;
+    for (int k = 0; k < count; ++k) most = std::max(most, pad(longer(rows[k], cols[k]), s.n));
+    double best = 1e30;
+    for (int t = 64; t <= 128; t += 64)
+      for (int parts = 1; parts <= 64; ++parts) {
+        const int kpart = parts == 1 ? ALL : pad((most + parts - 1) / parts, 64);
+        if (parts > 1 && kpart < 256) break;
+        // us, fitted to the calls above: a CU's step of 64 in K (a few blocks of
+        // 64 x 64 share a CU and hide each other's waits), the tiles' ends, the
+        // sums' way out and in, and the joining launch
+        long long sums;
+        const long long rounds = (triangle(t, kpart, &sums) + 255) / 256;
+        if (parts > 1 && rounds > 2) break;  // no block more brings anything
+        const int steps = (std::min(kpart, most) + 63) / 64;
+        const double step = full ? rounds * (t == 64 ? 0.32 : 0.8)
+                                 : t == 64 ? std::max(0.27, rounds * 0.17) : rounds * 0.38;
+        const double us = steps * step + rounds +
+                          (sums ? 4.0 + 0.15 * parts + sums * t * t * 1.6e-6 : 0.0);
+        if (us < best) {
+          best = us;
+          s.a = t;
+          s.kpart = kpart;
+        }
+      }
+  }
   return s;
 }
 
-size_t bytes_of(int rows, int cols, Sides s) {
-  const size_t mp = pad(rows < cols ? rows : cols, s.all), np = pad(rows < cols ? cols : rows, s.all);
-  const size_t ma = pad(mp, s.sym);
-  return kNormBlocks * sizeof(double) + (2 * ma * np + 4 * np * mp + 4 * ma * ma) * sizeof(f16);
+struct Sizes {
+  int mp, np, ma, split;
+  size_t bytes;  // sums of squares and planes
+  size_t sums;   // floats of A's parts
+};
+
+Sizes sizes_of(int rows, int cols, Sides s) {
+  Sizes z;
+  z.mp = pad(shorter(rows, cols), s.m);
+  z.np = pad(longer(rows, cols), s.n);
+  z.ma = pad(z.mp, s.a);
+  if (s.b != s.a) z.ma = pad(z.ma, s.b);
+  z.split = s.kpart < z.np ? (z.np + s.kpart - 1) / s.kpart : 1;
+  const size_t mp = z.mp, np = z.np, ma = z.ma, mt = ma / s.a;
+  z.bytes = kNormBlocks * sizeof(double) + (2 * ma * np + 4 * np * mp + 4 * ma * ma) * sizeof(f16);
+  z.sums = z.split > 1 ? mt * (mt + 1) / 2 * s.a * s.a * z.split : 0;
+  return z;
 }
 
 // one product for all matrices of a table; `first` of each is set here
@@ -1221,28 +1352,52 @@ void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
     Mat& t = tab.mat[k];
     t.first = blocks;
     const int mt = t.ma / T::TM;
-    blocks += TO == TO_A || TO == TO_B ? mt * (mt + 1) / 2 : (t.mp / T::TM) * (t.np / T::TN);
+    blocks += TO == TO_A   ? mt * (mt + 1) / 2 * t.split
+              : TO == TO_B ? mt * (mt + 1) / 2
+                           : (t.mp / T::TM) * (t.np / T::TN);
   }
   hipLaunchKernelGGL((flowml_ns_product<T, D22, D11, D12, TO>), dim3(blocks), dim3(T::WAVES * 64),
                      0, st, tab, turn, ka, kb);
+}
+
+template <int T>
+void join(Table& tab, float kb, hipStream_t st) {
+  int blocks = 0;
+  for (int k = 0; k < tab.count; ++k) {
+    Mat& t = tab.mat[k];
+    t.first = blocks;
+    const int mt = t.ma / T;
+    if (t.split > 1) blocks += mt * (mt + 1) / 2 * ((T / 32) * (T / 32) / 4);
+  }
+  if (blocks)
+    hipLaunchKernelGGL((flowml_ns_join<T>), dim3(blocks), dim3(256), 0, st, tab, kb);
 }
 
 template <int TO>
 void product(Sides s, Table& tab, int turn, float ka, float kb, hipStream_t st) {
   // tile, waves, and the depth of LDS for two planes, hi hi, hi (hi + lo)
   if constexpr (TO == TO_A || TO == TO_B) {
-    if (s.sym == 256)
+    const int side = TO == TO_A ? s.a : s.b;
+    if (side == 256)
       product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
-    else if (s.sym == 192)
+    else if (side == 192)
       product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
-    else if (s.sym == 128)
+    else if (side == 128)
       product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
     else
       product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+    if (TO == TO_A && s.kpart < (1 << 30)) {
+      if (side == 128)
+        join<128>(tab, kb, st);
+      else
+        join<64>(tab, kb, st);
+    }
   } else {
-    if (s.all == 256)
+    if (s.m == 256)
       product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
-    else if (s.all == 128)
+    else if (s.n == 256)
+      product_of<Tile<128, 256, 2, 4>, Depth<32, 3>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+    else if (s.m == 128)
       product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
     else
       product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 2>, Depth<32, 5>, TO>(tab, turn, ka, kb, st);
@@ -1323,14 +1478,18 @@ int large_shapes(int count, const int* rows, const int* cols, const int* way, in
 // ---- host entry points ------------------------------------------------------------
 
 // workspace of a call, in bytes; `scratch`: 3 * count integers
-extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int* scratch) {
+extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int full,
+                                    int* scratch) {
   int *way = scratch, *r = scratch + count, *c = scratch + 2 * count;
   ways(count, rows, cols, way);
   const int n = large_shapes(count, rows, cols, way, r, c);
-  const Sides s = sides_for(n, r, c);
+  const Sides s = sides_for(n, r, c, full);
   size_t sum = 0;
   for (int k = 0; k < count; ++k) {
-    if (way[k] == LARGE) sum += bytes_of(rows[k], cols[k], s);
+    if (way[k] == LARGE) {
+      const Sizes z = sizes_of(rows[k], cols[k], s);
+      sum += z.bytes + z.sums * sizeof(float);
+    }
     if (way[k] == THIN) sum += thin_bytes(rows[k], cols[k]);
   }
   return (long long)sum;
@@ -1349,7 +1508,7 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
   int* way = scratch;
   ways(count, rows, cols, way);
   const int n = large_shapes(count, rows, cols, way, scratch + count, scratch + 2 * count);
-  const Sides sides = sides_for(n, scratch + count, scratch + 2 * count);
+  const Sides sides = sides_for(n, scratch + count, scratch + 2 * count, full);
   const Call call = {count, rows, cols, g, mom, w, step};
   const float sa = kScaleA, sx = kScaleX, sb = scale_b;
   Table tab;
@@ -1392,15 +1551,23 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
   for (int k0 = 0; k0 < count;) {
     k0 = gather(tab, call, way, true, k0);
     if (!tab.count) break;
+    // the largest first: what a launch's last blocks do is then little
+    std::stable_sort(tab.mat, tab.mat + tab.count, [](const Mat& x, const Mat& y) {
+      return (double)x.m * x.n > (double)y.m * y.n;
+    });
     int blocks = 0;
     for (int k = 0; k < tab.count; ++k) {
       Mat& t = tab.mat[k];
-      t.mp = pad(t.m, sides.all);
-      t.np = pad(t.n, sides.all);
-      t.ma = pad(t.mp, sides.sym);
+      const Sizes z = sizes_of(t.rows, t.cols, sides);
+      t.mp = z.mp;
+      t.np = z.np;
+      t.ma = z.ma;
+      t.split = z.split;
+      t.kpart = sides.kpart;
       t.part = (double*)at;
       t.ws = (f16*)(at + kNormBlocks * sizeof(double));
-      at += bytes_of(t.rows, t.cols, sides);
+      t.sums = (float*)(at + z.bytes);
+      at += z.bytes + z.sums * sizeof(float);
       t.full = full || t.m < 256;
       const size_t want = ((size_t)t.rows * t.cols + kPerNormBlock - 1) / kPerNormBlock;
       t.parts = (int)(want < kNormBlocks ? want : kNormBlocks);

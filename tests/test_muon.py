@@ -106,6 +106,21 @@ def test_large(m, n, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shapes", [[(65, 9001)], [(520, 4100)], [(1000, 4000)], [(4100, 1030)],
+                                    [(16, 40001)], [(3001, 17)],
+                                    [(1000, 4000), (300, 256), (12, 5000), (4000, 1000), (70, 300)]])
+def test_long(shapes, dtype):
+    """One axis much longer than the other: sums over it are shared out."""
+    for kind in ("full", "one"):
+        grads = [gradient(kind, m, n, seed=m).to(dtype).cuda() for m, n in shapes]
+        out = ops.newton_schulz(grads)
+        for g, o, again in zip(grads, out, ops.newton_schulz(grads)):
+            check(g, o)
+            assert torch.equal(o, again)
+
+
+@pytest.mark.gpu
 def test_many_matrices():
     """More than one table of matrices, of one shape and of several."""
     stack = torch.stack([gradient("full", 70, 33, seed=k) for k in range(53)]).cuda()
