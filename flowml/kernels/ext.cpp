@@ -531,7 +531,7 @@ static void muon_call(const std::vector<torch::Tensor>& g,
                     g[k].scalar_type() == g[0].scalar_type(),
                 "gradients: contiguous matrices of one type on one device");
     // places in a working plane are 32-bit byte offsets
-    TORCH_CHECK((g[k].size(0) + 255) * (g[k].size(1) + 255) < (1LL << 30),
+    TORCH_CHECK((g[k].size(0) + 511) * (g[k].size(1) + 511) < (1LL << 30),
                 "matrix too large: 2^30 values at most");
     TORCH_CHECK(w[k].sizes() == g[k].sizes() && w[k].is_contiguous() &&
                     w[k].device() == g[0].device() &&

@@ -91,6 +91,8 @@ struct Table {
 // (in plain rows a step takes 64 or 128 bytes here and there, at distances
 // that fall on few channels of L2 when K is a power of two).
 //
+__host__ __device__ inline int tiles_of(int n, int side) { return (n + side - 1) / side; }
+
 // X has ma rows of np values (mp of them in use), its transpose np rows of mp,
 // A and B ma rows of ma.  Sums over m run to mp, so what lies behind it in A
 // and B meets nothing.
@@ -657,7 +659,7 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   int ti, tj, tile, part = 0;
   if (SYM) {
-    const int mt = t.ma / T::TM, tiles = mt * (mt + 1) / 2;
+    const int mt = tiles_of(t.mp, T::TM), tiles = mt * (mt + 1) / 2;
     tile = xcd_order(blockIdx.x - t.first, tiles * (TO == TO_A ? t.split : 1));
     if (TO == TO_A) {
       part = tile / tiles;
@@ -712,8 +714,8 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   float* piece = (float*)(lds + wave * kPieceHalfs);
   const int wi = i0 + (wave / T::WN) * (T::TM / T::WM), wj = j0 + (wave % T::WN) * (T::TN / T::WN);
   if (TO == TO_A && t.split > 1) {
-    float* to = t.sums + ((size_t)part * ((t.ma / T::TM) * (t.ma / T::TM + 1) / 2) + tile) *
-                            (T::TM * T::TN);
+    const int mt = tiles_of(t.mp, T::TM), tiles = mt * (mt + 1) / 2;
+    float* to = t.sums + ((size_t)part * tiles + tile) * (T::TM * T::TN);
 #pragma unroll
     for (int f = 0; f < T::FM; ++f)
 #pragma unroll
@@ -744,14 +746,14 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
 }
 
 // A from the sums of its parts of K, one 32 x 32 piece to a wave, parts in order.
-template <int T>
-__global__ __launch_bounds__(256) void flowml_ns_join(Table tab, float kb) {
-  __shared__ __align__(16) float lds[4 * 32 * kPieceLd];
-  constexpr int EACH = (T / 32) * (T / 32) / 4;  // blocks to a tile
+__global__ __launch_bounds__(256) void flowml_ns_join(Table tab, int side, float kb) {
+  __shared__ __align__(16) f16 lds[4 * kPieceHalfs];
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int b = blockIdx.x - t.first, tile = b / EACH, piece = b % EACH * 4 + wave;
-  const int mt = t.ma / T, tiles = mt * (mt + 1) / 2;
+  const int mt = tiles_of(t.mp, side), tiles = mt * (mt + 1) / 2;
+  const int across = side / 32, pieces = across * across;
+  const int at = (blockIdx.x - t.first) * 4 + wave, tile = at / pieces, piece = at - tile * pieces;
+  if (tile >= tiles) return;
   int ti, tj;
   tile_of_triangle(tile, mt, ti, tj);
   f32x16 acc;
@@ -759,7 +761,8 @@ __global__ __launch_bounds__(256) void flowml_ns_join(Table tab, float kb) {
   for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll 4
   for (int s = 0; s < t.split; ++s) {
-    const float* from = t.sums + ((size_t)s * tiles + tile) * (T * T) + piece * 1024 + lane * 4;
+    const float* from =
+        t.sums + (((size_t)s * tiles + tile) * pieces + piece) * 1024 + lane * 4;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float4 v = *(const float4*)(from + q * 256);
@@ -769,8 +772,9 @@ __global__ __launch_bounds__(256) void flowml_ns_join(Table tab, float kb) {
       acc[q * 4 + 3] += v.w;
     }
   }
-  finish<TO_A>(tab, t, 0, 0.f, kb, ti * T + piece / (T / 32) * 32, tj * T + piece % (T / 32) * 32,
-               ti != tj, acc, Old{}, lds + wave * 32 * kPieceLd);
+  const int pi = piece / across, pj = piece - pi * across;
+  finish<TO_A>(tab, t, 0, 0.f, kb, ti * side + pi * 32, tj * side + pj * 32, ti != tj, acc, Old{},
+               (float*)(lds + wave * kPieceHalfs));
 }
 
 // ---- matrices that one block holds ----------------------------------------------
@@ -1245,82 +1249,98 @@ constexpr int kPerNormBlock = 8192;
 
 int pad(int v, int t) { return (v + t - 1) / t * t; }
 
-// Tile sides of a call's products, and the parts of K of A.  A tile of 256 runs
-// at 1300 TFLOP/s and one of 64 at 650, but tiles are worth their size only if
-// there are enough for the 256 CUs.  Measured, us a product:
-//   A of 2048 x 4096, hi hi:     64 (528 tiles) 38   128 (136) 30   256 (36) 78
-//   A of 4096 x 4096, hi hi:     128 (528) 91  192 (253) 74   256 (136) 94
-//   B X of 1024 x 4096, full:    64 (1024) 36  128 (256) 29   256 (64) 62
-//   two of these:                128 (512) 75   128 x 256 (256) 66
-//   B X of 4096 x 4096:          128 (1024) 266               256 (256) 230
-// Where A has few tiles and a long K, blocks take parts of K and a launch more
-// joins them: two of 1024 x 4096, full, take 50 us as 272 tiles of 64, and
-// 32 + 6 us as 72 of 128 in 3 parts; all steps of 100 x 100000, 2800 and 377 us.
+// Tile sides of a call's products, and the parts of K of A.  Large tiles run at
+// twice the rate of small ones, but are worth it only if there are enough for
+// the 256 CUs.  Measured, us a product (tiles):
+//   A of 1024 x 4096, full:    64 (136) 25   96 (66) 49    128 (36) 57
+//   A of 2048 x 4096, hi hi:   64 (528) 44   96 (253) 29   128 (136) 32  192 (66) 51
+//   A of 4096 x 4096, hi hi:   96 (946) 101  128 (528) 101 192 (253) 73  256 (136) 93
+//   B X of 1024 x 4096, full:  64 (1024) 36  128 (256) 29  256 (64) 62
+//   two of these:              128 (512) 75  128 x 256 (256) 66
+//   B X of 4096 x 4096:        128 (1024) 266              256 (256) 230
+// For A and B a side is taken by the time that follows from such figures.  Where
+// A has few tiles and a long K, blocks take parts of K and a launch more joins
+// them: two of 1024 x 4096, full, take 50 us as 272 tiles of 64, and 32 + 6 us
+// as 72 of 128 in 3 parts; all steps of 100 x 100000, 2800 and 377 us.
 struct Sides {
   int a, b, m, n;  // A, B, and B X along m and n
   int kpart;       // K of A to a block
 };
+constexpr int kWhole = 1 << 30;  // a kpart that no K passes
 
 int shorter(int r, int c) { return std::min(r, c); }
 int longer(int r, int c) { return std::max(r, c); }
+
+struct Sym {
+  int side;
+  double full, half;  // us for 64 of K, full and hi hi, if a tile has a CU
+};
+constexpr Sym kSym[] = {{64, 0.30, 0.30}, {96, 0.63, 0.30}, {128, 0.83, 0.40},
+                        {192, 1.75, 0.72}, {256, 2.80, 1.17}};
+
+// us of a symmetric product of so many blocks, from times measured over matrices
+// of 512 to 4096 rows.  A full chip runs slower than one block alone: clocks
+// and memory are shared.  Of the small tiles' hi hi products a few share a CU.
+double time_of(const Sym& y, bool full, long long blocks, int K) {
+  const double fill = blocks / 256.0, rounds = (double)((blocks + 255) / 256);
+  double each = (full ? y.full : y.half) * (rounds + 0.5 * fill);
+  if (y.side == 64 && !full) each = std::max(y.half, 0.16 + 0.23 * fill);
+  return each * ((K + 63) / 64) + 2.0 + y.side / 32.0;
+}
 
 Sides sides_for(int count, const int* rows, const int* cols, bool full) {
   auto tiles = [&](int ti, int tj) {
     long long sum = 0;
     for (int k = 0; k < count; ++k)
-      sum += (long long)(pad(shorter(rows[k], cols[k]), ti) / ti) *
-             (pad(longer(rows[k], cols[k]), tj) / tj);
+      sum += (long long)tiles_of(shorter(rows[k], cols[k]), ti) *
+             tiles_of(longer(rows[k], cols[k]), tj);
     return sum;
   };
-  constexpr int ALL = 1 << 30;
   Sides s;
   // a larger side has to make good the padding of matrices that are low
   const long long t64 = tiles(64, 64), t128 = tiles(128, 128), t256 = tiles(256, 256);
   s.m = t256 >= 200 && 3 * t256 <= t128 ? 256 : t128 >= 128 && 8 * t128 <= 3 * t64 ? 128 : 64;
   s.n = s.m == 128 && tiles(128, 256) >= 200 ? 256 : s.m;
+
+  int km = 0, kn = 0;  // the longest K of B and of A
+  for (int k = 0; k < count; ++k) {
+    km = std::max(km, pad(shorter(rows[k], cols[k]), s.m));
+    kn = std::max(kn, pad(longer(rows[k], cols[k]), s.n));
+  }
   // blocks of a symmetric product, and how many of them leave their sums
-  auto triangle = [&](int t, int kpart, long long* parts = nullptr) {
-    long long sum = 0, several = 0;
+  auto triangle = [&](int side, int kpart, long long* several) {
+    long long sum = 0;
+    *several = 0;
     for (int k = 0; k < count; ++k) {
-      const long long a = pad(shorter(rows[k], cols[k]), t) / t;
-      const int n = pad(longer(rows[k], cols[k]), s.n), split = (n - 1) / kpart + 1;
-      sum += a * (a + 1) / 2 * split;
-      if (split > 1) several += a * (a + 1) / 2 * split;
+      const long long mt = tiles_of(pad(shorter(rows[k], cols[k]), s.m), side);
+      const int split = tiles_of(pad(longer(rows[k], cols[k]), s.n), kpart);
+      sum += mt * (mt + 1) / 2 * split;
+      if (split > 1) *several += mt * (mt + 1) / 2 * split;
     }
-    if (parts) *parts = several;
     return sum;
   };
-  s.b = triangle(256, ALL) >= 400   ? 256
-        : triangle(192, ALL) >= 200 ? 192
-        : triangle(128, ALL) >= 128 ? 128
-                                    : 64;
-  s.a = s.b;
-  s.kpart = ALL;
-  if (s.b == 64) {
-    int most = 0;
-    for (int k = 0; k < count; ++k) most = std::max(most, pad(longer(rows[k], cols[k]), s.n));
-    double best = 1e30;
-    for (int t = 64; t <= 128; t += 64)
-      for (int parts = 1; parts <= 64; ++parts) {
-        const int kpart = parts == 1 ? ALL : pad((most + parts - 1) / parts, 64);
-        if (parts > 1 && kpart < 256) break;
-        // us, fitted to the calls above: a CU's step of 64 in K (a few blocks of
-        // 64 x 64 share a CU and hide each other's waits), the tiles' ends, the
-        // sums' way out and in, and the joining launch
-        long long sums;
-        const long long rounds = (triangle(t, kpart, &sums) + 255) / 256;
-        if (parts > 1 && rounds > 2) break;  // no block more brings anything
-        const int steps = (std::min(kpart, most) + 63) / 64;
-        const double step = full ? rounds * (t == 64 ? 0.32 : 0.8)
-                                 : t == 64 ? std::max(0.27, rounds * 0.17) : rounds * 0.38;
-        const double us = steps * step + rounds +
-                          (sums ? 4.0 + 0.15 * parts + sums * t * t * 1.6e-6 : 0.0);
-        if (us < best) {
-          best = us;
-          s.a = t;
-          s.kpart = kpart;
-        }
+  double best_a = 1e30, best_b = 1e30;
+  for (const Sym& y : kSym) {
+    long long sums;
+    const long long whole = triangle(y.side, kWhole, &sums);
+    const double us = time_of(y, full, whole, km);
+    if (us < best_b) {
+      best_b = us;
+      s.b = y.side;
+    }
+    for (int parts = 1; parts <= 64; ++parts) {
+      const int kpart = parts == 1 ? kWhole : pad(tiles_of(kn, parts), 64);
+      const long long blocks = parts == 1 ? whole : triangle(y.side, kpart, &sums);
+      // parts that are short or for which there is no CU bring nothing
+      if (parts > 1 && (kpart < 256 || blocks > 512)) break;
+      const double us = time_of(y, full, blocks, std::min(kpart, kn)) +
+                        (sums ? 4.0 + 0.15 * parts + sums * y.side * y.side * 1.2e-6 : 0.0);
+      if (us < best_a) {
+        best_a = us;
+        s.a = y.side;
+        s.kpart = kpart;
       }
+    }
   }
   return s;
 }
@@ -1335,10 +1355,9 @@ Sizes sizes_of(int rows, int cols, Sides s) {
   Sizes z;
   z.mp = pad(shorter(rows, cols), s.m);
   z.np = pad(longer(rows, cols), s.n);
-  z.ma = pad(z.mp, s.a);
-  if (s.b != s.a) z.ma = pad(z.ma, s.b);
-  z.split = s.kpart < z.np ? (z.np + s.kpart - 1) / s.kpart : 1;
-  const size_t mp = z.mp, np = z.np, ma = z.ma, mt = ma / s.a;
+  z.ma = std::max(pad(z.mp, s.a), pad(z.mp, s.b));
+  z.split = tiles_of(z.np, s.kpart);
+  const size_t mp = z.mp, np = z.np, ma = z.ma, mt = tiles_of(z.mp, s.a);
   z.bytes = kNormBlocks * sizeof(double) + (2 * ma * np + 4 * np * mp + 4 * ma * ma) * sizeof(f16);
   z.sums = z.split > 1 ? mt * (mt + 1) / 2 * s.a * s.a * z.split : 0;
   return z;
@@ -1351,7 +1370,7 @@ void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
   for (int k = 0; k < tab.count; ++k) {
     Mat& t = tab.mat[k];
     t.first = blocks;
-    const int mt = t.ma / T::TM;
+    const int mt = tiles_of(t.mp, T::TM);
     blocks += TO == TO_A   ? mt * (mt + 1) / 2 * t.split
               : TO == TO_B ? mt * (mt + 1) / 2
                            : (t.mp / T::TM) * (t.np / T::TN);
@@ -1360,17 +1379,15 @@ void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
                      0, st, tab, turn, ka, kb);
 }
 
-template <int T>
-void join(Table& tab, float kb, hipStream_t st) {
+void join(Sides s, Table& tab, float kb, hipStream_t st) {
   int blocks = 0;
   for (int k = 0; k < tab.count; ++k) {
     Mat& t = tab.mat[k];
     t.first = blocks;
-    const int mt = t.ma / T;
-    if (t.split > 1) blocks += mt * (mt + 1) / 2 * ((T / 32) * (T / 32) / 4);
+    const int mt = tiles_of(t.mp, s.a), pieces = mt * (mt + 1) / 2 * (s.a / 32) * (s.a / 32);
+    if (t.split > 1) blocks += tiles_of(pieces, 4);
   }
-  if (blocks)
-    hipLaunchKernelGGL((flowml_ns_join<T>), dim3(blocks), dim3(256), 0, st, tab, kb);
+  if (blocks) hipLaunchKernelGGL(flowml_ns_join, dim3(blocks), dim3(256), 0, st, tab, s.a, kb);
 }
 
 template <int TO>
@@ -1382,16 +1399,13 @@ void product(Sides s, Table& tab, int turn, float ka, float kb, hipStream_t st) 
       product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
     else if (side == 192)
       product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+    else if (side == 96)
+      product_of<Tile<96, 96, 3, 1>, Depth<32, 6>, Depth<64, 6>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
     else if (side == 128)
       product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
     else
       product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
-    if (TO == TO_A && s.kpart < (1 << 30)) {
-      if (side == 128)
-        join<128>(tab, kb, st);
-      else
-        join<64>(tab, kb, st);
-    }
+    if (TO == TO_A && s.kpart < kWhole) join(s, tab, kb, st);
   } else {
     if (s.m == 256)
       product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
