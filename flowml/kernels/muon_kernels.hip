@@ -91,27 +91,31 @@ struct Table {
 // (in plain rows a step takes 64 or 128 bytes here and there, at distances
 // that fall on few channels of L2 when K is a power of two).
 //
+// X is kept as its transpose alone, np rows of ma values (mp of them in use):
+// B X sums over these and A over the rows, which LDS turns as it reads.  (With
+// X as well, read by A alone, 1000 x 4000 twice took 575 us for 553 in fp32.)
+// A and B have ma rows of ma.  Sums over m run to mp, so what lies behind it
+// meets nothing.
 __host__ __device__ inline int tiles_of(int n, int side) { return (n + side - 1) / side; }
 
-// X has ma rows of np values (mp of them in use), its transpose np rows of mp,
-// A and B ma rows of ma.  Sums over m run to mp, so what lies behind it in A
-// and B meets nothing.
-__host__ __device__ inline size_t plane_x(const Mat& t) { return (size_t)t.ma * t.np; }
-__host__ __device__ inline size_t plane_xt(const Mat& t) { return (size_t)t.np * t.mp; }
+// A's tiles are panels of X', whose distance is not to be a power of two: 5 KB
+// more (2048 x 4096 bf16: 595 and 585 us, 1024 x 4096 f32 330 and 327).
+constexpr int kGap = 80;
+__host__ __device__ inline int rows_xt(int np) { return np + kGap; }
+__host__ __device__ inline size_t plane_xt(const Mat& t) { return (size_t)rows_xt(t.np) * t.ma; }
 __host__ __device__ inline size_t plane_a(const Mat& t) { return (size_t)t.ma * t.ma; }
 // place of (row, k) in a plane of `rows` rows
 __device__ __forceinline__ size_t place(int rows, int row, int k) {
   return ((size_t)(k >> 5) * rows + row) * 32 + (k & 31);
 }
-__device__ __forceinline__ f16* ws_x(const Mat& t, int p) { return t.ws + p * plane_x(t); }
 __device__ __forceinline__ f16* ws_xt(const Mat& t, int which, int p) {
-  return t.ws + 2 * plane_x(t) + (2 * which + p) * plane_xt(t);
+  return t.ws + (2 * which + p) * plane_xt(t);
 }
 __device__ __forceinline__ f16* ws_a(const Mat& t, int p) {
-  return t.ws + 2 * plane_x(t) + 4 * plane_xt(t) + p * plane_a(t);
+  return t.ws + 4 * plane_xt(t) + p * plane_a(t);
 }
 __device__ __forceinline__ f16* ws_b(const Mat& t, int p) {
-  return t.ws + 2 * plane_x(t) + 4 * plane_xt(t) + (2 + p) * plane_a(t);
+  return t.ws + 4 * plane_xt(t) + (2 + p) * plane_a(t);
 }
 
 // (Every function that takes the table is inlined: it stays in the arguments'
@@ -250,7 +254,6 @@ __global__ __launch_bounds__(256) void flowml_ns_first(Table tab) {
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   const int b = blockIdx.x - t.first, tid = threadIdx.x;
   const bool turned = t.rows > t.cols;  // the caller's rows run along n
-  const int rows_straight = turned ? t.np : t.ma, rows_turned = turned ? t.ma : t.np;
   const int across = (turned ? t.mp : t.np) / 64;
   const int r0 = b / across * 64, c0 = b % across * 64;
 
@@ -263,13 +266,7 @@ __global__ __launch_bounds__(256) void flowml_ns_first(Table tab) {
   const double norm = sqrt(red[0] + red[1] + red[2] + red[3]);
   const float scale = norm <= (double)tab.eps ? (float)(kScaleX / (double)tab.eps)
                                               : (float)(kScaleX / norm);  // NaN stays
-  // hi hi alone takes X X^T from the higher halves
-  f16* straight[2];
-  f16* other[2];
-  for (int p = 0; p < 2; ++p) {
-    straight[p] = turned ? ws_xt(t, 0, p) : ws_x(t, p);
-    other[p] = turned ? ws_x(t, p) : ws_xt(t, 0, p);
-  }
+  f16 *const to_hi = ws_xt(t, 0, 0), *const to_lo = ws_xt(t, 0, 1);
   const int r8 = tid >> 3, c8 = (tid & 7) * 8;
 #pragma unroll
   for (int h = 0; h < 64; h += 32) {
@@ -286,10 +283,13 @@ __global__ __launch_bounds__(256) void flowml_ns_first(Table tab) {
       tile[r8 + h][c8 + k] = (uint32_t)__builtin_bit_cast(uint16_t, x) |
                              ((uint32_t)__builtin_bit_cast(uint16_t, y) << 16);
     }
-    const size_t at = place(rows_straight, r, c);
-    *(f16x8*)(straight[0] + at) = hi;
-    if (turned || t.full) *(f16x8*)(straight[1] + at) = lo;
+    if (turned) {
+      const size_t at = place(rows_xt(t.np), r, c);
+      *(f16x8*)(to_hi + at) = hi;
+      *(f16x8*)(to_lo + at) = lo;
+    }
   }
+  if (turned) return;
   __syncthreads();
 #pragma unroll
   for (int h = 0; h < 64; h += 32) {
@@ -300,9 +300,9 @@ __global__ __launch_bounds__(256) void flowml_ns_first(Table tab) {
       hi[k] = __builtin_bit_cast(f16, (uint16_t)(v & 0xffff));
       lo[k] = __builtin_bit_cast(f16, (uint16_t)(v >> 16));
     }
-    const size_t at = place(rows_turned, c0 + r8 + h, r0 + c8);
-    *(f16x8*)(other[0] + at) = hi;
-    if (!turned || t.full) *(f16x8*)(other[1] + at) = lo;
+    const size_t at = place(rows_xt(t.np), c0 + r8 + h, r0 + c8);
+    *(f16x8*)(to_hi + at) = hi;
+    *(f16x8*)(to_lo + at) = lo;
   }
 }
 
@@ -332,6 +332,21 @@ __device__ __forceinline__ void block_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// 8 values of a column: a lane gets those of its own column from two times 4
+// rows, whose 4 x 16 values the 16 lanes around it address, 4 values each.
+__device__ __forceinline__ f16x8 read_turned(const f16* at, int rows4) {
+#ifdef __HIP_DEVICE_COMPILE__
+  typedef __fp16 h4 __attribute__((vector_size(8)));
+  typedef __attribute__((address_space(3))) h4 lds_h4;
+  const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4*)at));
+  const f16x4 b =
+      __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4*)(at + rows4)));
+  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+#else
+  return f16x8{};
+#endif
+}
+
 // acc += P Q^T over K: P has TM rows, Q TN rows.  PA, PB: planes of each (2:
 // hi and lo).  S stages of operands in LDS: the copies of S - 1 steps are under
 // way while a step is multiplied, and a step waits for its own copies alone.
@@ -342,7 +357,7 @@ __device__ __forceinline__ void block_barrier() {
 // of the multiplications keeps the matrix core idle as long as LDS takes to
 // accept them (64 x 64 tiles: 1040 cycles a step, 400 of them multiplying).
 // The scheduling barriers keep the compiler from gathering them again.
-template <class T, int BK, int S, int PA, int PB>
+template <class T, int BK, int S, int PA, int PB, bool TURNED>
 __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, const f16* const (&Q)[2],
                                         int rows_q, int K, f16* lds, f32x16 (&acc)[T::FM][T::FN]) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know buffer resources
@@ -373,15 +388,26 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
   auto copy = [&](int k0, f16* s, int which) {
     const bool first = which < PA * LA;
     const int w = first ? which : which - PA * LA, l = first ? LA : LB;
-    const int p = w / l, i = w % l, panel = i / (l / (BK / 32)), j = i % (l / (BK / 32));
+    const int p = w / l, i = w % l;
+    const auto plane = first ? rp[p] : rq[p];
+    f16* to = s + (first ? p * T::TM : PA * T::TM + p * T::TN) * BK;
+    if (TURNED) {
+      const int panel = (wave * l + i) / (BK / 16), piece = (wave * l + i) % (BK / 16);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          plane, (lds_void*)(to + (panel * BK + piece * 16) * 32), 16, lane * 16,
+          (panel * (first ? rows_p : rows_q) + k0 + piece * 16) * 64, 0, 0);
+      return;
+    }
+    const int panel = i / (l / (BK / 32)), j = i % (l / (BK / 32));
     const int rows = first ? T::TM : T::TN, piece = wave * (l / (BK / 32)) + j;
-    f16* to = s + (first ? p * T::TM : PA * T::TM + p * T::TN) * BK + panel * rows * 32 + piece * 512;
     const int panels = (k0 >> 5) + panel;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        first ? rp[p] : rq[p], (lds_void*)to, 16, from,
+        plane, (lds_void*)(to + panel * rows * 32 + piece * 512), 16, from,
         panels * (first ? rows_p : rows_q) * 64 + piece * 1024, 0, 0);
   };
+  const int column = ((lane >> 5) * 8 + ((lane & 15) >> 2)) * 32 + (lane & 16) + (lane & 3) * 4;
   auto read = [&](const f16* plane, int rows, int row, int kk) {
+    if (TURNED) return read_turned(plane + ((row >> 5) * BK + kk * 16) * 32 + column, 4 * 32);
     return *(const f16x8*)(plane + (kk >> 1) * rows * 32 + row * 32 +
                            swizzle((kk & 1) * 2 + (lane >> 5), row) * 8);
   };
@@ -426,12 +452,16 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
   else
     wait_loads<0>();
   block_barrier();
+  [&](const f16* __restrict s) __attribute__((always_inline)) {
 #pragma unroll
-  for (int r = 0; r < PA + PB * T::FN; ++r) read_one(lds, 0, r);
+    for (int r = 0; r < PA + PB * T::FN; ++r) read_one(s, 0, r);
+  }(lds);
   int cur = 0, free = (S - 1) * STAGE;  // the stage read, and the one to fill
-  auto step = [&](auto more, int i) {
+  // (Stages are distinct memory as far as the compiler is told, or it lets every
+  // turned read wait for all copies.)
+  auto step = [&](auto more, int i, const f16* __restrict now, const f16* __restrict then,
+                  f16* __restrict later) __attribute__((always_inline)) {
     constexpr bool MORE = decltype(more)::value;
-    const int next = cur + STAGE == S * STAGE ? 0 : cur + STAGE;
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const bool last = u + 1 == UNITS;
@@ -444,28 +474,35 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
         if (MORE) {
 #pragma unroll
           for (int c = m * copies / MULS; c < (m + 1) * copies / MULS; ++c)
-            copy((i + S - 1) * BK, lds + free, c0 + c);
+            copy((i + S - 1) * BK, later, c0 + c);
         }
         if (last && m == 0 && (MORE || i + 1 < steps)) {
           // of this step's own copies, REST are still to be sent
           wait_loads<MORE ? LOADS*(S - 2) - REST : 0>();
-          block_barrier();
+          // (naming the stages keeps their reads and copies on their sides)
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::"s"((lds_void*)now),
+                       "s"((lds_void*)then), "s"((lds_void*)later)
+                       : "memory");
         }
         if (!last || MORE || i + 1 < steps) {
           // two at a time: what LDS delivers during a matrix instruction
           const int r1 = m + 1 == MULS || 2 * m + 2 > reads ? reads : 2 * m + 2;
 #pragma unroll
-          for (int r = 2 * m; r < r1; ++r) read_one(lds + (last ? next : cur), (u + 1) % UNITS, r);
+          for (int r = 2 * m; r < r1; ++r) read_one(last ? then : now, (u + 1) % UNITS, r);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+  };
+  auto turn_step = [&](auto more, int i) __attribute__((always_inline)) {
+    const int next = cur + STAGE == S * STAGE ? 0 : cur + STAGE;
+    step(more, i, lds + cur, lds + next, lds + free);
     free = cur;
     cur = next;
   };
   int i = 0;
-  for (; i + S - 1 < steps; ++i) step(std::true_type{}, i);
-  for (; i < steps; ++i) step(std::false_type{}, i);
+  for (; i + S - 1 < steps; ++i) turn_step(std::true_type{}, i);
+  for (; i < steps; ++i) turn_step(std::false_type{}, i);
 #endif
 }
 
@@ -497,7 +534,7 @@ __device__ __forceinline__ Old load_old(const Mat& t, int turn, int i0, int j0) 
   Old o;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const size_t at = place(TO == TO_B ? t.ma : t.np, j0 + h * 16 + r4, i0 + c8);
+    const size_t at = place(TO == TO_B ? t.ma : rows_xt(t.np), j0 + h * 16 + r4, i0 + c8);
     o.hi[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 0) : ws_xt(t, turn, 0)) + at);
     o.lo[h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
     if (TO != TO_B || t.full)
@@ -521,7 +558,7 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
   f16* ch = TO == TO_A ? ws_a(t, 0) : TO == TO_B ? ws_b(t, 0) : ws_xt(t, turn ^ 1, 0);
   f16* cl = TO == TO_A ? ws_a(t, 1) : TO == TO_B ? ws_b(t, 1) : ws_xt(t, turn ^ 1, 1);
   const int r4 = lane >> 2, c8 = (lane & 3) * 8;
-  const int rows_j = TO == TO_A || TO == TO_B ? t.ma : t.np;  // of a plane whose rows are columns j
+  const int rows_j = TO == TO_A || TO == TO_B ? t.ma : rows_xt(t.np);  // of a plane whose rows are columns j
 #pragma unroll
   for (int q = 0; q < 4; ++q)
     *(float4*)(lds + (lane & 31) * kPieceLd + q * 8 + (lane >> 5) * 4) =
@@ -563,10 +600,8 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
     *(uint4*)p = make_uint4(both[0], both[1], both[2], both[3]);
     *(uint4*)(p + 4) = make_uint4(both[4], both[5], both[6], both[7]);
   }
-  if (!mirror || (TO == TO_END && turned)) return;
+  if (TO == TO_X || !mirror || (TO == TO_END && turned)) return;
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  f16* sh = TO == TO_X ? ws_x(t, 0) : ch;
-  f16* sl = TO == TO_X ? ws_x(t, 1) : cl;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int i = h * 16 + r4;
@@ -585,8 +620,8 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
       lo[k] = __builtin_bit_cast(f16, (uint16_t)(u >> 16));
     }
     const size_t at = place(t.ma, i0 + i, j0 + c8);
-    *(f16x8*)(sh + at) = hi;
-    if (t.full) *(f16x8*)(sl + at) = lo;
+    *(f16x8*)(ch + at) = hi;
+    if (t.full) *(f16x8*)(cl + at) = lo;
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
@@ -677,18 +712,23 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
   const f16* Q[2];
 #pragma unroll
   for (int p = 0; p < 2; ++p) {
-    P[p] = (TO == TO_A ? ws_x(t, p) : TO == TO_B ? ws_a(t, p) : ws_b(t, p)) + i0 * 32;
-    Q[p] = (TO == TO_A ? ws_x(t, p) : TO == TO_B ? ws_a(t, p) : ws_xt(t, turn, p)) + j0 * 32;
+    if (TO == TO_A) {
+      P[p] = ws_xt(t, turn, p) + place(rows_xt(t.np), 0, i0);
+      Q[p] = ws_xt(t, turn, p) + place(rows_xt(t.np), 0, j0);
+    } else {
+      P[p] = (TO == TO_B ? ws_a(t, p) : ws_b(t, p)) + i0 * 32;
+      Q[p] = (TO == TO_B ? ws_a(t, p) : ws_xt(t, turn, p)) + j0 * 32;
+    }
   }
   int K = TO == TO_A ? t.np : t.mp;
-  const int rows_q = SYM ? t.ma : t.np;
+  const int rows_p = TO == TO_A ? rows_xt(t.np) : t.ma, rows_q = TO == TO_B ? t.ma : rows_xt(t.np);
   if (TO == TO_A && t.split > 1) {
     const int k0 = part * t.kpart;
     K = K - k0 < t.kpart ? K - k0 : t.kpart;
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      P[p] += (size_t)k0 * t.ma;
-      Q[p] += (size_t)k0 * t.ma;
+      P[p] += (size_t)k0 * 32;
+      Q[p] += (size_t)k0 * 32;
     }
   }
 
@@ -700,11 +740,11 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[f][g][r] = 0.f;
   if (t.full)
-    product<T, D22::BK, D22::S, 2, 2>(P, t.ma, Q, rows_q, K, lds, acc);
+    product<T, D22::BK, D22::S, 2, 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
   else if (SYM)
-    product<T, D11::BK, D11::S, 1, 1>(P, t.ma, Q, rows_q, K, lds, acc);
+    product<T, D11::BK, D11::S, 1, 1, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
   else
-    product<T, D12::BK, D12::S, 1, 2>(P, t.ma, Q, rows_q, K, lds, acc);
+    product<T, D12::BK, D12::S, 1, 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool mirror = !SYM || ti != tj;
@@ -815,17 +855,8 @@ __device__ __forceinline__ Halves small_read(const f16* plane, int low, int at) 
 
 // the same of 32 rows from `k` on, columns i to i + 15
 __device__ __forceinline__ f16x8 read_columns(const f16* plane, int ld, int k, int i, int lane) {
-#ifdef __HIP_DEVICE_COMPILE__
-  typedef __fp16 h4 __attribute__((vector_size(8)));
-  typedef __attribute__((address_space(3))) h4 lds_h4;
-  const f16* at = plane + (k + (lane >> 4) * 8 + ((lane & 15) >> 2)) * ld + i + (lane & 3) * 4;
-  const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4*)at));
-  const f16x4 b =
-      __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_h4*)(at + 4 * ld)));
-  return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-#else
-  return f16x8{};
-#endif
+  return read_turned(
+      plane + (k + (lane >> 4) * 8 + ((lane & 15) >> 2)) * ld + i + (lane & 3) * 4, 4 * ld);
 }
 
 __device__ __forceinline__ Halves small_columns(const f16* plane, int low, int ld, int k, int i,
@@ -1357,8 +1388,8 @@ Sizes sizes_of(int rows, int cols, Sides s) {
   z.np = pad(longer(rows, cols), s.n);
   z.ma = std::max(pad(z.mp, s.a), pad(z.mp, s.b));
   z.split = tiles_of(z.np, s.kpart);
-  const size_t mp = z.mp, np = z.np, ma = z.ma, mt = tiles_of(z.mp, s.a);
-  z.bytes = kNormBlocks * sizeof(double) + (2 * ma * np + 4 * np * mp + 4 * ma * ma) * sizeof(f16);
+  const size_t np = z.np, ma = z.ma, mt = tiles_of(z.mp, s.a);
+  z.bytes = kNormBlocks * sizeof(double) + (4 * rows_xt(np) * ma + 4 * ma * ma) * sizeof(f16);
   z.sums = z.split > 1 ? mt * (mt + 1) / 2 * s.a * s.a * z.split : 0;
   return z;
 }
@@ -1596,7 +1627,7 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
     }
     hipLaunchKernelGGL(flowml_ns_first, dim3(blocks), dim3(256), 0, st, tab);
     for (int s = 0; s < steps; ++s) {
-      product<TO_A>(sides, tab, 0, 0.f, sa / (sx * sx), st);
+      product<TO_A>(sides, tab, s & 1, 0.f, sa / (sx * sx), st);
       product<TO_B>(sides, tab, 0, coef[1] * sb / sa, coef[2] * sb / (sa * sa), st);
       if (s + 1 < steps)
         product<TO_X>(sides, tab, s & 1, coef[0], 1.f / sb, st);
