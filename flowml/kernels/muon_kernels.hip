@@ -16,7 +16,7 @@
 // fp16 numbers, x 2^s = hi + lo, 22 bits, and a product is three fp16 matrix
 // products accumulated in fp32: hi hi + hi lo + lo hi.  That is as exact as
 // fp32 (1.0 to 1.25 times its error on full-rank, low-rank and rank-1
-// gradients) at a third of the fp16 matrix rate, 5 times the fp32 rate.
+// gradients) at a third of the fp16 matrix rate, 3 times the fp32 rate.
 // Where the result is rounded to bf16, A and A^2 take hi hi alone and B X
 // takes hi (hi + lo): an error in A or B turns the left singular vectors by
 // 2^-12 but leaves the row space of X exact, so no noise grows.
@@ -24,14 +24,12 @@
 // A and A^2 are symmetric: tiles on or above the diagonal are computed, and
 // each is written to both places.
 //
-// All operands are stored with the summed index side by side, so that every
-// product is rows times rows: X serves X X^T, its transpose serves B X, and
-// the epilogue of B X writes both.  Working matrices are padded with zeros to
-// whole tiles, which the iteration keeps, so that only the first and the last
-// kernel look at ragged edges.
-//
-// The matrices of one call share their launches: 2 + 3 * steps, whatever
-// their number and shapes.
+// Three ways, by size: matrices of 16 rows or fewer are iterated as their small
+// square alone, in fp64; those that fit a CU's LDS are held there, in one launch
+// for all of a call; the rest goes through working planes in memory, padded with
+// zeros to whole tiles, which the iteration keeps, so that only the first and
+// the last kernel look at ragged edges.  These share their launches too: 2 + 3 *
+// steps, and one more a step where sums are shared out.
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
@@ -56,7 +54,7 @@ constexpr float kScaleX = 16384.f;  // |x| <= 1.9: within fp16
 constexpr float kScaleA = 16384.f;  // |x|^2 <= 3.7
 
 struct Mat {
-  f16* ws;         // X, X^T (two), A, B: two planes each
+  f16* ws;         // X^T (two), A, B: two planes each
   double* part;    // sums of squares
   const void* g;   // gradient, rows x cols
   float* mom;      // momentum buffer, or null
@@ -682,14 +680,14 @@ constexpr int lds_halfs() {
 }
 constexpr int most(int a, int b) { return a > b ? a : b; }
 
-// One tile of A, B, X' or the result.  D22, D11, D12: LDS depths for full
-// products, hi hi, and hi (hi + lo).
-template <class T, class D22, class D11, class D12, int TO>
+// One tile of A, B, X' or the result.  FULL, PART: LDS depths for full products
+// and for hi hi, of B X hi (hi + lo).
+template <class T, class FULL, class PART, int TO>
 __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, int turn, float ka,
                                                                   float kb) {
   constexpr bool SYM = TO == TO_A || TO == TO_B;
-  constexpr int HALFS = most(most(lds_halfs<T, D22, 2, 2>(), T::WAVES * kPieceHalfs),
-                             SYM ? lds_halfs<T, D11, 1, 1>() : lds_halfs<T, D12, 1, 2>());
+  constexpr int HALFS = most(most(lds_halfs<T, FULL, 2, 2>(), T::WAVES * kPieceHalfs),
+                             lds_halfs<T, PART, 1, SYM ? 1 : 2>());
   __shared__ __align__(16) f16 lds[HALFS];
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   int ti, tj, tile, part = 0;
@@ -740,11 +738,9 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[f][g][r] = 0.f;
   if (t.full)
-    product<T, D22::BK, D22::S, 2, 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
-  else if (SYM)
-    product<T, D11::BK, D11::S, 1, 1, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
+    product<T, FULL::BK, FULL::S, 2, 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
   else
-    product<T, D12::BK, D12::S, 1, 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
+    product<T, PART::BK, PART::S, 1, SYM ? 1 : 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool mirror = !SYM || ti != tj;
@@ -1388,14 +1384,14 @@ Sizes sizes_of(int rows, int cols, Sides s) {
   z.np = pad(longer(rows, cols), s.n);
   z.ma = std::max(pad(z.mp, s.a), pad(z.mp, s.b));
   z.split = tiles_of(z.np, s.kpart);
-  const size_t np = z.np, ma = z.ma, mt = tiles_of(z.mp, s.a);
-  z.bytes = kNormBlocks * sizeof(double) + (4 * rows_xt(np) * ma + 4 * ma * ma) * sizeof(f16);
+  const size_t nx = rows_xt(z.np), ma = z.ma, mt = tiles_of(z.mp, s.a);
+  z.bytes = kNormBlocks * sizeof(double) + (4 * nx * ma + 4 * ma * ma) * sizeof(f16);
   z.sums = z.split > 1 ? mt * (mt + 1) / 2 * s.a * s.a * z.split : 0;
   return z;
 }
 
 // one product for all matrices of a table; `first` of each is set here
-template <class T, class D22, class D11, class D12, int TO>
+template <class T, class FULL, class PART, int TO>
 void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
   int blocks = 0;
   for (int k = 0; k < tab.count; ++k) {
@@ -1406,7 +1402,7 @@ void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
               : TO == TO_B ? mt * (mt + 1) / 2
                            : (t.mp / T::TM) * (t.np / T::TN);
   }
-  hipLaunchKernelGGL((flowml_ns_product<T, D22, D11, D12, TO>), dim3(blocks), dim3(T::WAVES * 64),
+  hipLaunchKernelGGL((flowml_ns_product<T, FULL, PART, TO>), dim3(blocks), dim3(T::WAVES * 64),
                      0, st, tab, turn, ka, kb);
 }
 
@@ -1423,29 +1419,29 @@ void join(Sides s, Table& tab, float kb, hipStream_t st) {
 
 template <int TO>
 void product(Sides s, Table& tab, int turn, float ka, float kb, hipStream_t st) {
-  // tile, waves, and the depth of LDS for two planes, hi hi, hi (hi + lo)
+  // tile, waves, and the depth of LDS for full products and for others
   if constexpr (TO == TO_A || TO == TO_B) {
     const int side = TO == TO_A ? s.a : s.b;
     if (side == 256)
-      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, TO>(tab, turn, ka, kb, st);
     else if (side == 192)
-      product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, TO>(tab, turn, ka, kb, st);
     else if (side == 96)
-      product_of<Tile<96, 96, 3, 1>, Depth<32, 6>, Depth<64, 6>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<96, 96, 3, 1>, Depth<32, 6>, Depth<64, 6>, TO>(tab, turn, ka, kb, st);
     else if (side == 128)
-      product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, TO>(tab, turn, ka, kb, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, Depth<32, 2>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, st);
     if (TO == TO_A && s.kpart < kWhole) join(s, tab, kb, st);
   } else {
     if (s.m == 256)
-      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
     else if (s.n == 256)
-      product_of<Tile<128, 256, 2, 4>, Depth<32, 3>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<128, 256, 2, 4>, Depth<32, 3>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
     else if (s.m == 128)
-      product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 2>, Depth<32, 5>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, st);
   }
 }
 

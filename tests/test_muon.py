@@ -63,9 +63,9 @@ def tolerance(G, sizes, dtype, coef=COEF):
     return tol
 
 
-def check(G, got, steps=5, coef=COEF, eps=1e-7):
-    ref, sizes = reference(G.cpu(), steps, coef, eps)
-    off = float((got.cpu().double() - ref).norm())
+def check(G, got, steps=5, coef=COEF, eps=1e-7, dev="cpu"):
+    ref, sizes = reference(G.to(dev), steps, coef, eps)
+    off = float((got.to(dev).double() - ref).norm())
     tol = tolerance(G, sizes, G.dtype, coef)
     size = float(ref.norm())
     if G.dtype == torch.bfloat16:
@@ -103,6 +103,17 @@ def test_large(m, n, dtype):
         got = ops.newton_schulz(G)
         check(G, got)
         assert torch.equal(got, ops.newton_schulz(G))  # one order of sums
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(1600, 1500), (2000, 4100), (4096, 4096), (5632, 5640)])
+def test_tiles(m, n, dtype):
+    """Sizes that take tiles of every side; the reference on the GPU in 64 bits."""
+    G = gradient("full", m, n, seed=1).to(dtype).cuda()
+    got = ops.newton_schulz(G)
+    check(G, got, dev="cuda")
+    assert torch.equal(got, ops.newton_schulz(G))
 
 
 @pytest.mark.gpu
