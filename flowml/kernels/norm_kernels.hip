@@ -487,8 +487,8 @@ __global__ __launch_bounds__(256) void flowml_layer_norm_grad_cols(
   slab[D + c] = db;
 }
 
-// dg[c], db[c]: sums of part[s][0][c] and part[s][1][c] over the slabs, in an order that G alone sets:
-// 32 columns x 32 runs of slabs per block.
+// dg[c], db[c]: sums of part[s][0][c] and part[s][1][c] over the slabs, in an
+// order that G alone sets: 32 columns x 32 runs of slabs per block.
 __global__ __launch_bounds__(1024) void flowml_layer_norm_slabs(
     const float* __restrict__ part, float* __restrict__ dg, float* __restrict__ db, int G, int D) {
   __shared__ float s[32][33];
@@ -597,8 +597,6 @@ void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, fl
   LN_CASE(64, 2);
   LN_CASE(256, 1);
   LN_CASE(256, 2);
-  LN_CASE(512, 2);
-  LN_CASE(1024, 2);
   if constexpr (Piece<T>::VEC == 4) {
     LN_CASE(256, 3);
     LN_CASE(256, 4);
@@ -606,6 +604,9 @@ void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, fl
     LN_CASE(512, 4);
     LN_CASE(1024, 3);
     LN_CASE(1024, 4);
+  } else {
+    LN_CASE(512, 2);
+    LN_CASE(1024, 2);
   }
 #undef LN_CASE
 }

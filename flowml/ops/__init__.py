@@ -823,7 +823,7 @@ def _ns_scale(steps: int, coefficients: Tuple[float, float, float]) -> float:
     pairs scaled by 2^14, so they must stay under 1.9; a polynomial that lets
     them grow further does not orthogonalise either.
     """
-    if steps < 1 or int(steps) != steps:
+    if not math.isfinite(steps) or steps < 1 or int(steps) != steps:
         raise ValueError(f"steps must be a whole number >= 1, got {steps!r}")
     if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
         raise ValueError(f"coefficients must be three finite numbers, got {coefficients!r}")
@@ -893,11 +893,13 @@ def newton_schulz(
     side, X ← a·X + (b·A + c·A²)·X. The polynomial moves every singular value
     towards 1 (the default one into [0.7, 1.2], fast for small ones). The
     result has G's type; f32 and f16 are computed as exactly as in fp32. All
-    matrices of a call share their kernel launches. A matrix that holds a NaN
+    matrices of a call share their kernel launches; one may have about 2^30 values
+    on a GPU. A matrix that holds a NaN
     or an infinity comes out as NaN, an empty one as it is.
     """
     coefficients = tuple(float(v) for v in coefficients)
     scale = _ns_scale(steps, coefficients)
+    steps = int(steps)
     if not 1e-30 <= eps < math.inf:
         raise ValueError(f"eps must be finite and at least 1e-30, got {eps!r}")
     if isinstance(G, torch.Tensor):
@@ -942,11 +944,14 @@ def muon_update(
 
     The factor gives every update the same mean square (0.2·lr)², whatever the
     shape, the same for a matrix and its transpose. Weights and buffers must be
-    contiguous and apart from each other in memory. The numbers are taken at
-    the call: a captured graph repeats the step with the lr it was captured with.
+    contiguous and apart from each other in memory; autograd does not record the
+    step, but refuses a backward pass through values from before it. The numbers
+    are taken at the call: a captured graph repeats the step with the lr it was
+    captured with.
     """
     coefficients = tuple(float(v) for v in coefficients)
     scale = _ns_scale(steps, coefficients)
+    steps = int(steps)
     if not 1e-30 <= eps < math.inf:
         raise ValueError(f"eps must be finite and at least 1e-30, got {eps!r}")
     if not 0 <= momentum < 1:
@@ -996,14 +1001,17 @@ def muon_update(
                 [lr * 0.2 * math.sqrt(max(weights[k].shape)) for k in live],
                 momentum, keep, nesterov, steps, coefficients, eps, scale,
             )
+            torch.autograd.graph.increment_version(
+                [t for t in weights + buffers if not t.is_inference()])
         return
-    for w, g, m in zip(weights, grads, buffers):
-        if not w.numel():
-            continue
-        g = g.to(torch.float32)
-        m.mul_(momentum).add_(g)
-        o = _ns_torch(g + momentum * m if nesterov else m, steps, coefficients, eps)
-        w.copy_(keep * w.to(torch.float32) - lr * 0.2 * math.sqrt(max(w.shape)) * o)
+    with torch.no_grad():
+        for w, g, m in zip(weights, grads, buffers):
+            if not w.numel():
+                continue
+            g = g.to(torch.float32)
+            m.mul_(momentum).add_(g)
+            o = _ns_torch(g + momentum * m if nesterov else m, steps, coefficients, eps)
+            w.copy_(keep * w.to(torch.float32) - lr * 0.2 * math.sqrt(max(w.shape)) * o)
 
 
 def softmax_xent_grad(

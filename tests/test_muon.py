@@ -259,6 +259,22 @@ def test_update_twice_the_same_and_in_a_graph(shapes):
         assert all(torch.equal(p, q) for p, q in zip(ws + ms, we + me))
 
 
+@pytest.mark.parametrize("dev", DEVICES)
+def test_parameters(dev):
+    """A leaf that wants gradients is stepped, and no backward pass goes through
+    what it was."""
+    w = torch.randn(30, 40, device=dev, requires_grad=True)
+    was = w.detach().clone()
+    y = (w * w).sum()
+    ops.muon_update([w], [torch.ones_like(was)], [torch.zeros_like(was)], lr=0.1)
+    assert w.requires_grad and w.is_leaf and not torch.equal(w.detach(), was)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        v = torch.randn(30, 40, device=dev)
+        ops.muon_update([v], [torch.ones_like(was)], [torch.zeros_like(was)], lr=0.1)
+
+
 def test_refusals():
     w, g, m = torch.randn(6, 4), torch.randn(6, 4), torch.zeros(6, 4)
     step = lambda *a, **k: ops.muon_update(*a, lr=0.1, **k)  # noqa: E731
@@ -272,6 +288,7 @@ def test_refusals():
         lambda: ops.newton_schulz([g, 3.0]),
         lambda: ops.newton_schulz(g, steps=0),
         lambda: ops.newton_schulz(g, steps=1.5),
+        lambda: ops.newton_schulz(g, steps=math.inf),
         lambda: ops.newton_schulz(g, eps=0.0),
         lambda: ops.newton_schulz(g, eps=float("nan")),
         lambda: ops.newton_schulz(g, eps=1e-35),
