@@ -520,36 +520,35 @@ __device__ __forceinline__ void deliver(const Table& tab, const Mat& t, int row,
 constexpr int kPieceLd = 36;                  // floats from row to row of a piece in LDS
 constexpr int kPieceHalfs = 32 * kPieceLd * 2;
 
-// The old values of a piece, 8 to a lane, twice, from the copy in which i runs
-// along rows.
+// A's values at a piece of B, 8 to a lane, twice.
 struct Old {
   f16x8 hi[2], lo[2];
 };
 
-template <int TO>
-__device__ __forceinline__ Old load_old(const Mat& t, int turn, int i0, int j0) {
+__device__ __forceinline__ Old load_old(const Mat& t, int i0, int j0) {
   const int lane = threadIdx.x & 63, r4 = lane >> 2, c8 = (lane & 3) * 8;
   Old o;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const size_t at = place(TO == TO_B ? t.ma : rows_xt(t.np), j0 + h * 16 + r4, i0 + c8);
-    o.hi[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 0) : ws_xt(t, turn, 0)) + at);
+    const size_t at = place(t.ma, j0 + h * 16 + r4, i0 + c8);
+    o.hi[h] = *(const f16x8*)(ws_a(t, 0) + at);
     o.lo[h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (TO != TO_B || t.full)
-      o.lo[h] = *(const f16x8*)((TO == TO_B ? ws_a(t, 1) : ws_xt(t, turn, 1)) + at);
+    if (t.full) o.lo[h] = *(const f16x8*)(ws_a(t, 1) + at);
   }
   return o;
 }
 
-// The 32 x 32 piece at (i0, j0) of A, B, X' or the result: ka * (old value) +
-// kb * (product).  A lane holds 4 neighbouring rows of a column, 4 times; the
-// piece goes through the wave's own LDS so that every global access is 16
-// bytes per lane, side by side.  (Written from the registers, 2 and 8
-// bytes per lane, the tiles' ends took 8 us of 31 at 128 x 128 and 100 us of
-// 360 at 256 x 256.)
+// The 32 x 32 piece at (i0, j0) of A, B, X' or the result: kb * (product), for B
+// with ka * A and kd on the diagonal besides.  B holds a I + b A + c A^2, for
+// then B X is X' and nothing is read here to make it.  (With a X added here
+// instead, 1000 x 4000 twice took 546 us for 532 in fp32, 368 for 352 in bf16.)
+// A lane holds 4 neighbouring rows of a column, 4 times; the piece goes through
+// the wave's own LDS so that every global access is 16 bytes per lane, side by
+// side.  (Written from the registers, 2 and 8 bytes per lane, the tiles' ends
+// took 8 us of 31 at 128 x 128 and 100 us of 360 at 256 x 256.)
 template <int TO>
 __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn, float ka, float kb,
-                                       int i0, int j0, bool mirror, const f32x16& acc,
+                                       float kd, int i0, int j0, bool mirror, const f32x16& acc,
                                        const Old& old, float* lds) {
   const int lane = threadIdx.x & 63;
   const bool turned = t.rows > t.cols;
@@ -568,9 +567,12 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
     float* p = lds + j * kPieceLd + c8;
     const float4 x = *(const float4*)p, y = *(const float4*)(p + 4);
     float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    if (TO != TO_A) {
+    if (TO == TO_B) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) v[k] += ka * ((float)old.hi[h][k] + (float)old.lo[h][k]);
+      for (int k = 0; k < 8; ++k) {
+        v[k] += ka * ((float)old.hi[h][k] + (float)old.lo[h][k]);
+        if (i0 + c8 + k == j0 + j) v[k] += kd;
+      }
     }
     if (TO == TO_END) {
       if (turned) {
@@ -684,7 +686,7 @@ constexpr int most(int a, int b) { return a > b ? a : b; }
 // and for hi hi, of B X hi (hi + lo).
 template <class T, class FULL, class PART, int TO>
 __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, int turn, float ka,
-                                                                  float kb) {
+                                                                  float kb, float kd) {
   constexpr bool SYM = TO == TO_A || TO == TO_B;
   constexpr int HALFS = most(most(lds_halfs<T, FULL, 2, 2>(), T::WAVES * kPieceHalfs),
                              lds_halfs<T, PART, 1, SYM ? 1 : 2>());
@@ -765,17 +767,17 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
       }
     return;
   }
-  // a piece's old values are under way while the piece before it is finished
+  // a piece's values of A are under way while the piece before it is finished
   Old old = {}, next = {};
-  if (TO != TO_A) old = load_old<TO>(t, turn, wi, wj);
+  if (TO == TO_B) old = load_old(t, wi, wj);
 #pragma unroll
   for (int f = 0; f < T::FM; ++f)
 #pragma unroll
     for (int g = 0; g < T::FN; ++g) {
       const int p = f * T::FN + g + 1;
-      if (TO != TO_A && p < T::FM * T::FN)
-        next = load_old<TO>(t, turn, wi + p / T::FN * 32, wj + p % T::FN * 32);
-      finish<TO>(tab, t, turn, ka, kb, wi + f * 32, wj + g * 32, mirror, acc[f][g], old, piece);
+      if (TO == TO_B && p < T::FM * T::FN)
+        next = load_old(t, wi + p / T::FN * 32, wj + p % T::FN * 32);
+      finish<TO>(tab, t, turn, ka, kb, kd, wi + f * 32, wj + g * 32, mirror, acc[f][g], old, piece);
       old = next;
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -809,7 +811,7 @@ __global__ __launch_bounds__(256) void flowml_ns_join(Table tab, int side, float
     }
   }
   const int pi = piece / across, pj = piece - pi * across;
-  finish<TO_A>(tab, t, 0, 0.f, kb, ti * side + pi * 32, tj * side + pj * 32, ti != tj, acc, Old{},
+  finish<TO_A>(tab, t, 0, 0.f, kb, 0.f, ti * side + pi * 32, tj * side + pj * 32, ti != tj, acc, Old{},
                (float*)(lds + wave * kPieceHalfs));
 }
 
@@ -1392,7 +1394,7 @@ Sizes sizes_of(int rows, int cols, Sides s) {
 
 // one product for all matrices of a table; `first` of each is set here
 template <class T, class FULL, class PART, int TO>
-void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
+void product_of(Table& tab, int turn, float ka, float kb, float kd, hipStream_t st) {
   int blocks = 0;
   for (int k = 0; k < tab.count; ++k) {
     Mat& t = tab.mat[k];
@@ -1403,7 +1405,7 @@ void product_of(Table& tab, int turn, float ka, float kb, hipStream_t st) {
                            : (t.mp / T::TM) * (t.np / T::TN);
   }
   hipLaunchKernelGGL((flowml_ns_product<T, FULL, PART, TO>), dim3(blocks), dim3(T::WAVES * 64),
-                     0, st, tab, turn, ka, kb);
+                     0, st, tab, turn, ka, kb, kd);
 }
 
 void join(Sides s, Table& tab, float kb, hipStream_t st) {
@@ -1418,30 +1420,30 @@ void join(Sides s, Table& tab, float kb, hipStream_t st) {
 }
 
 template <int TO>
-void product(Sides s, Table& tab, int turn, float ka, float kb, hipStream_t st) {
+void product(Sides s, Table& tab, int turn, float ka, float kb, float kd, hipStream_t st) {
   // tile, waves, and the depth of LDS for full products and for others
   if constexpr (TO == TO_A || TO == TO_B) {
     const int side = TO == TO_A ? s.a : s.b;
     if (side == 256)
-      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, TO>(tab, turn, ka, kb, kd, st);
     else if (side == 192)
-      product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, TO>(tab, turn, ka, kb, kd, st);
     else if (side == 96)
-      product_of<Tile<96, 96, 3, 1>, Depth<32, 6>, Depth<64, 6>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<96, 96, 3, 1>, Depth<32, 6>, Depth<64, 6>, TO>(tab, turn, ka, kb, kd, st);
     else if (side == 128)
-      product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, TO>(tab, turn, ka, kb, kd, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, kd, st);
     if (TO == TO_A && s.kpart < kWhole) join(s, tab, kb, st);
   } else {
     if (s.m == 256)
-      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, kd, st);
     else if (s.n == 256)
-      product_of<Tile<128, 256, 2, 4>, Depth<32, 3>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<128, 256, 2, 4>, Depth<32, 3>, Depth<32, 3>, TO>(tab, turn, ka, kb, kd, st);
     else if (s.m == 128)
-      product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 3>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 3>, TO>(tab, turn, ka, kb, kd, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, st);
+      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, kd, st);
   }
 }
 
@@ -1623,12 +1625,12 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
     }
     hipLaunchKernelGGL(flowml_ns_first, dim3(blocks), dim3(256), 0, st, tab);
     for (int s = 0; s < steps; ++s) {
-      product<TO_A>(sides, tab, s & 1, 0.f, sa / (sx * sx), st);
-      product<TO_B>(sides, tab, 0, coef[1] * sb / sa, coef[2] * sb / (sa * sa), st);
+      product<TO_A>(sides, tab, s & 1, 0.f, sa / (sx * sx), 0.f, st);
+      product<TO_B>(sides, tab, 0, coef[1] * sb / sa, coef[2] * sb / (sa * sa), coef[0] * sb, st);
       if (s + 1 < steps)
-        product<TO_X>(sides, tab, s & 1, coef[0], 1.f / sb, st);
+        product<TO_X>(sides, tab, s & 1, 0.f, 1.f / sb, 0.f, st);
       else
-        product<TO_END>(sides, tab, s & 1, coef[0] / sx, 1.f / (sb * sx), st);
+        product<TO_END>(sides, tab, s & 1, 0.f, 1.f / (sb * sx), 0.f, st);
     }
   }
 }

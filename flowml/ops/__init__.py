@@ -817,7 +817,7 @@ NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 @functools.lru_cache(maxsize=64)
 def _ns_scale(steps: int, coefficients: Tuple[float, float, float]) -> float:
     """Check the polynomial a·s + b·s³ + c·s⁵ and find the power of two that
-    brings b·A + c·A² into fp16.
+    brings b·A + c·A², and a·I + this, into fp16.
 
     Singular values start in [0, 1]. The kernels hold the iterates in fp16
     pairs scaled by 2^14, so they must stay under 1.9; a polynomial that lets
@@ -853,7 +853,8 @@ def _ns_scale(steps: int, coefficients: Tuple[float, float, float]) -> float:
                 f"coefficients {coefficients!r} let singular values grow to {top:.3g} "
                 "(at most 1.9)"
             )
-    most = crest(lambda s: b * s**2 + c * s**4, (b, 2 * c, 0.0), widest)
+    most = max(abs(a), *(crest(lambda s: k + b * s**2 + c * s**4, (b, 2 * c, 0.0), widest)
+                         for k in (0.0, a)))
     return 2.0 ** min(14, math.floor(math.log2(32768.0 / max(most, 1e-30))))
 
 
