@@ -970,10 +970,10 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
 
   const float sx = kScaleX, sa = kScaleA, sb = poly.scale_b;
   const float to_a = sa / (sx * sx), b_old = poly.b * sb / sa, b_new = poly.c * sb / (sa * sa);
-  const float to_x = 1.f / sb, to_end = 1.f / sx;
+  const float to_x = 1.f / sb, to_end = 1.f / (sb * sx);
   const int row = (lane >> 4) * 4, col = lane & 15;  // 4 rows of a column to a lane
   const int from = (lane >> 4) * 8;                  // of an operand's chunk of 32
-  // A and B: AW pieces of a row of pieces to a wave
+  // A and B, which is a I + b A + c A^2: AW pieces of a row of pieces to a wave
   constexpr int AW = MT * MT / kSmallWaves < 1 ? 1 : MT * MT / kSmallWaves;
   const int ai = wave * AW / MT * 16, aj = wave * AW % MT * 16;
   const bool has_a = wave * AW < MT * MT;
@@ -1022,7 +1022,10 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
           small_multiply<ALL>(
               x[k], small_read(A, lo_a, (aj + q * 16 + col) * ld + from + k * 32), w);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[q][r] = b_new * w[r] + b_old * ((float)h[r] + (float)l[r]);
+        for (int r = 0; r < 4; ++r) {
+          v[q][r] = b_new * w[r] + b_old * ((float)h[r] + (float)l[r]);
+          if (ai + row + r == aj + q * 16 + col) v[q][r] += poly.a * sb;
+        }
       }
     }
     if (!APART) __syncthreads();
@@ -1032,7 +1035,7 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
         put(B, lo_a, (aj + q * 16 + col) * ld + ai + row, v[q]);
     }
     __syncthreads();
-    // X' = a X + B X; a wave takes whole rows of X^T, which nobody else reads here
+    // X' = B X; a wave takes whole rows of X^T, which nobody else reads here
     for (int j = wave * 16; j < np; j += kSmallWaves * 16) {
       Halves y[KC];
 #pragma unroll
@@ -1044,15 +1047,10 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
 #pragma unroll
         for (int k = 0; k < KC; ++k)
           small_multiply<ALL>(small_read(B, lo_a, (p * 16 + col) * ld + from + k * 32), y[k], x[p]);
-        const int at = (j + col) * ld + p * 16 + row;
-        const f16x4 h = *(const f16x4*)(XT + at), l = *(const f16x4*)(XT + lo_x + at);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          x[p][r] = poly.a * ((float)h[r] + (float)l[r]) + to_x * x[p][r];
       }
       if (s + 1 < poly.steps) {
 #pragma unroll
-        for (int p = 0; p < MT; ++p) put(XT, lo_x, (j + col) * ld + p * 16 + row, x[p]);
+        for (int p = 0; p < MT; ++p) put(XT, lo_x, (j + col) * ld + p * 16 + row, x[p] * to_x);
       } else {
 #pragma unroll
         for (int p = 0; p < MT; ++p)
