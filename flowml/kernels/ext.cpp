@@ -4,6 +4,7 @@
 
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <tuple>
@@ -414,6 +415,13 @@ std::tuple<torch::Tensor, torch::Tensor> wgrad_f32(torch::Tensor X,
 
 // ---- layer norm ------------------------------------------------------------
 
+// a new tensor on the current device, without the dispatcher's way there: short
+// calls are bound by the host (layer norm of 256 x 64: 6.5 us instead of 7.0)
+static torch::Tensor fresh(at::IntArrayRef size, const torch::Tensor& like,
+                           at::ScalarType type) {
+  return torch::Tensor(at::detail::empty_cuda(size, type, like.device(), c10::nullopt));
+}
+
 static int float_type(const torch::Tensor& t) {
   switch (t.scalar_type()) {
     case torch::kFloat32: return 0;
@@ -458,9 +466,9 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm(
   const float* b = opt_columns(bias, X, "bias");
   const long long N = X.size(0);
   const int D = (int)X.size(1);
-  auto Y = torch::empty({N, D}, X.options());
-  auto mean = torch::empty({N}, X.options().dtype(torch::kFloat32));
-  auto rstd = torch::empty_like(mean);
+  auto Y = fresh({N, D}, X, X.scalar_type());
+  auto mean = fresh({N}, X, torch::kFloat32);
+  auto rstd = fresh({N}, X, torch::kFloat32);
   if (N)
     launch_layer_norm(type, X.data_ptr(), X.stride(0), g, b, Y.data_ptr(),
                       mean.data_ptr<float>(), rstd.data_ptr<float>(), N, D,
@@ -489,11 +497,10 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_grad(
                 "mean and rstd must be one contiguous f32 per row");
   const at::cuda::OptionalCUDAGuard guard(X.device());
   const float* g = opt_columns(weight, X, "weight");
-  const auto f32 = X.options().dtype(torch::kFloat32);
-  auto dX = torch::empty({N, D}, X.options());
-  auto dW = torch::empty({D}, f32);
-  auto dB = torch::empty({D}, f32);
-  auto part = torch::empty({layer_norm_grad_slabs(type, N, D), 2, D}, f32);
+  auto dX = fresh({N, D}, X, X.scalar_type());
+  auto dW = fresh({D}, X, torch::kFloat32);
+  auto dB = fresh({D}, X, torch::kFloat32);
+  auto part = fresh({layer_norm_grad_slabs(type, N, D), 2, D}, X, torch::kFloat32);
   launch_layer_norm_grad(type, dY.data_ptr(), dY.stride(0), X.data_ptr(),
                          X.stride(0), act ? Y->data_ptr() : nullptr,
                          act ? Y->stride(0) : 0, mean.data_ptr<float>(),
@@ -555,9 +562,9 @@ static void muon_call(const std::vector<torch::Tensor>& g,
   // three products everywhere unless the result is rounded to bf16
   const int full = wtype != 1;
   std::vector<int> scratch(3 * n);
-  auto ws = torch::empty(
+  auto ws = fresh(
       {muon_workspace((int)n, rows.data(), cols.data(), full, scratch.data())},
-      g[0].options().dtype(torch::kUInt8));
+      g[0], torch::kUInt8);
   launch_muon((int)n, rows.data(), cols.data(), gp.data(),
               mom.empty() ? nullptr : mp.data(), wp.data(),
               mom.empty() ? nullptr : sp.data(), gtype, wtype, (float)mu,
