@@ -30,6 +30,8 @@
 #include <hip/hip_bf16.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 namespace {
 
 enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
@@ -117,45 +119,44 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// Threads of a block whose rows take `lanes` lanes: one row, or what four waves
-// hold.
-constexpr int block_of(int lanes) { return lanes > 64 ? lanes : 256; }
+// Rows of up to a wave's lanes share blocks of four waves; a longer row has a
+// block to itself, of as many waves as it needs (LANES = 0: blockDim.x).
+constexpr int kWaves = 16;  // most waves of a block
+constexpr int block_of(int lanes) { return lanes ? 256 : kWaves * 64; }
+
+// `lds` of the sums below: words that no wave still reads (callers alternate),
+// 0 where the block has no wave.
+__device__ __forceinline__ void clear_sums(float* lds, int n) {
+  if ((int)threadIdx.x < n) lds[threadIdx.x] = 0.f;
+  __syncthreads();
+}
 
 // Sum over the lanes that share a row: part of a wave, or the whole block.
-// `lds`: LANES / 64 floats that no wave still reads (callers alternate).
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v, float* lds) {
-  if constexpr (LANES <= 64) {
+  if constexpr (LANES > 0) {
     return lanes_sum<LANES>(v);
   } else {
     v = lanes_sum<64>(v);
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
     __syncthreads();
-    float s = 0.f;
-#pragma unroll
-    for (int k = 0; k < LANES / 64; ++k) s += lds[k];
-    return s;
+    return lanes_sum<kWaves>(lds[threadIdx.x % kWaves]);
   }
 }
 
-// Two such sums behind one barrier; `lds`: 2 * LANES / 64 floats.
+// Two such sums behind one barrier.
 template <int LANES>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float* lds) {
-  a = lanes_sum<(LANES < 64 ? LANES : 64)>(a);
-  b = lanes_sum<(LANES < 64 ? LANES : 64)>(b);
-  if constexpr (LANES > 64) {
-    constexpr int W = LANES / 64;
+  a = lanes_sum<(LANES ? LANES : 64)>(a);
+  b = lanes_sum<(LANES ? LANES : 64)>(b);
+  if constexpr (LANES == 0) {
     if ((threadIdx.x & 63) == 0) {
       lds[threadIdx.x >> 6] = a;
-      lds[W + (threadIdx.x >> 6)] = b;
+      lds[kWaves + (threadIdx.x >> 6)] = b;
     }
     __syncthreads();
-    a = b = 0.f;
-#pragma unroll
-    for (int k = 0; k < W; ++k) {
-      a += lds[k];
-      b += lds[W + k];
-    }
+    a = lanes_sum<kWaves>(lds[threadIdx.x % kWaves]);
+    b = lanes_sum<kWaves>(lds[kWaves + threadIdx.x % kWaves]);
   }
 }
 
@@ -183,18 +184,19 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm(
     const float* __restrict__ beta, T* __restrict__ Y, float* __restrict__ mean,
     float* __restrict__ rstd, long long N, int D, float eps, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
-  constexpr int BLOCK = block_of(LANES);
-  constexpr int GROUPS = BLOCK / LANES;
-  __shared__ float s_red[2][LANES > 64 ? LANES / 64 : 1];
-  const int lane = threadIdx.x % LANES;
-  const int group = threadIdx.x / LANES;
+  constexpr int GROUPS = LANES ? 256 / LANES : 1;
+  __shared__ float s_red[2][LANES ? 1 : kWaves];
+  const int lanes = LANES ? LANES : blockDim.x;
+  const int lane = threadIdx.x % lanes;
+  const int group = threadIdx.x / lanes;
   const float d = (float)D;
+  if (!LANES) clear_sums(s_red[0], 2 * kWaves);
 
   float g[NV][VEC], b[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_columns<VEC>(gamma, (i * LANES + lane) * VEC, D, 1.f, g[i]);
-    load_columns<VEC>(beta, (i * LANES + lane) * VEC, D, 0.f, b[i]);
+    load_columns<VEC>(gamma, (i * lanes + lane) * VEC, D, 1.f, g[i]);
+    load_columns<VEC>(beta, (i * lanes + lane) * VEC, D, 0.f, b[i]);
   }
 
   const long long stride = (long long)gridDim.x * GROUPS;
@@ -205,7 +207,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm(
     const T* x = X + (row < N ? row : N - 1) * ldx;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * VEC;
+      const int c = (i * lanes + lane) * VEC;
       raw[i] = load_raw<T>(x + c, D - c);
     }
   };
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm(
     float q = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * VEC;
+      const int c = (i * lanes + lane) * VEC;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         v[i][k] -= mu;
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm(
       T* y = Y + row * D;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LANES + lane) * VEC;
+        const int c = (i * lanes + lane) * VEC;
         if (c < D) {
 #pragma unroll
           for (int k = 0; k < VEC; ++k)
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_long(
     const float* __restrict__ beta, T* __restrict__ Y, float* __restrict__ mean,
     float* __restrict__ rstd, long long N, int D, float eps, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
-  __shared__ float s_red[2][16];
+  __shared__ float s_red[2][kWaves];
   const float d = (float)D;
   for (long long row = blockIdx.x; row < N; row += gridDim.x) {
     const T* x = X + row * ldx;
@@ -272,14 +274,14 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_long(
 #pragma unroll
       for (int k = 0; k < VEC; ++k) s += v[k];
     }
-    const float mu = row_sum<1024>(s, s_red[0]) / d;
+    const float mu = row_sum<0>(s, s_red[0]) / d;
     float q = 0.f;
     for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
       load_piece<T>(x + c, D - c, v);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) q += c + k < D ? (v[k] - mu) * (v[k] - mu) : 0.f;
     }
-    const float r = 1.f / sqrtf(row_sum<1024>(q, s_red[1]) / d + eps);
+    const float r = 1.f / sqrtf(row_sum<0>(q, s_red[1]) / d + eps);
     T* y = Y + row * D;
     for (int c = threadIdx.x * VEC; c < D; c += 1024 * VEC) {
       float g[VEC], b[VEC];
@@ -308,19 +310,20 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
     const float* __restrict__ rstd, const float* __restrict__ gamma,
     T* __restrict__ dX, float* __restrict__ part, long long N, int D, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
-  constexpr int BLOCK = block_of(LANES);
-  constexpr int GROUPS = BLOCK / LANES;
+  constexpr int GROUPS = LANES ? 256 / LANES : 1;
   constexpr int WIDTH = LANES * NV * VEC;
-  __shared__ float s_red[2][LANES > 64 ? LANES / 32 : 1];
-  __shared__ float s_cols[GROUPS > 1 ? BLOCK * NV * VEC : 1];
-  const int lane = threadIdx.x % LANES;
-  const int group = threadIdx.x / LANES;
+  __shared__ float s_red[2][LANES ? 1 : 2 * kWaves];
+  __shared__ float s_cols[GROUPS > 1 ? 256 * NV * VEC : 1];
+  const int lanes = LANES ? LANES : blockDim.x;
+  const int lane = threadIdx.x % lanes;
+  const int group = threadIdx.x / lanes;
   const float d = (float)D;
+  if (!LANES) clear_sums(s_red[0], 4 * kWaves);
 
   float g[NV][VEC], dg[NV][VEC], db[NV][VEC];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    load_columns<VEC>(gamma, (i * LANES + lane) * VEC, D, 1.f, g[i]);
+    load_columns<VEC>(gamma, (i * lanes + lane) * VEC, D, 1.f, g[i]);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) dg[i][k] = db[i][k] = 0.f;
   }
@@ -334,14 +337,14 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
     next_r = rstd[row];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * VEC;
+      const int c = (i * lanes + lane) * VEC;
       rx[i] = load_raw<T>(X + row * ldx + c, D - c);
       rd[i] = load_raw<T>(dY + row * lddy + c, D - c);
       if constexpr (ACT) ry[i] = load_raw<T>(Y + row * ldy + c, D - c);
     }
   };
   // with 16 values of four arrays to a lane, 128 registers do not hold two rows
-  constexpr bool AHEAD = LANES < 1024 || NV * VEC < 16;
+  constexpr bool AHEAD = LANES || NV * VEC < 16;
   if (AHEAD) fetch((long long)blockIdx.x * GROUPS + group);
   int turn = 0;  // the block-wide sums of two neighbouring rows use other words
   for (long long row0 = (long long)blockIdx.x * GROUPS; row0 < N; row0 += stride, turn ^= 1) {
@@ -353,7 +356,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
     float s = 0.f, q = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * VEC;
+      const int c = (i * lanes + lane) * VEC;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         dz[i][k] = (float)rd[i][k];
@@ -376,7 +379,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
     if (live) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int c = (i * LANES + lane) * VEC;
+        const int c = (i * lanes + lane) * VEC;
         if (c < D) {
           float o[VEC];
 #pragma unroll
@@ -392,7 +395,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
   if constexpr (GROUPS == 1) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * LANES + lane) * VEC;
+      const int c = (i * lanes + lane) * VEC;
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
         if (c + k < D) {
@@ -408,9 +411,9 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < VEC; ++k)
-          s_cols[group * WIDTH + (i * LANES + lane) * VEC + k] = half ? db[i][k] : dg[i][k];
+          s_cols[group * WIDTH + (i * lanes + lane) * VEC + k] = half ? db[i][k] : dg[i][k];
       __syncthreads();
-      for (int c = threadIdx.x; c < D; c += BLOCK) {
+      for (int c = threadIdx.x; c < D; c += 256) {
         float t = 0.f;
         for (int o = 0; o < GROUPS; ++o) t += s_cols[o * WIDTH + c];
         slab[half * D + c] = t;
@@ -427,7 +430,7 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
     const float* __restrict__ rstd, const float* __restrict__ gamma,
     T* __restrict__ dX, long long N, int D, int act, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
-  __shared__ float s_red[2][32];
+  __shared__ float s_red[2][2 * kWaves];
   const float d = (float)D;
   int turn = 0;
   for (long long row = blockIdx.x; row < N; row += gridDim.x, turn ^= 1) {
@@ -455,7 +458,7 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
         if (look) store_piece<T>(dX + row * D + c, D - c, x, stream);
       }
       if (look == 0) {
-        row_sum2<1024>(s, q, s_red[turn]);
+        row_sum2<0>(s, q, s_red[turn]);
         s /= d;
         q /= d;
       }
@@ -530,24 +533,41 @@ constexpr int kCUs = 256;
 // there by whoever reads it next
 bool streams(long long N, int D, size_t size) { return N * D * (long long)size > (128LL << 20); }
 
-// Lanes and pieces for a row of D values of VEC to the piece: one piece per
-// lane up to a wave, then more pieces, then more waves.
+// Lanes and pieces for a row of D values of VEC to the piece: up to a wave, the
+// smallest power of two with one piece to a lane; beyond, waves and pieces by
+// the rules below.
 struct Shape {
   int lanes, nv;
 };
 
-// Forward: the smallest block whose lanes hold the row in 16 values each (with
-// as many weights and biases), for a CU then works on several rows and their
-// barriers do not meet.
+// Forward: up to 16 values to a lane (as many weights and biases).  Lanes
+// without a piece cost their share of the row, and waves that wait for each
+// other 3 % apiece (us, lanes x pieces; 5003 x 2051 f32: 192 x 3 14, 256 x 3
+// 16, 320 x 2 16, 576 x 1 18; 8000 x 5000 f16: 320 x 2 34, 640 x 1 40).
 Shape forward_shape(int D, int vec) {
   const int pieces = (D + vec - 1) / vec;
   for (int l = 1; l <= 64; l *= 2)
     if (pieces <= l) return {l, 1};
-  if (pieces <= 128) return {64, 2};
-  for (int l = 256; l <= 1024; l *= 2)
-    for (int v = 1; v <= 16 / vec; ++v)
-      if (pieces <= l * v) return {l, v};
-  return {0, 0};
+  Shape best = {0, 0};
+  int least = 1 << 30;
+  for (int v = 1; v <= 16 / vec; ++v) {
+    const int w = std::max(2, (pieces + 64 * v - 1) / (64 * v)), cost = w * v * (100 + 3 * w);
+    if (w <= kWaves && cost < least) {
+      least = cost;
+      best = {w * 64, v};
+    }
+  }
+  return best;
+}
+
+// Blocks of the forward pass that a CU holds: by the registers of so many
+// values, and a place less on its four SIMDs where a block's waves do not
+// divide among them.  More wait for a second round (20000 x 2056 bf16, 320
+// lanes: 40 us with 5, 48 with 6).
+int forward_blocks(Shape s, int vec) {
+  const int w = s.lanes / 64, values = s.nv * vec;
+  const int places = 4 * (values <= 8 ? 8 : values <= 12 ? 6 : vec == 8 ? 5 : 4);
+  return std::max(1, (w < 4 || w % 4 == 0 ? places : places - 4) / w);
 }
 
 // Backward: one piece to a lane as far as a block goes, for four arrays and two
@@ -559,14 +579,21 @@ Shape backward_shape(int D, int vec) {
   for (int l = 1; l <= 64; l *= 2)
     if (pieces <= l) return {l, 1};
   if (pieces <= 128) return {64, 2};
-  for (int l = 256; l <= 1024; l *= 2)
-    if (pieces <= l) return {l, 1};
-  for (int v = 2; v <= 16 / vec; v *= 2)
-    if (pieces <= 1024 * v) return {1024, v};
+  for (int v = 1; v <= 16 / vec; v *= 2) {
+    const int w = (pieces + 64 * v - 1) / (64 * v);
+    if (w <= kWaves) return {w * 64, v};
+  }
   return {0, 0};
 }
 
-int rows_per_block(Shape s) { return block_of(s.lanes) / s.lanes; }
+// Its blocks to a CU: what registers allow, and few, for each leaves sums to add
+// (20000 x 2056 bf16, 320 lanes: 67 us with 3, 83 with 4).
+int backward_blocks(Shape s, int vec) {
+  return s.lanes <= 64 ? 4 : std::max(1, (s.nv * vec == 4 ? 20 : 16) / (s.lanes / 64));
+}
+
+int rows_per_block(Shape s) { return s.lanes > 64 ? 1 : 256 / s.lanes; }
+int threads_of(Shape s) { return s.lanes > 64 ? s.lanes : 256; }
 
 template <typename T>
 void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, float* mean,
@@ -581,12 +608,12 @@ void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, fl
   }
   const int rpb = rows_per_block(s);
   const long long want = (N + rpb - 1) / rpb;
-  const long long most = (long long)kCUs * (s.lanes > 64 ? 8 : 16);
+  const long long most = kCUs * (s.lanes > 64 ? forward_blocks(s, Piece<T>::VEC) : 16);
   const int grid = (int)(want < most ? want : most);
-#define LN_CASE(L, V)                                                              \
-  if (s.lanes == L && s.nv == V)                                                   \
-    hipLaunchKernelGGL((flowml_layer_norm<T, L, V>), dim3(grid),                   \
-                       dim3(block_of(L)), 0, st, X, ldx, g, b, Y, mean, rstd, N, D, eps, act, stream)
+#define LN_CASE(L, V)                                                                           \
+  if ((s.lanes > 64 ? 0 : s.lanes) == L && s.nv == V)                                           \
+    hipLaunchKernelGGL((flowml_layer_norm<T, L, V>), dim3(grid), dim3(threads_of(s)), 0, st, X, \
+                       ldx, g, b, Y, mean, rstd, N, D, eps, act, stream)
   LN_CASE(1, 1);
   LN_CASE(2, 1);
   LN_CASE(4, 1);
@@ -594,19 +621,11 @@ void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, fl
   LN_CASE(16, 1);
   LN_CASE(32, 1);
   LN_CASE(64, 1);
-  LN_CASE(64, 2);
-  LN_CASE(256, 1);
-  LN_CASE(256, 2);
+  LN_CASE(0, 1);
+  LN_CASE(0, 2);
   if constexpr (Piece<T>::VEC == 4) {
-    LN_CASE(256, 3);
-    LN_CASE(256, 4);
-    LN_CASE(512, 3);
-    LN_CASE(512, 4);
-    LN_CASE(1024, 3);
-    LN_CASE(1024, 4);
-  } else {
-    LN_CASE(512, 2);
-    LN_CASE(1024, 2);
+    LN_CASE(0, 3);
+    LN_CASE(0, 4);
   }
 #undef LN_CASE
 }
@@ -623,7 +642,7 @@ int grad_slabs(long long N, int D, int vec) {
   } else {
     const int rpb = rows_per_block(s);
     want = (N + rpb - 1) / rpb;
-    most = kCUs * (s.lanes == 1024 ? 1 : s.lanes == 512 ? 2 : 4);
+    most = kCUs * backward_blocks(s, vec);
   }
   return (int)(want < most ? want : most);
 }
@@ -643,15 +662,15 @@ void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y
     hipLaunchKernelGGL((flowml_layer_norm_grad_cols<T>), dim3((D + 255) / 256, slabs),
                        dim3(256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, part, N, D, chunk, act);
   } else if (slabs) {
-#define LN_CASE1(L, V, A)                                                               \
-  hipLaunchKernelGGL((flowml_layer_norm_grad<T, L, V, A>), dim3(slabs),                 \
-                     dim3(block_of(L)), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act, stream)
-#define LN_CASE(L, V)                \
-  if (s.lanes == L && s.nv == V) {   \
-    if (act)                         \
-      LN_CASE1(L, V, true);          \
-    else                             \
-      LN_CASE1(L, V, false);         \
+#define LN_CASE1(L, V, A)                                                                     \
+  hipLaunchKernelGGL((flowml_layer_norm_grad<T, L, V, A>), dim3(slabs), dim3(threads_of(s)),  \
+                     0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act, stream)
+#define LN_CASE(L, V)                                     \
+  if ((s.lanes > 64 ? 0 : s.lanes) == L && s.nv == V) {   \
+    if (act)                                              \
+      LN_CASE1(L, V, true);                               \
+    else                                                  \
+      LN_CASE1(L, V, false);                              \
   }
     LN_CASE(1, 1);
     LN_CASE(2, 1);
@@ -661,11 +680,9 @@ void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y
     LN_CASE(32, 1);
     LN_CASE(64, 1);
     LN_CASE(64, 2);
-    LN_CASE(256, 1);
-    LN_CASE(512, 1);
-    LN_CASE(1024, 1);
-    LN_CASE(1024, 2);
-    if constexpr (Piece<T>::VEC == 4) LN_CASE(1024, 4);
+    LN_CASE(0, 1);
+    LN_CASE(0, 2);
+    if constexpr (Piece<T>::VEC == 4) LN_CASE(0, 4);
 #undef LN_CASE
 #undef LN_CASE1
   }
