@@ -63,8 +63,10 @@ __device__ __forceinline__ void load_piece(const T* p, int left, float* v) {
   for (int k = 0; k < Piece<T>::VEC; ++k) v[k] = (float)r[k];
 }
 
-// stream: past the caches, for results that do not fit them (1M x 128 bf16:
-// 95 us instead of 113; loads past the caches lose as much).
+// stream: past the caches, for results that do not fit them (1M x 128 bf16: 87
+// us instead of 102, 200000 x 500 bf16 75 instead of 97; loads past the caches
+// lose as much).  The empty statements keep the compiler from making one store
+// of the two, which is not past anything.
 template <typename T>
 __device__ __forceinline__ void store_piece(T* p, int left, const float* v, bool stream) {
   constexpr int VEC = Piece<T>::VEC;
@@ -72,10 +74,13 @@ __device__ __forceinline__ void store_piece(T* p, int left, const float* v, bool
     typename Piece<T>::raw r;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) r[k] = (T)v[k];
-    if (stream)
+    if (stream) {
+      asm volatile("" ::: "memory");
       __builtin_nontemporal_store(r, reinterpret_cast<typename Piece<T>::vec*>(p));
-    else
+      asm volatile("" ::: "memory");
+    } else {
       *reinterpret_cast<typename Piece<T>::vec*>(p) = r;
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
@@ -428,7 +433,7 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
     const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
     const T* __restrict__ Y, long long ldy, const float* __restrict__ mean,
     const float* __restrict__ rstd, const float* __restrict__ gamma,
-    T* __restrict__ dX, long long N, int D, int act, bool stream) {
+    T* __restrict__ dX, long long N, int D, int act) {
   constexpr int VEC = Piece<T>::VEC;
   __shared__ float s_red[2][2 * kWaves];
   const float d = (float)D;
@@ -455,7 +460,7 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
             x[k] = r * (p - s - xh * q);
           }
         }
-        if (look) store_piece<T>(dX + row * D + c, D - c, x, stream);
+        if (look) store_piece<T>(dX + row * D + c, D - c, x, false);
       }
       if (look == 0) {
         row_sum2<0>(s, q, s_red[turn]);
@@ -529,9 +534,14 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_slabs(
 
 constexpr int kCUs = 256;
 
-// whether a result is too large for the 256 MB of last-level cache to be found
-// there by whoever reads it next
-bool streams(long long N, int D, size_t size) { return N * D * (long long)size > (128LL << 20); }
+// Whether a result is too large for the 256 MB of last-level cache to be found
+// there by whoever reads it next.  Short rows with ragged ends go through the
+// caches all the same, which make whole lines of them (2M x 41 f32: 156 us, past
+// them 165).
+bool streams(long long N, int D, size_t size) {
+  const long long row = D * (long long)size;
+  return N * row >= (128LL << 20) && (row >= 256 || row % 16 == 0);
+}
 
 // Lanes and pieces for a row of D values of VEC to the piece: up to a wave, the
 // smallest power of two with one piece to a lane; beyond, waves and pieces by
@@ -657,7 +667,7 @@ void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y
   if (slabs && !s.lanes) {
     const int grid = (int)(N < 2 * kCUs ? N : 2 * kCUs);
     hipLaunchKernelGGL((flowml_layer_norm_grad_long<T>), dim3(grid), dim3(1024), 0, st, dY, lddy, X,
-                       ldx, Y, ldy, mean, rstd, g, dX, N, D, act, stream);
+                       ldx, Y, ldy, mean, rstd, g, dX, N, D, act);
     const long long chunk = (N + slabs - 1) / slabs;
     hipLaunchKernelGGL((flowml_layer_norm_grad_cols<T>), dim3((D + 255) / 256, slabs),
                        dim3(256), 0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, part, N, D, chunk, act);
