@@ -1279,12 +1279,13 @@ int pad(int v, int t) { return (v + t - 1) / t * t; }
 // Tile sides of a call's products, and the parts of K of A.  Large tiles run at
 // twice the rate of small ones, but are worth it only if there are enough for
 // the 256 CUs.  Measured, us a product (tiles):
-//   A of 1024 x 4096, full:    64 (136) 25   96 (66) 49    128 (36) 57
-//   A of 2048 x 4096, hi hi:   64 (528) 44   96 (253) 29   128 (136) 32  192 (66) 51
-//   A of 4096 x 4096, hi hi:   96 (946) 101  128 (528) 101 192 (253) 73  256 (136) 93
-//   B X of 1024 x 4096, full:  64 (1024) 36  128 (256) 29  256 (64) 62
-//   two of these:              128 (512) 75  128 x 256 (256) 66
-//   B X of 4096 x 4096:        128 (1024) 266              256 (256) 230
+//   A of 1024 x 4096, full:    64 (136) 28   96 (66) 53    128 (36) 58
+//   A of 2048 x 4096, hi hi:   64 (528) 47   96 (253) 37   128 (136) 36  192 (66) 53
+//   its A^2:                   64 (528) 26   96 (253) 22   128 (136) 24  192 (66) 35
+//   A of 4096 x 4096, hi hi:   96 (946) 110  128 (528) 98  192 (253) 73  256 (136) 90
+//   B X of 1024 x 4096, full:  64 (1024) 31  128 (256) 26  256 (64) 55
+//   two of these:              128 (512) 50  128 x 256 (256) 48
+//   B X of 4096 x 4096:        128 (1024) 251              256 (256) 208
 // For A and B a side is taken by the time that follows from such figures.  Where
 // A has few tiles and a long K, blocks take parts of K and a launch more joins
 // them: two of 1024 x 4096, full, take 50 us as 272 tiles of 64, and 32 + 6 us
