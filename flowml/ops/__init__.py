@@ -573,7 +573,7 @@ def mlp_forward(
     norms: Optional[List[Tuple[torch.Tensor, torch.Tensor]]] = None,
 ) -> torch.Tensor:
     """Forward pass: N×K logits (no softmax). Reference site: BLAS.gemm in
-    spark ml/ann AffineLayer (SURVEY.md §2.4 K5).
+    spark ml/ann AffineLayer.
 
     ``norms``: (weight, bias) of a layer norm between each hidden layer's
     product and its activation.
