@@ -57,7 +57,7 @@ void launch_wgrad_f32_splitk(const float*, const float*, float*, long long,
 void launch_layer_norm(int, const void*, long long, const float*, const float*,
                        void*, float*, float*, long long, int, float, int,
                        void*);
-int layer_norm_grad_slabs(int, long long, int);
+int layer_norm_grad_slabs(int, long long, int, int);
 void launch_layer_norm_grad(int, const void*, long long, const void*,
                             long long, const void*, long long, const float*,
                             const float*, const float*, void*, float*, float*,
@@ -500,7 +500,7 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> layer_norm_grad(
   auto dX = fresh({N, D}, X, X.scalar_type());
   auto dW = fresh({D}, X, torch::kFloat32);
   auto dB = fresh({D}, X, torch::kFloat32);
-  auto part = fresh({layer_norm_grad_slabs(type, N, D), 2, D}, X, torch::kFloat32);
+  auto part = fresh({layer_norm_grad_slabs(type, N, D, (int)act), 2, D}, X, torch::kFloat32);
   launch_layer_norm_grad(type, dY.data_ptr(), dY.stride(0), X.data_ptr(),
                          X.stride(0), act ? Y->data_ptr() : nullptr,
                          act ? Y->stride(0) : 0, mean.data_ptr<float>(),

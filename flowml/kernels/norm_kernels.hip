@@ -548,21 +548,33 @@ bool streams(long long N, int D, size_t size) {
   return N * row >= (128LL << 20) && (row >= 256 || row % 16 == 0);
 }
 
-// Lanes and pieces for a row of D values of VEC to the piece: up to a wave, the
-// smallest power of two with one piece to a lane; beyond, waves and pieces by
-// the rules below.
+// Lanes and pieces for a row of D values of VEC to the piece.  Up to a wave, a
+// power of two with one piece to a lane, unless that leaves a quarter or more of
+// the lanes idle and three pieces to fewer lanes do not: rows that share a wave
+// are what keeps memory busy.
 struct Shape {
   int lanes, nv;
 };
 
-// Forward: up to 16 values to a lane (as many weights and biases).  Lanes
-// without a piece cost their share of the row, and waves that wait for each
-// other 3 % apiece (us, lanes x pieces; 5003 x 2051 f32: 192 x 3 14, 256 x 3
-// 16, 320 x 2 16, 576 x 1 18; 8000 x 5000 f16: 320 x 2 34, 640 x 1 40).
+// pieces that three to each of `lanes` hold, and one to each of twice as many does not
+bool three_fit(int pieces, int lanes) { return pieces > 2 * lanes && pieces <= 3 * lanes; }
+
+// Forward, beyond a wave's lanes: two or three pieces to them (112500 x 800 bf16:
+// 68 us, with two waves 79; 150000 x 600 bf16: 32 lanes x 3 71, two waves 99; of
+// f32 60 and 67 to 76), then up to 16 values to a lane (as many weights and
+// biases).  Lanes without a piece cost their share of the row there, and waves
+// that wait for each other 3 % apiece (us, lanes x pieces; 5003 x 2051 f32: 192 x
+// 3 14, 256 x 3 16, 320 x 2 16, 576 x 1 18; 8000 x 5000 f16: 320 x 2 34, 640 x 1
+// 40).  Three pieces to a part of a wave: 300000 x 300 bf16 97 and 81 us; not of
+// f32 (340909 x 132: 74 and 76).
 Shape forward_shape(int D, int vec) {
   const int pieces = (D + vec - 1) / vec;
+  if (vec == 8 && three_fit(pieces, 16)) return {16, 3};
   for (int l = 1; l <= 64; l *= 2)
     if (pieces <= l) return {l, 1};
+  if (three_fit(pieces, 32)) return {32, 3};
+  if (pieces <= 128) return {64, 2};
+  if (pieces <= 192) return {64, 3};
   Shape best = {0, 0};
   int least = 1 << 30;
   for (int v = 1; v <= 16 / vec; ++v) {
@@ -585,15 +597,23 @@ int forward_blocks(Shape s, int vec) {
   return std::max(1, (w < 4 || w % 4 == 0 ? places : places - 4) / w);
 }
 
-// Backward: one piece to a lane as far as a block goes, for four arrays and two
-// sums of columns live in registers (20000 x 2056 bf16: 61 us with one piece to
-// 320 lanes, 70 with two to 192) -- but two to a wave before two waves share a
-// row (20000 x 1000 bf16: 30 us, with 128 lanes 36; 100000 rows 150 and 138).
-Shape backward_shape(int D, int vec) {
+// Backward.  Three pieces to fewer lanes serve all but f32 with an activation,
+// which has a third array (300000 x 300 bf16 186 and 140 us, 150000 x 600 bf16 181
+// and 128, 561600 x 80 f32 131 and 109; 236842 x 190 f32 with relu 163 and 184),
+// four pieces to half a wave 16-bit rows without one (90000 x 1000 bf16: 110 us,
+// 64 x 2 132; with relu 159 and 151).  Beyond, one piece to a lane as far as a
+// block goes, for four arrays and two sums of columns live in registers (20000 x
+// 2056 bf16: 61 us with one piece to 320 lanes, 70 with two to 192).
+Shape backward_shape(int D, int vec, bool act) {
   const int pieces = (D + vec - 1) / vec;
+  const bool three = vec == 8 || !act;
+  for (int l = 8; three && l <= 16; l *= 2)
+    if (three_fit(pieces, l)) return {l, 3};
   for (int l = 1; l <= 64; l *= 2)
     if (pieces <= l) return {l, 1};
-  if (pieces <= 128) return {64, 2};
+  if (vec == 8 && three_fit(pieces, 32)) return {32, 3};
+  if (pieces <= 128) return vec == 8 && !act ? Shape{32, 4} : Shape{64, 2};
+  if (three && pieces <= 192) return {64, 3};
   for (int v = 1; v <= 16 / vec; v *= 2) {
     const int w = (pieces + 64 * v - 1) / (64 * v);
     if (w <= kWaves) return {w * 64, v};
@@ -636,18 +656,23 @@ void forward(const T* X, long long ldx, const float* g, const float* b, T* Y, fl
   LN_CASE(16, 1);
   LN_CASE(32, 1);
   LN_CASE(64, 1);
+  LN_CASE(32, 3);
+  LN_CASE(64, 2);
+  LN_CASE(64, 3);
   LN_CASE(0, 1);
   LN_CASE(0, 2);
   if constexpr (Piece<T>::VEC == 4) {
     LN_CASE(0, 3);
     LN_CASE(0, 4);
+  } else {
+    LN_CASE(16, 3);
   }
 #undef LN_CASE
 }
 
 // slabs (and blocks) of the backward pass
-int grad_slabs(long long N, int D, int vec) {
-  const Shape s = backward_shape(D, vec);
+int grad_slabs(long long N, int D, int vec, bool act) {
+  const Shape s = backward_shape(D, vec, act);
   long long want, most;
   if (!s.lanes) {
     // columns kernel: 256 columns to a block, chunks of rows to fill the chip
@@ -666,9 +691,9 @@ template <typename T>
 void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y, long long ldy,
               const float* mean, const float* rstd, const float* g, T* dX, float* part,
               float* dg, float* db, long long N, int D, int act, hipStream_t st) {
-  const Shape s = backward_shape(D, Piece<T>::VEC);
+  const Shape s = backward_shape(D, Piece<T>::VEC, act);
   const bool stream = streams(N, D, sizeof(T));
-  const int slabs = N ? grad_slabs(N, D, Piece<T>::VEC) : 0;
+  const int slabs = N ? grad_slabs(N, D, Piece<T>::VEC, act) : 0;
   if (slabs && !s.lanes) {
     const int grid = (int)(N < 2 * kCUs ? N : 2 * kCUs);
     hipLaunchKernelGGL((flowml_layer_norm_grad_long<T>), dim3(grid), dim3(1024), 0, st, dY, lddy, X,
@@ -680,24 +705,35 @@ void backward(const T* dY, long long lddy, const T* X, long long ldx, const T* Y
 #define LN_CASE1(L, V, A)                                                                     \
   hipLaunchKernelGGL((flowml_layer_norm_grad<T, L, V, A>), dim3(slabs), dim3(threads_of(s)),  \
                      0, st, dY, lddy, X, ldx, Y, ldy, mean, rstd, g, dX, part, N, D, act, stream)
-#define LN_CASE(L, V)                                     \
-  if ((s.lanes > 64 ? 0 : s.lanes) == L && s.nv == V) {   \
-    if (act)                                              \
-      LN_CASE1(L, V, true);                               \
-    else                                                  \
-      LN_CASE1(L, V, false);                              \
-  }
-    LN_CASE(1, 1);
-    LN_CASE(2, 1);
-    LN_CASE(4, 1);
-    LN_CASE(8, 1);
-    LN_CASE(16, 1);
-    LN_CASE(32, 1);
-    LN_CASE(64, 1);
-    LN_CASE(64, 2);
-    LN_CASE(0, 1);
-    LN_CASE(0, 2);
-    if constexpr (Piece<T>::VEC == 4) LN_CASE(0, 4);
+#define LN_CASE(L, V, A) \
+  if ((s.lanes > 64 ? 0 : s.lanes) == L && s.nv == V && (act != 0) == A) LN_CASE1(L, V, A)
+#define LN_CASES(L, V)   \
+  LN_CASE(L, V, false);  \
+  LN_CASE(L, V, true)
+    LN_CASES(1, 1);
+    LN_CASES(2, 1);
+    LN_CASES(4, 1);
+    LN_CASES(8, 1);
+    LN_CASES(16, 1);
+    LN_CASES(32, 1);
+    LN_CASES(64, 1);
+    LN_CASES(0, 1);
+    LN_CASES(0, 2);
+    LN_CASE(8, 3, false);
+    LN_CASE(16, 3, false);
+    LN_CASE(64, 2, true);
+    LN_CASE(64, 3, false);
+    if constexpr (Piece<T>::VEC == 4) {
+      LN_CASE(64, 2, false);
+      LN_CASES(0, 4);
+    } else {
+      LN_CASE(8, 3, true);
+      LN_CASE(16, 3, true);
+      LN_CASES(32, 3);
+      LN_CASE(32, 4, false);
+      LN_CASE(64, 3, true);
+    }
+#undef LN_CASES
 #undef LN_CASE
 #undef LN_CASE1
   }
@@ -724,8 +760,8 @@ extern "C" void launch_layer_norm(int type, const void* X, long long ldx, const 
 }
 
 // slabs of 2 * D floats that the backward pass wants as a workspace
-extern "C" int layer_norm_grad_slabs(int type, long long N, int D) {
-  return N ? grad_slabs(N, D, type == T_F32 ? 4 : 8) : 0;
+extern "C" int layer_norm_grad_slabs(int type, long long N, int D, int act) {
+  return N ? grad_slabs(N, D, type == T_F32 ? 4 : 8, act) : 0;
 }
 
 extern "C" void launch_layer_norm_grad(int type, const void* dY, long long lddy, const void* X,

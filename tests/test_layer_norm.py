@@ -115,6 +115,24 @@ def test_forward_and_backward(n, d, dtype, dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["none", "relu"])
+def test_every_layout(act, dtype):
+    """Row lengths at both sides of each change of lanes and pieces."""
+    vec = 16 // dtype.itemsize
+    for k in [1, 2, 4, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 320, 512, 640, 1024, 1500, 2048,
+              3000, 4096]:
+        for d in (k * vec, k * vec + 1):
+            n = 37 if d < 3000 else 5
+            x, w, b, dy = make(n, d, dtype, seed=d, dev="cuda")
+            out = ops.layer_norm(x, w, b, activation=act)
+            check_forward(x, w, b, 1e-5, act, out)
+            y, mean, rstd = out
+            check_backward(dy, x, y, mean, rstd, w, act,
+                           ops.layer_norm_grad(dy, x, mean, rstd, w, y=y, activation=act))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [16384, 16385, 40000, 100001])
 def test_long_rows(d, dtype):
     x, w, b, dy = make(6, d, dtype, seed=d, dev="cuda")
