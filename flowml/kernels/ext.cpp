@@ -537,9 +537,8 @@ static void muon_call(const std::vector<torch::Tensor>& g,
                     g[k].device() == g[0].device() &&
                     g[k].scalar_type() == g[0].scalar_type(),
                 "gradients: contiguous matrices of one type on one device");
-    // places in a working plane are 32-bit byte offsets
-    TORCH_CHECK((g[k].size(0) + 511) * (g[k].size(1) + 511) < (1LL << 30),
-                "matrix too large: 2^30 values at most");
+    TORCH_CHECK(g[k].size(0) < (1LL << 30) && g[k].size(1) < (1LL << 30),
+                "matrix too large: sides under 2^30");
     TORCH_CHECK(w[k].sizes() == g[k].sizes() && w[k].is_contiguous() &&
                     w[k].device() == g[0].device() &&
                     w[k].scalar_type() == w[0].scalar_type(),
@@ -562,9 +561,10 @@ static void muon_call(const std::vector<torch::Tensor>& g,
   // three products everywhere unless the result is rounded to bf16
   const int full = wtype != 1;
   std::vector<int> scratch(3 * n);
-  auto ws = fresh(
-      {muon_workspace((int)n, rows.data(), cols.data(), full, scratch.data())},
-      g[0], torch::kUInt8);
+  const int64_t bytes =
+      muon_workspace((int)n, rows.data(), cols.data(), full, scratch.data());
+  TORCH_CHECK(bytes >= 0, "matrix too large: about 2^30 values");
+  auto ws = fresh({bytes}, g[0], torch::kUInt8);
   launch_muon((int)n, rows.data(), cols.data(), gp.data(),
               mom.empty() ? nullptr : mp.data(), wp.data(),
               mom.empty() ? nullptr : sp.data(), gtype, wtype, (float)mu,

@@ -1526,7 +1526,8 @@ int large_shapes(int count, const int* rows, const int* cols, const int* way, in
 
 // ---- host entry points ------------------------------------------------------------
 
-// workspace of a call, in bytes; `scratch`: 3 * count integers
+// workspace of a call, in bytes, or -1 if a plane's 32-bit places do not reach
+// over one of its matrices; `scratch`: 3 * count integers
 extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int full,
                                     int* scratch) {
   int *way = scratch, *r = scratch + count, *c = scratch + 2 * count;
@@ -1537,6 +1538,7 @@ extern "C" long long muon_workspace(int count, const int* rows, const int* cols,
   for (int k = 0; k < count; ++k) {
     if (way[k] == LARGE) {
       const Sizes z = sizes_of(rows[k], cols[k], s);
+      if ((long long)std::max(rows_xt(z.np), z.ma) * z.ma >= 1LL << 30) return -1;
       sum += z.bytes + z.sums * sizeof(float);
     }
     if (way[k] == THIN) sum += thin_bytes(rows[k], cols[k]);

@@ -895,8 +895,8 @@ def newton_schulz(
     towards 1 (the default one into [0.7, 1.2], fast for small ones). The
     result has G's type; f32 and f16 are computed as exactly as in fp32. All
     matrices of a call share their kernel launches; on a GPU one may have about
-    2^30 values. A matrix that holds a NaN or an infinity comes out as NaN, an
-    empty one as it is.
+    2^30 values, its shorter side padded to 64 if it is over 16. A matrix that
+    holds a NaN or an infinity comes out as NaN, an empty one as it is.
     """
     coefficients = tuple(float(v) for v in coefficients)
     scale = _ns_scale(steps, coefficients)

@@ -132,6 +132,21 @@ def test_long(shapes, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(2, 3000001), (2100001, 17)])
+def test_very_long(m, n):
+    G = gradient("full", m, n, seed=5).cuda()
+    check(G, ops.newton_schulz(G), dev="cuda")
+
+
+@pytest.mark.gpu
+def test_too_large():
+    """Refused before anything is launched."""
+    G = torch.empty(33000, 33000, dtype=torch.float16, device="cuda")
+    with pytest.raises(RuntimeError, match="too large"):
+        ops.newton_schulz([G.new_zeros(3, 3), G])
+
+
+@pytest.mark.gpu
 def test_many_matrices():
     """More than one table of matrices, of one shape and of several."""
     stack = torch.stack([gradient("full", 70, 33, seed=k) for k in range(53)]).cuda()
