@@ -62,10 +62,10 @@ void launch_layer_norm_grad(int, const void*, long long, const void*,
                             long long, const void*, long long, const float*,
                             const float*, const float*, void*, float*, float*,
                             float*, long long, int, int, void*);
-long long muon_workspace(int, const int*, const int*, int, int*);
+long long muon_workspace(int, const int*, const int*, int*);
 void launch_muon(int, const int*, const int*, const void* const*, float* const*,
                  void* const*, const float*, int, int, float, float, float, int,
-                 int, const float*, float, int, void*, int*, void*);
+                 int, const float*, float, void*, int*, void*);
 }
 
 static void* cur_stream() {
@@ -558,19 +558,15 @@ static void muon_call(const std::vector<torch::Tensor>& g,
   }
   const float cf[3] = {(float)coef[0], (float)coef[1], (float)coef[2]};
   const int gtype = float_type(g[0]), wtype = float_type(w[0]);
-  // three products everywhere unless the result is rounded to bf16
-  const int full = wtype != 1;
   std::vector<int> scratch(3 * n);
-  const int64_t bytes =
-      muon_workspace((int)n, rows.data(), cols.data(), full, scratch.data());
+  const int64_t bytes = muon_workspace((int)n, rows.data(), cols.data(), scratch.data());
   TORCH_CHECK(bytes >= 0, "matrix too large: about 2^30 values");
   auto ws = fresh({bytes}, g[0], torch::kUInt8);
   launch_muon((int)n, rows.data(), cols.data(), gp.data(),
               mom.empty() ? nullptr : mp.data(), wp.data(),
               mom.empty() ? nullptr : sp.data(), gtype, wtype, (float)mu,
               (float)keep, (float)eps, nesterov, (int)steps, cf,
-              (float)scale_b, full, ws.data_ptr(), scratch.data(),
-              cur_stream());
+              (float)scale_b, ws.data_ptr(), scratch.data(), cur_stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

@@ -17,9 +17,10 @@
 // products accumulated in fp32: hi hi + hi lo + lo hi.  That is as exact as
 // fp32 (1.0 to 1.25 times its error on full-rank, low-rank and rank-1
 // gradients) at a third of the fp16 matrix rate, 3 times the fp32 rate.
-// Where the result is rounded to bf16, A and A^2 take hi hi alone and B X
-// takes hi (hi + lo): an error in A or B turns the left singular vectors by
-// 2^-12 but leaves the row space of X exact, so no noise grows.
+// Results of 16 bits are computed in the same way and rounded at the store: a
+// bf16 result is as good as its rounding (4096 x 4096: off by 1.66e-3 of its
+// norm; with hi hi alone in A and A^2, and hi (hi + lo) in B X, 1.82e-3, in 1854
+// us for 3415).
 //
 // A and A^2 are symmetric: tiles on or above the diagonal are computed, and
 // each is written to both places.
@@ -65,7 +66,6 @@ struct Mat {
   int parts;       // sums of squares, or chunks of a thin matrix
   int chunk;       // its columns to a block
   int rows, cols;  // as the caller has it
-  int full;        // 1: three products everywhere
   float step;
   int first;       // first block of this matrix in a launch
   int split;       // blocks to a tile of A, each with kpart of K
@@ -97,7 +97,7 @@ struct Table {
 __host__ __device__ inline int tiles_of(int n, int side) { return (n + side - 1) / side; }
 
 // A's tiles are panels of X', whose distance is not to be a power of two: 5 KB
-// more (2048 x 4096 bf16: 595 and 585 us, 1024 x 4096 f32 330 and 327).
+// more (1024 x 4096 f32: 330 us without, 327 with).
 constexpr int kGap = 80;
 __host__ __device__ inline int rows_xt(int np) { return np + kGap; }
 __host__ __device__ inline size_t plane_xt(const Mat& t) { return (size_t)rows_xt(t.np) * t.ma; }
@@ -348,9 +348,9 @@ __device__ __forceinline__ f16x8 read_turned(const f16* at, int rows4) {
 #endif
 }
 
-// acc += P Q^T over K: P has TM rows, Q TN rows.  PA, PB: planes of each (2:
-// hi and lo).  S stages of operands in LDS: the copies of S - 1 steps are under
-// way while a step is multiplied, and a step waits for its own copies alone.
+// acc += P Q^T over K: P has TM rows, Q TN rows, each as two planes, hi and lo.
+// S stages of operands in LDS: the copies of S - 1 steps are under way while a
+// step is multiplied, and a step waits for its own copies alone.
 //
 // A step is cut into units of some matrix instructions.  Between them a unit
 // sends its share of the copies and reads the next unit's fragments, across
@@ -358,13 +358,13 @@ __device__ __forceinline__ f16x8 read_turned(const f16* at, int rows4) {
 // of the multiplications keeps the matrix core idle as long as LDS takes to
 // accept them (64 x 64 tiles: 1040 cycles a step, 400 of them multiplying).
 // The scheduling barriers keep the compiler from gathering them again.
-template <class T, int BK, int S, int PA, int PB, bool TURNED>
+template <class T, int BK, int S, bool TURNED>
 __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, const f16* const (&Q)[2],
                                         int rows_q, int K, f16* lds, f32x16 (&acc)[T::FM][T::FN]) {
 #ifdef __HIP_DEVICE_COMPILE__  // the host pass does not know buffer resources
-  constexpr int STAGE = (PA * T::TM + PB * T::TN) * BK;
+  constexpr int STAGE = 2 * (T::TM + T::TN) * BK;
   constexpr int LA = T::TM * BK / 512 / T::WAVES, LB = T::TN * BK / 512 / T::WAVES;
-  constexpr int LOADS = PA * LA + PB * LB;  // copies per wave and stage
+  constexpr int LOADS = 2 * (LA + LB);  // copies per wave and stage
   constexpr int KG = BK / 16, UNITS = KG * T::FM;
   // units that send copies: with two stages these are waited for at this
   // step's end, and leave early
@@ -378,20 +378,19 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
 
   // 1 KB, 16 rows of a panel, to a copy.  A lane's 16 bytes land at 16 * lane,
   // so the swizzle is in the place they come from; the rest of it is scalar.
-  __amdgpu_buffer_rsrc_t rp[PA], rq[PB];
+  __amdgpu_buffer_rsrc_t rp[2], rq[2];
 #pragma unroll
-  for (int p = 0; p < PA; ++p)
+  for (int p = 0; p < 2; ++p) {
     rp[p] = __builtin_amdgcn_make_buffer_rsrc((void*)P[p], 0, -1, 0x00020000);
-#pragma unroll
-  for (int p = 0; p < PB; ++p)
     rq[p] = __builtin_amdgcn_make_buffer_rsrc((void*)Q[p], 0, -1, 0x00020000);
+  }
   const int from = (lane >> 2) * 64 + swizzle(lane & 3, lane >> 2) * 16;
   auto copy = [&](int k0, f16* s, int which) {
-    const bool first = which < PA * LA;
-    const int w = first ? which : which - PA * LA, l = first ? LA : LB;
+    const bool first = which < 2 * LA;
+    const int w = first ? which : which - 2 * LA, l = first ? LA : LB;
     const int p = w / l, i = w % l;
     const auto plane = first ? rp[p] : rq[p];
-    f16* to = s + (first ? p * T::TM : PA * T::TM + p * T::TN) * BK;
+    f16* to = s + (first ? p * T::TM : 2 * T::TM + p * T::TN) * BK;
     if (TURNED) {
       const int panel = (wave * l + i) / (BK / 16), piece = (wave * l + i) % (BK / 16);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
@@ -412,27 +411,27 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
     return *(const f16x8*)(plane + (kk >> 1) * rows * 32 + row * 32 +
                            swizzle((kk & 1) * 2 + (lane >> 5), row) * 8);
   };
-  f16x8 a[2][PA], b[2][PB][T::FN];
+  f16x8 a[2][2], b[2][2][T::FN];
   // Reads and multiplications of a unit, in the order in which the fragments
   // are needed: lo hi, hi lo, hi hi.
   auto read_one = [&](const f16* s, int u, int which) {
     const int kg = u / T::FM, f = u % T::FM;
     const bool late = which > T::FN && f == 0;  // the planes of the second product
-    const int pb = PB == 2 && (PA == 2) == late ? 1 : 0;
-    if (which == 0 || (PA == 2 && which == (f == 0 ? T::FN + 1 : 1))) {
-      const int p = which == 0 ? PA - 1 : 0;
+    const int pb = late ? 1 : 0;
+    if (which == 0 || which == (f == 0 ? T::FN + 1 : 1)) {
+      const int p = which == 0 ? 1 : 0;
       a[u & 1][p] = read(s + p * T::TM * BK, T::TM, wm + f * 32 + (lane & 31), kg);
     } else {
-      const int g = late ? which - T::FN - PA : which - 1;
-      b[kg & 1][pb][g] = read(s + (PA * T::TM + pb * T::TN) * BK, T::TN,
+      const int g = late ? which - T::FN - 2 : which - 1;
+      b[kg & 1][pb][g] = read(s + (2 * T::TM + pb * T::TN) * BK, T::TN,
                               wn + g * 32 + (lane & 31), kg);
     }
   };
-  constexpr int PAIRS = PA == 2 ? 3 : PB, MULS = PAIRS * T::FN;
+  constexpr int MULS = 3 * T::FN;
   auto multiply_one = [&](int u, int which) {
     const int kg = u / T::FM, f = u % T::FM;
     const int c = which / T::FN, g = which % T::FN;
-    const int pa = PA == 2 && c == 0 ? 1 : 0, pb = PB == 2 && c == PAIRS - 2 ? 1 : 0;
+    const int pa = c == 0 ? 1 : 0, pb = c == 1 ? 1 : 0;
     acc[f][g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a[u & 1][pa], b[kg & 1][pb][g], acc[f][g],
                                                        0, 0, 0);
   };
@@ -455,7 +454,7 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
   block_barrier();
   [&](const f16* __restrict s) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < PA + PB * T::FN; ++r) read_one(s, 0, r);
+    for (int r = 0; r < 2 + 2 * T::FN; ++r) read_one(s, 0, r);
   }(lds);
   int cur = 0, free = (S - 1) * STAGE;  // the stage read, and the one to fill
   // (Stages are distinct memory as far as the compiler is told, or it lets every
@@ -466,7 +465,7 @@ __device__ __forceinline__ void product(const f16* const (&P)[2], int rows_p, co
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
       const bool last = u + 1 == UNITS;
-      const int reads = PA + ((u + 1) % T::FM == 0 ? PB * T::FN : 0);
+      const int reads = 2 + ((u + 1) % T::FM == 0 ? 2 * T::FN : 0);
       const int c0 = u < SPREAD ? u * LOADS / SPREAD : LOADS;
       const int copies = u < SPREAD ? (u + 1) * LOADS / SPREAD - c0 : 0;
 #pragma unroll
@@ -535,8 +534,7 @@ __device__ __forceinline__ Old load_old(const Mat& t, int i0, int j0) {
   for (int h = 0; h < 2; ++h) {
     const size_t at = place(t.ma, j0 + h * 16 + r4, i0 + c8);
     o.hi[h] = *(const f16x8*)(ws_a(t, 0) + at);
-    o.lo[h] = f16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    if (t.full) o.lo[h] = *(const f16x8*)(ws_a(t, 1) + at);
+    o.lo[h] = *(const f16x8*)(ws_a(t, 1) + at);
   }
   return o;
 }
@@ -544,7 +542,7 @@ __device__ __forceinline__ Old load_old(const Mat& t, int i0, int j0) {
 // The 32 x 32 piece at (i0, j0) of A, B, X' or the result: kb * (product), for B
 // with ka * A and kd on the diagonal besides.  B holds a I + b A + c A^2, for
 // then B X is X' and nothing is read here to make it.  (With a X added here
-// instead, 1000 x 4000 twice took 546 us for 532 in fp32, 368 for 352 in bf16.)
+// instead, 1000 x 4000 twice took 546 us for 532.)
 // A lane holds 4 neighbouring rows of a column, 4 times; the piece goes through
 // the wave's own LDS so that every global access is 16 bytes per lane, side by
 // side.  (Written from the registers, 2 and 8 bytes per lane, the tiles' ends
@@ -599,7 +597,7 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
     }
     const size_t at = place(rows_j, j0 + j, i0 + c8);
     *(f16x8*)(ch + at) = hi;
-    if (TO == TO_X || t.full) *(f16x8*)(cl + at) = lo;
+    *(f16x8*)(cl + at) = lo;
     *(uint4*)p = make_uint4(both[0], both[1], both[2], both[3]);
     *(uint4*)(p + 4) = make_uint4(both[4], both[5], both[6], both[7]);
   }
@@ -624,7 +622,7 @@ __device__ __forceinline__ void finish(const Table& tab, const Mat& t, int turn,
     }
     const size_t at = place(t.ma, i0 + i, j0 + c8);
     *(f16x8*)(ch + at) = hi;
-    if (t.full) *(f16x8*)(cl + at) = lo;
+    *(f16x8*)(cl + at) = lo;
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
@@ -673,29 +671,17 @@ __device__ __forceinline__ void tile_of_triangle(int b, int rows, int& ti, int& 
   }
 }
 
-// BK and S for a pair of plane counts.
-template <int BK_, int S_>
-struct Depth {
-  static constexpr int BK = BK_, S = S_;
-};
-
-template <class T, class D, int PA, int PB>
-constexpr int lds_halfs() {
-  return (PA * T::TM + PB * T::TN) * D::BK * D::S;
-}
 constexpr int most(int a, int b) { return a > b ? a : b; }
 
 // One tile of A, B, X' or the result.  Bound by the matrix rate where there are
-// tiles enough (4096 x 4096 bf16: B X 209 us, 1.3 PFLOP/s; A 73 us, 0.97), by the
+// tiles enough (4096 x 4096: B X 330 us, 1.25 PFLOP/s; A 206 us, 1.0), by the
 // time of a copy into LDS and by the tiles' ends where there are not (1024 x
-// 4096, full: B X 26 us, 0.98 PFLOP/s, A 17 and 7 to join).  FULL, PART: LDS depths for full products
-// and for hi hi, of B X hi (hi + lo).
-template <class T, class FULL, class PART, int TO>
+// 4096: B X 26 us, 0.98 PFLOP/s, A 17 and 7 to join).
+template <class T, int BK, int S, int TO>
 __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, int turn, float ka,
                                                                   float kb, float kd) {
   constexpr bool SYM = TO == TO_A || TO == TO_B;
-  constexpr int HALFS = most(most(lds_halfs<T, FULL, 2, 2>(), T::WAVES * kPieceHalfs),
-                             lds_halfs<T, PART, 1, SYM ? 1 : 2>());
+  constexpr int HALFS = most(2 * (T::TM + T::TN) * BK * S, T::WAVES * kPieceHalfs);
   __shared__ __align__(16) f16 lds[HALFS];
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   int ti, tj, tile, part = 0;
@@ -745,10 +731,7 @@ __global__ __launch_bounds__(T::WAVES * 64) void flowml_ns_product(Table tab, in
     for (int g = 0; g < T::FN; ++g)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[f][g][r] = 0.f;
-  if (t.full)
-    product<T, FULL::BK, FULL::S, 2, 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
-  else
-    product<T, PART::BK, PART::S, 1, SYM ? 1 : 2, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
+  product<T, BK, S, TO == TO_A>(P, rows_p, Q, rows_q, K, lds, acc);
 
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const bool mirror = !SYM || ti != tj;
@@ -1286,16 +1269,17 @@ int pad(int v, int t) { return (v + t - 1) / t * t; }
 // Tile sides of a call's products, and the parts of K of A.  Large tiles run at
 // twice the rate of small ones, but are worth it only if there are enough for
 // the 256 CUs.  Measured, us a product (tiles):
-//   A of 1024 x 4096, full:    64 (136) 28   96 (66) 53    128 (36) 58
-//   A of 2048 x 4096, hi hi:   64 (528) 47   96 (253) 37   128 (136) 36  192 (66) 53
-//   its A^2:                   64 (528) 26   96 (253) 22   128 (136) 24  192 (66) 35
-//   A of 4096 x 4096, hi hi:   96 (946) 110  128 (528) 98  192 (253) 73  256 (136) 90
-//   B X of 1024 x 4096, full:  64 (1024) 31  128 (256) 26  256 (64) 55
-//   two of these:              128 (512) 50  128 x 256 (256) 48
-//   B X of 4096 x 4096:        128 (1024) 251              256 (256) 208
+//   A of 1024 x 4096:    64 (136) 28   96 (66) 53    128 (36) 58
+//   A of 2048 x 4096:    64 (528) 92   96 (253) 80   128 (136) 83   192 (66) 128
+//   its A^2:             64 (528) 47   96 (253) 42   128 (136) 45   192 (66) 70
+//   A of 4096 x 4096:    96 (946) 283  128 (528) 259 192 (253) 206  256 (136) 253
+//   B X of 1024 x 4096:  64 (1024) 31  128 (256) 26  256 (64) 55
+//   two of these:        128 (512) 50  128 x 256 (256) 48
+//   B X of 2048 x 4096:  128 (512) 105 128 x 256 (256) 98  256 (128) 118
+//   B X of 4096 x 4096:  128 (1024) 378  128 x 256 (512) 353  256 (256) 330
 // For A and B a side is taken by the time that follows from such figures.  Where
 // A has few tiles and a long K, blocks take parts of K and a launch more joins
-// them: two of 1024 x 4096, full, take 50 us as 272 tiles of 64, and 32 + 6 us
+// them: two of 1024 x 4096 take 50 us as 272 tiles of 64, and 32 + 6 us
 // as 72 of 128 in 3 parts; all steps of 100 x 100000, 2800 and 377 us.
 struct Sides {
   int a, b, m, n;  // A, B, and B X along m and n
@@ -1308,22 +1292,19 @@ int longer(int r, int c) { return std::max(r, c); }
 
 struct Sym {
   int side;
-  double full, half;  // us for 64 of K, full and hi hi, if a tile has a CU
+  double us;  // for 64 of K, if a tile has a CU
 };
-constexpr Sym kSym[] = {{64, 0.30, 0.30}, {96, 0.63, 0.30}, {128, 0.83, 0.40},
-                        {192, 1.75, 0.72}, {256, 2.80, 1.17}};
+constexpr Sym kSym[] = {{64, 0.30}, {96, 0.63}, {128, 0.83}, {192, 1.75}, {256, 2.80}};
 
 // us of a symmetric product of so many blocks, from times measured over matrices
 // of 512 to 4096 rows.  A full chip runs slower than one block alone: clocks
-// and memory are shared.  Of the small tiles' hi hi products a few share a CU.
-double time_of(const Sym& y, bool full, long long blocks, int K) {
+// and memory are shared.
+double time_of(const Sym& y, long long blocks, int K) {
   const double fill = blocks / 256.0, rounds = (double)((blocks + 255) / 256);
-  double each = (full ? y.full : y.half) * (rounds + 0.5 * fill);
-  if (y.side == 64 && !full) each = std::max(y.half, 0.16 + 0.23 * fill);
-  return each * ((K + 63) / 64) + 2.0 + y.side / 32.0;
+  return y.us * (rounds + 0.5 * fill) * ((K + 63) / 64) + 2.0 + y.side / 32.0;
 }
 
-Sides sides_for(int count, const int* rows, const int* cols, bool full) {
+Sides sides_for(int count, const int* rows, const int* cols) {
   auto tiles = [&](int ti, int tj) {
     long long sum = 0;
     for (int k = 0; k < count; ++k)
@@ -1358,7 +1339,7 @@ Sides sides_for(int count, const int* rows, const int* cols, bool full) {
   for (const Sym& y : kSym) {
     long long sums;
     const long long whole = triangle(y.side, kWhole, &sums);
-    const double us = time_of(y, full, whole, km);
+    const double us = time_of(y, whole, km);
     if (us < best_b) {
       best_b = us;
       s.b = y.side;
@@ -1368,7 +1349,7 @@ Sides sides_for(int count, const int* rows, const int* cols, bool full) {
       const long long blocks = parts == 1 ? whole : triangle(y.side, kpart, &sums);
       // parts that are short or for which there is no CU bring nothing
       if (parts > 1 && (kpart < 256 || blocks > 512)) break;
-      const double us = time_of(y, full, blocks, std::min(kpart, kn)) +
+      const double us = time_of(y, blocks, std::min(kpart, kn)) +
                         (sums ? 4.0 + 0.15 * parts + sums * y.side * y.side * 1.2e-6 : 0.0);
       if (us < best_a) {
         best_a = us;
@@ -1399,7 +1380,7 @@ Sizes sizes_of(int rows, int cols, Sides s) {
 }
 
 // one product for all matrices of a table; `first` of each is set here
-template <class T, class FULL, class PART, int TO>
+template <class T, int BK, int S, int TO>
 void product_of(Table& tab, int turn, float ka, float kb, float kd, hipStream_t st) {
   int blocks = 0;
   for (int k = 0; k < tab.count; ++k) {
@@ -1410,7 +1391,7 @@ void product_of(Table& tab, int turn, float ka, float kb, float kd, hipStream_t 
               : TO == TO_B ? mt * (mt + 1) / 2
                            : (t.mp / T::TM) * (t.np / T::TN);
   }
-  hipLaunchKernelGGL((flowml_ns_product<T, FULL, PART, TO>), dim3(blocks), dim3(T::WAVES * 64),
+  hipLaunchKernelGGL((flowml_ns_product<T, BK, S, TO>), dim3(blocks), dim3(T::WAVES * 64),
                      0, st, tab, turn, ka, kb, kd);
 }
 
@@ -1427,29 +1408,29 @@ void join(Sides s, Table& tab, float kb, hipStream_t st) {
 
 template <int TO>
 void product(Sides s, Table& tab, int turn, float ka, float kb, float kd, hipStream_t st) {
-  // tile, waves, and the depth of LDS for full products and for others
+  // tile, waves, and the depth and stages of LDS
   if constexpr (TO == TO_A || TO == TO_B) {
     const int side = TO == TO_A ? s.a : s.b;
     if (side == 256)
-      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<64, 2>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<256, 256, 2, 4>, 32, 2, TO>(tab, turn, ka, kb, kd, st);
     else if (side == 192)
-      product_of<Tile<192, 192, 2, 2>, Depth<32, 3>, Depth<64, 3>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<192, 192, 2, 2>, 32, 3, TO>(tab, turn, ka, kb, kd, st);
     else if (side == 96)
-      product_of<Tile<96, 96, 3, 1>, Depth<32, 6>, Depth<64, 6>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<96, 96, 3, 1>, 32, 6, TO>(tab, turn, ka, kb, kd, st);
     else if (side == 128)
-      product_of<Tile<128, 128, 2, 2>, Depth<32, 4>, Depth<64, 4>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<128, 128, 2, 2>, 32, 4, TO>(tab, turn, ka, kb, kd, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<64, 64, 2, 2>, 32, 5, TO>(tab, turn, ka, kb, kd, st);
     if (TO == TO_A && s.kpart < kWhole) join(s, tab, kb, st);
   } else {
     if (s.m == 256)
-      product_of<Tile<256, 256, 2, 4>, Depth<32, 2>, Depth<32, 3>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<256, 256, 2, 4>, 32, 2, TO>(tab, turn, ka, kb, kd, st);
     else if (s.n == 256)
-      product_of<Tile<128, 256, 2, 4>, Depth<32, 3>, Depth<32, 3>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<128, 256, 2, 4>, 32, 3, TO>(tab, turn, ka, kb, kd, st);
     else if (s.m == 128)
-      product_of<Tile<128, 128, 2, 4>, Depth<32, 4>, Depth<32, 3>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<128, 128, 2, 4>, 32, 4, TO>(tab, turn, ka, kb, kd, st);
     else
-      product_of<Tile<64, 64, 2, 2>, Depth<32, 5>, Depth<32, 5>, TO>(tab, turn, ka, kb, kd, st);
+      product_of<Tile<64, 64, 2, 2>, 32, 5, TO>(tab, turn, ka, kb, kd, st);
   }
 }
 
@@ -1528,12 +1509,11 @@ int large_shapes(int count, const int* rows, const int* cols, const int* way, in
 
 // workspace of a call, in bytes, or -1 if a plane's 32-bit places do not reach
 // over one of its matrices; `scratch`: 3 * count integers
-extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int full,
-                                    int* scratch) {
+extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int* scratch) {
   int *way = scratch, *r = scratch + count, *c = scratch + 2 * count;
   ways(count, rows, cols, way);
   const int n = large_shapes(count, rows, cols, way, r, c);
-  const Sides s = sides_for(n, r, c, full);
+  const Sides s = sides_for(n, r, c);
   size_t sum = 0;
   for (int k = 0; k < count; ++k) {
     if (way[k] == LARGE) {
@@ -1548,18 +1528,16 @@ extern "C" long long muon_workspace(int count, const int* rows, const int* cols,
 
 // g: gradients; mom: momentum buffers, or null for the orthogonalisation
 // alone; w: weights, or results.  coef: a, b, c; scale_b: a power of two that
-// brings B into fp16.  full: three products for every matrix, whatever its
-// size.  ws: muon_workspace() bytes; scratch: as there.
+// brings B into fp16.  ws: muon_workspace() bytes; scratch: as there.
 extern "C" void launch_muon(int count, const int* rows, const int* cols, const void* const* g,
                             float* const* mom, void* const* w, const float* step, int gtype,
                             int wtype, float mu, float keep, float eps, int nesterov, int steps,
-                            const float* coef, float scale_b, int full, void* ws, int* scratch,
-                            void* stream) {
+                            const float* coef, float scale_b, void* ws, int* scratch, void* stream) {
   hipStream_t st = (hipStream_t)stream;
   int* way = scratch;
   ways(count, rows, cols, way);
   const int n = large_shapes(count, rows, cols, way, scratch + count, scratch + 2 * count);
-  const Sides sides = sides_for(n, scratch + count, scratch + 2 * count, full);
+  const Sides sides = sides_for(n, scratch + count, scratch + 2 * count);
   const Call call = {count, rows, cols, g, mom, w, step};
   const float sa = kScaleA, sx = kScaleX, sb = scale_b;
   Table tab;
@@ -1619,7 +1597,6 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
       t.ws = (f16*)(at + kNormBlocks * sizeof(double));
       t.sums = (float*)(at + z.bytes);
       at += z.bytes + z.sums * sizeof(float);
-      t.full = full || t.m < 256;
       const size_t want = ((size_t)t.rows * t.cols + kPerNormBlock - 1) / kPerNormBlock;
       t.parts = (int)(want < kNormBlocks ? want : kNormBlocks);
       t.first = blocks;

@@ -892,8 +892,9 @@ def newton_schulz(
 
     X₀ = G / max(‖G‖_F, eps), then `steps` times, with A = X·Xᵀ on the shorter
     side, X ← a·X + (b·A + c·A²)·X. The polynomial moves every singular value
-    towards 1 (the default one into [0.7, 1.2], fast for small ones). The
-    result has G's type; f32 and f16 are computed as exactly as in fp32. All
+    towards 1 (the default one into [0.7, 1.2], fast for small ones). Every
+    type is computed in fp32 or as exactly, and the result, which has G's
+    type, is rounded to it once. All
     matrices of a call share their kernel launches; on a GPU one may have about
     2^30 values, its shorter side padded to 64 if it is over 16. A matrix that
     holds a NaN or an infinity comes out as NaN, an empty one as it is.

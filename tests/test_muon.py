@@ -331,3 +331,21 @@ def test_refusals():
             print("not refused:", i)
     assert all(torch.equal(p, q) for p, q in zip(keep, (w, g, m)))
     step([], [], [])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("shapes", [[(41, 128), (64, 5)], [(256, 300)], [(700, 310), (4, 900)],
+                                    pytest.param([(2048, 4096)], marks=pytest.mark.gpu),
+                                    pytest.param([(4096, 1500), (70, 30)], marks=pytest.mark.gpu)])
+def test_bf16_is_rounded_once(shapes, dev):
+    """Results in bf16 are those in fp32, rounded: nothing else is lost."""
+    gs = [gradient("full", *s, seed=1).bfloat16().to(dev) for s in shapes]
+    got, want = ops.newton_schulz(gs), ops.newton_schulz([g.float() for g in gs])
+    assert all(torch.equal(o, w.bfloat16()) for o, w in zip(got, want))
+    ws = [gradient("offset", *s, seed=2).bfloat16().to(dev) for s in shapes]
+    ms = [gradient("low", *s, seed=3).to(dev) for s in shapes]
+    wf, mf = [w.float() for w in ws], [m.clone() for m in ms]
+    ops.muon_update(ws, gs, ms, lr=0.05, weight_decay=0.1)
+    ops.muon_update(wf, [g.float() for g in gs], mf, lr=0.05, weight_decay=0.1)
+    assert all(torch.equal(w, f.bfloat16()) for w, f in zip(ws, wf))
+    assert all(torch.equal(p, q) for p, q in zip(ms, mf))
