@@ -62,7 +62,7 @@ void launch_layer_norm_grad(int, const void*, long long, const void*,
                             long long, const void*, long long, const float*,
                             const float*, const float*, void*, float*, float*,
                             float*, long long, int, int, void*);
-long long muon_workspace(int, const int*, const int*, int*);
+long long muon_workspace(int, const int*, const int*, int, int*);
 void launch_muon(int, const int*, const int*, const void* const*, float* const*,
                  void* const*, const float*, int, int, float, float, float, int,
                  int, const float*, float, void*, int*, void*);
@@ -559,7 +559,8 @@ static void muon_call(const std::vector<torch::Tensor>& g,
   const float cf[3] = {(float)coef[0], (float)coef[1], (float)coef[2]};
   const int gtype = float_type(g[0]), wtype = float_type(w[0]);
   std::vector<int> scratch(3 * n);
-  const int64_t bytes = muon_workspace((int)n, rows.data(), cols.data(), scratch.data());
+  const int64_t bytes =
+      muon_workspace((int)n, rows.data(), cols.data(), (int)steps, scratch.data());
   TORCH_CHECK(bytes >= 0, "matrix too large: about 2^30 values");
   auto ws = fresh({bytes}, g[0], torch::kUInt8);
   launch_muon((int)n, rows.data(), cols.data(), gp.data(),

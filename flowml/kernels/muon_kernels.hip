@@ -47,7 +47,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2 };
+enum { T_F32 = 0, T_BF16 = 1, T_F16 = 2, T_F64 = 3 };
 
 constexpr int kMats = 24;        // matrices to a launch: the table is an argument
 constexpr int kNormBlocks = 1024;  // most blocks that sum one matrix' squares
@@ -55,7 +55,7 @@ constexpr float kScaleX = 16384.f;  // |x| <= 1.9: within fp16
 constexpr float kScaleA = 16384.f;  // |x|^2 <= 3.7
 
 struct Mat {
-  f16* ws;         // X^T (two), A, B: two planes each
+  f16* ws;         // X^T (two), A, B: two planes each; of a thin one X, in fp64
   double* part;    // sums of squares
   const void* g;   // gradient, rows x cols
   float* mom;      // momentum buffer, or null
@@ -1067,12 +1067,17 @@ __device__ __forceinline__ void small_matrix(const Table& tab, const Mat& t, con
 //   Q = a I + b A + c A^2     P <- Q P     A <- Q A Q      O = P U / |U|
 //
 // on 16 x 16 matrices.  A squares the condition of U, which 64 bits bear (in
-// fp32 this form is 10 to 100 times less exact than the other).  Longer ones
-// take a block for every 256 columns or more, 64 blocks at most; the sums of
-// A_0 are then made by a launch of their own, and every block adds them and
-// iterates for itself.  (5 x 1024: one block 15 us, four 14.)
+// fp32 this form is 10 to 100 times less exact than the other), but not for any
+// number of steps: where U has no part, A is rounding noise, 2^-53 and as often
+// below 0 as above, which a step multiplies by a^2 <= 91 and of which, below 0, Q
+// makes more without end.  So after a run of 5 steps (2^-53 a^10: 3e-11 for a =
+// 3.44) X <- P X is written out, in fp64, and the next run begins with A = X X^T:
+// as exact as steps on X itself in fp64.  Longer ones take a block for every 256
+// columns or more, 64 blocks at most; the sums of A_0 are then made by a launch
+// of their own, and every block adds them and iterates for itself.  (5 x 1024:
+// one block 15 us, four 14.)
 
-constexpr int kThinM = 16, kThinLd = 17;
+constexpr int kThinM = 16, kThinLd = 17, kThinRun = 5;
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // Place of (i, j) in the caller's matrix, i on its shorter side.
@@ -1080,13 +1085,27 @@ __device__ __forceinline__ size_t thin_place(const Mat& t, int i, int j) {
   return t.rows > t.cols ? (size_t)j * t.cols + i : (size_t)i * t.cols + j;
 }
 
-// U(i, j).  Places outside are read at the nearest one inside and dropped: no
-// branch, so that many loads are under way.
+// Where X lies between two runs: columns of m values.
+__device__ __forceinline__ double* thin_x(const Mat& t, int i, int j) {
+  return (double*)t.ws + (size_t)j * t.m + i;
+}
+
 template <typename G>
-__device__ __forceinline__ float thin_u(const Table& tab, const Mat& t, bool update, int i, int j,
-                                        int end) {
+using Held = std::conditional_t<std::is_same<G, double>::value, double, float>;
+
+// U(i, j), or X(i, j) for G = double.  Places outside are read at the nearest one
+// inside and dropped: no branch, so that many loads are under way.
+template <typename G>
+__device__ __forceinline__ Held<G> thin_u(const Table& tab, const Mat& t, bool update, int i, int j,
+                                          int end) {
   const bool in = i < t.m && j < end;
-  const size_t at = thin_place(t, i < t.m ? i : t.m - 1, j < end ? j : end - 1);
+  i = i < t.m ? i : t.m - 1;
+  j = j < end ? j : end - 1;
+  if constexpr (std::is_same<G, double>::value) {
+    const double x = *thin_x(t, i, j);
+    return in ? x : 0.0;
+  }
+  const size_t at = thin_place(t, i, j);
   float u = (float)((const G*)t.g)[at];
   if (t.mom) {
     float m = t.mom[at];
@@ -1099,7 +1118,7 @@ __device__ __forceinline__ float thin_u(const Table& tab, const Mat& t, bool upd
   return in ? u : 0.f;
 }
 
-// f(a value of the gradients' type): the type is asked for once, not at every
+// f(a value of the type that is read): the type is asked for once, not at every
 // load, where the branches would let one load follow the other.
 template <typename F>
 __device__ __forceinline__ void by_type(int type, F f) {
@@ -1107,19 +1126,22 @@ __device__ __forceinline__ void by_type(int type, F f) {
     f(0.f);
   else if (type == T_BF16)
     f((__bf16)0.f);
-  else
+  else if (type == T_F16)
     f((f16)0.f);
+  else
+    f(0.0);
 }
 
-// this block's share of U U^T into 256 doubles of LDS
-__device__ __forceinline__ void thin_gram(const Table& tab, const Mat& t, int chunk, double* lds) {
+// this block's share of U U^T, or of X X^T in a later run, into 256 doubles of LDS
+__device__ __forceinline__ void thin_gram(const Table& tab, const Mat& t, int run, int chunk,
+                                          double* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int WAVES = kSmallWaves;
   f64x4 acc = {0.0, 0.0, 0.0, 0.0};
   const int end = t.n - chunk * t.chunk < t.chunk ? t.n : (chunk + 1) * t.chunk;
-  by_type(tab.gtype, [&](auto like) {
+  by_type(run ? T_F64 : tab.gtype, [&](auto like) {
     for (int j = chunk * t.chunk + wave * 16; j < end; j += 4 * WAVES * 16) {
-      float u[4][4];
+      Held<decltype(like)> u[4][4];
 #pragma unroll
       for (int h = 0; h < 4; ++h)
 #pragma unroll
@@ -1146,21 +1168,24 @@ __device__ __forceinline__ void thin_gram(const Table& tab, const Mat& t, int ch
   __syncthreads();
 }
 
-__global__ __launch_bounds__(kSmallThreads) void flowml_ns_thin_gram(Table tab) {
+__global__ __launch_bounds__(kSmallThreads) void flowml_ns_thin_gram(Table tab, int run) {
   __shared__ double lds[kSmallThreads / 64 * 256];
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
   const int chunk = blockIdx.x - t.first;
   if (t.parts == 1) return;  // one block does it all
-  thin_gram(tab, t, chunk, lds);
+  thin_gram(tab, t, run, chunk, lds);
   if (threadIdx.x < 256) t.part[(size_t)chunk * 256 + threadIdx.x] = lds[threadIdx.x];
 }
 
-__device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, const Poly& poly, int chunk,
-                            double* lds) {
+// One run of steps, from A's sums to P applied.
+__device__ __forceinline__ void thin_run(const Table& tab, const Mat& t, const Poly& poly, int run,
+                                         int chunk, double* lds) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int WAVES = kSmallWaves;
+  const int left = poly.steps - run * kThinRun, steps = left < kThinRun ? left : kThinRun;
+  const bool last = left <= kThinRun;
   if (t.parts == 1) {
-    thin_gram(tab, t, 0, lds);
+    thin_gram(tab, t, run, 0, lds);
   } else {
     double s = 0.0;
     if (tid < 256) {
@@ -1169,10 +1194,13 @@ __device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, cons
     }
     __syncthreads();
   }
-  double total = 0.0;
-  for (int k = 0; k < 16; ++k) total += lds[k * 17];
-  const double norm = sqrt(total);
-  const double inv = norm <= (double)tab.eps ? 1.0 / (double)tab.eps : 1.0 / norm;
+  double inv = 1.0;
+  if (run == 0) {
+    double total = 0.0;
+    for (int k = 0; k < 16; ++k) total += lds[k * 17];
+    const double norm = sqrt(total);
+    inv = norm <= (double)tab.eps ? 1.0 / (double)tab.eps : 1.0 / norm;
+  }
 
   // Wave 0 iterates.  A lane's operands of a product of symmetric matrices are
   // the values (lane & 15, 4 s + lane / 16); it is given (4 r + lane / 16, lane & 15).
@@ -1199,13 +1227,13 @@ __device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, cons
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       return o;
     };
-    for (int s = 0; s < poly.steps; ++s) {
+    for (int s = 0; s < steps; ++s) {
       f64x4 Q = operand(times(A, A));
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         Q[r] = (double)poly.c * Q[r] + (double)poly.b * A[r] + (c == 4 * r + q ? (double)poly.a : 0.0);
       P = s ? operand(times(Q, P)) : Q;
-      if (s + 1 < poly.steps) A = operand(times(operand(times(Q, A)), Q));
+      if (s + 1 < steps) A = operand(times(operand(times(Q, A)), Q));
     }
 #pragma unroll
     for (int r = 0; r < 4; ++r) buf[c * kThinLd + 4 * r + q] = P[r] * inv;
@@ -1215,9 +1243,9 @@ __device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, cons
 #pragma unroll
   for (int r = 0; r < 4; ++r) P[r] = buf[c * kThinLd + 4 * r + q];
   const int end = t.n - chunk * t.chunk < t.chunk ? t.n : (chunk + 1) * t.chunk;
-  by_type(tab.gtype, [&](auto like) {
+  by_type(run ? T_F64 : tab.gtype, [&](auto like) {
     for (int j0 = chunk * t.chunk + wave * 16; j0 < end; j0 += 4 * WAVES * 16) {
-      float u[4][4];
+      Held<decltype(like)> u[4][4];
 #pragma unroll
       for (int h = 0; h < 4; ++h)
 #pragma unroll
@@ -1234,12 +1262,15 @@ __device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, cons
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 4 * r + q;
-          if (i < t.m && j < end) {
-            const size_t at = thin_place(t, i, j);
-            float o = (float)acc[r];
-            if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
-            store_as(t.w, at, tab.wtype, o);
+          if (i >= t.m || j >= end) continue;
+          if (!last) {
+            *thin_x(t, i, j) = acc[r];
+            continue;
           }
+          const size_t at = thin_place(t, i, j);
+          float o = (float)acc[r];
+          if (t.mom) o = tab.keep * load_as(t.w, at, tab.wtype) - t.step * o;
+          store_as(t.w, at, tab.wtype, o);
         }
       }
     }
@@ -1248,10 +1279,19 @@ __device__ __forceinline__ void thin_matrix(const Table& tab, const Mat& t, cons
 
 extern __shared__ __align__(16) char flowml_ns_lds[];
 
-__global__ __launch_bounds__(kSmallThreads) void flowml_ns_small(Table tab, Poly poly) {
+// Matrices of one block all runs, others run `run`.
+__global__ __launch_bounds__(kSmallThreads) void flowml_ns_small(Table tab, Poly poly, int run) {
   const Mat& t = tab.mat[find(tab, blockIdx.x)];
+  if (t.parts > 1) {
+    thin_run(tab, t, poly, run, blockIdx.x - t.first, (double*)flowml_ns_lds);
+    return;
+  }
+  if (run) return;
   if (t.m <= kThinM)
-    thin_matrix(tab, t, poly, blockIdx.x - t.first, (double*)flowml_ns_lds);
+    for (int r = 0; r * kThinRun < poly.steps; ++r) {
+      thin_run(tab, t, poly, r, 0, (double*)flowml_ns_lds);
+      __syncthreads();  // X is written, P is read
+    }
   else if (small_pieces(t.m) == 2)
     small_matrix<2>(tab, t, poly, (f16*)flowml_ns_lds);
   else if (small_pieces(t.m) == 4)
@@ -1458,9 +1498,14 @@ int thin_chunk(int n) {
   return c < 256 ? 256 : c;
 }
 
-size_t thin_bytes(int rows, int cols) {
+// its blocks' sums, and X if there is more than one run
+size_t thin_sums(int rows, int cols) {
   const int n = rows < cols ? cols : rows, c = thin_chunk(n), chunks = (n + c - 1) / c;
   return chunks > 1 ? (size_t)chunks * 256 * sizeof(double) : 0;
+}
+size_t thin_bytes(int rows, int cols, int steps) {
+  const size_t x = steps > kThinRun ? (size_t)rows * cols * sizeof(double) : 0;
+  return thin_sums(rows, cols) + (x + 255) / 256 * 256;
 }
 
 struct Call {
@@ -1509,7 +1554,8 @@ int large_shapes(int count, const int* rows, const int* cols, const int* way, in
 
 // workspace of a call, in bytes, or -1 if a plane's 32-bit places do not reach
 // over one of its matrices; `scratch`: 3 * count integers
-extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int* scratch) {
+extern "C" long long muon_workspace(int count, const int* rows, const int* cols, int steps,
+                                    int* scratch) {
   int *way = scratch, *r = scratch + count, *c = scratch + 2 * count;
   ways(count, rows, cols, way);
   const int n = large_shapes(count, rows, cols, way, r, c);
@@ -1521,7 +1567,7 @@ extern "C" long long muon_workspace(int count, const int* rows, const int* cols,
       if ((long long)std::max(rows_xt(z.np), z.ma) * z.ma >= 1LL << 30) return -1;
       sum += z.bytes + z.sums * sizeof(float);
     }
-    if (way[k] == THIN) sum += thin_bytes(rows[k], cols[k]);
+    if (way[k] == THIN) sum += thin_bytes(rows[k], cols[k], steps);
   }
   return (long long)sum;
 }
@@ -1563,7 +1609,8 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
       if (t.m <= kThinM) {
         t.chunk = thin_chunk(t.n);
         t.parts = (t.n + t.chunk - 1) / t.chunk;
-        at += thin_bytes(t.rows, t.cols);
+        t.ws = (f16*)(at + thin_sums(t.rows, t.cols));
+        at += thin_bytes(t.rows, t.cols, steps);
         chunks |= t.parts > 1;
       } else {
         const size_t b = small_lds(t.m, t.n);
@@ -1571,10 +1618,12 @@ extern "C" void launch_muon(int count, const int* rows, const int* cols, const v
       }
       blocks += t.parts;
     }
-    if (chunks)
-      hipLaunchKernelGGL(flowml_ns_thin_gram, dim3(blocks), dim3(kSmallThreads), 0, st, tab);
     const Poly poly = {coef[0], coef[1], coef[2], sb, steps};
-    hipLaunchKernelGGL(flowml_ns_small, dim3(blocks), dim3(kSmallThreads), lds, st, tab, poly);
+    for (int run = 0; run == 0 || (chunks && run * kThinRun < steps); ++run) {
+      if (chunks)
+        hipLaunchKernelGGL(flowml_ns_thin_gram, dim3(blocks), dim3(kSmallThreads), 0, st, tab, run);
+      hipLaunchKernelGGL(flowml_ns_small, dim3(blocks), dim3(kSmallThreads), lds, st, tab, poly, run);
+    }
   }
 
   for (int k0 = 0; k0 < count;) {

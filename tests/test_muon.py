@@ -349,3 +349,89 @@ def test_bf16_is_rounded_once(shapes, dev):
     ops.muon_update(wf, [g.float() for g in gs], mf, lr=0.05, weight_decay=0.1)
     assert all(torch.equal(w, f.bfloat16()) for w, f in zip(ws, wf))
     assert all(torch.equal(p, q) for p, q in zip(ms, mf))
+
+
+def hard(kind):
+    """Matrices with singular values far below the largest, or none."""
+    g = torch.Generator().manual_seed(11)
+    rn = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    if kind == "rows":  # logspaced row scales
+        return rn(12, 12) * torch.logspace(0, -9, 12)[:, None]
+    if kind == "graded":  # logspaced singular values
+        q, r = torch.linalg.qr(rn(12, 12).double())[0], torch.linalg.qr(rn(12, 12).double())[0]
+        return (q * torch.logspace(0, -9, 12).double() @ r).float()
+    if kind == "one":
+        return rn(8, 1) @ rn(1, 100)
+    if kind == "half":
+        return rn(16, 8) @ rn(8, 16)
+    if kind == "softmax":  # a last layer's gradient: its columns sum to 0
+        d = torch.softmax(rn(200, 5), 1) - torch.eye(5)[torch.randint(0, 5, (200,), generator=g)]
+        return torch.relu(rn(200, 64)).T @ d
+    if kind == "same":
+        return torch.ones(8, 100)
+    if kind == "long":
+        return rn(9, 2) @ rn(2, 3000)
+    raise ValueError(kind)
+
+
+HARD = ["rows", "graded", "one", "half", "softmax", "same", "long"]
+FP32 = lambda coef: tuple(torch.tensor(coef, dtype=torch.float32).double().tolist())  # noqa: E731
+
+
+def tolerance64(G, sizes, coef):
+    """As ``tolerance`` with 53 bits for 22, for the result and the reference both,
+    and the result's rounding to fp32."""
+    a, b, c = coef
+    s = torch.linspace(0, 1.2025, 2000).double()
+    L = max(1.0, float((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs().max()))
+    eta = 2.0 ** -53 * (16 + max(G.shape) ** 0.5)
+    return 2 * sum(L ** (len(sizes) - 1 - k) * eta * v for k, v in enumerate(sizes))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("coef,steps", [(COEF, 5), (COEF, 6), (COEF, 10), (COEF, 12), (COEF, 16),
+                                        (COEF, 20), ((2.0, -1.5, 0.5), 30), ((1.5, -0.5, 0.0), 40)])
+def test_thin_in_many_steps(coef, steps):
+    """Shorter sides of 16 or less are computed in 64 bits, however many steps."""
+    coef = FP32(coef)  # as the kernels have them
+    grads = [hard(k).cuda() for k in HARD]
+    for G, o, again in zip(grads, ops.newton_schulz(grads, steps=steps, coefficients=coef),
+                           ops.newton_schulz(grads[::-1], steps=steps, coefficients=coef)[::-1]):
+        ref, sizes = reference(G.cpu(), steps, coef)
+        off, size = float((o.cpu().double() - ref).norm()), float(ref.norm())
+        assert off <= tolerance64(G, sizes, coef) + 2.0 ** -24 * size, (tuple(G.shape), off, size)
+        assert torch.equal(o, again)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("coef", [COEF, (2.0, -1.5, 0.5), (1.5, -0.5, 0.0)])
+@pytest.mark.parametrize("steps", [12, 20, 30, 100])
+def test_many_steps_stay_bounded(steps, coef, dev):
+    """No singular value leaves the polynomial's range, whatever the matrix and the
+    way it goes: 1.2025 for the default one, 1 for the others."""
+    grads = [hard(k).to(dev) for k in HARD]
+    grads += [gradient(kind, m, n, seed=m).to(dev) for m, n in ((30, 50), (200, 90), (300, 260))
+              for kind in ("low", "one")]
+    for few in (grads[:-2], grads):  # with a large one all but the thin go its way
+        for o in ops.newton_schulz(few, steps=steps, coefficients=coef):
+            top = float(torch.linalg.matrix_norm(o.cpu().double(), 2))
+            # a last step's roundings: 1 % is 2^17 of them
+            assert top <= 1.01 * (1.2025 if coef is COEF else 1.0)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_update_in_many_steps(dev):
+    """The momentum moves on once, not once in every run of steps."""
+    shapes = [(5, 64), (9, 3000), (16, 16), (40, 16)]
+    ws, gs, ms = [[gradient("full", *s, seed=k).to(dev) for s in shapes] for k in (1, 2, 3)]
+    w0, m0 = [[t.cpu().clone() for t in ts] for ts in (ws, ms)]
+    ops.muon_update(ws, gs, ms, lr=0.05, momentum=0.9, weight_decay=0.1, steps=12)
+    for w, g, m, wb, mb in zip(ws, gs, ms, w0, m0):
+        ref, mref, u, sizes, s = step_reference(wb, g.cpu(), mb, 0.05, 0.9, 0.1, True, steps=12)
+        e = 2.0 ** -23 * ((0.9 * mb.double()).abs() + mref.abs())
+        assert ((m.cpu().double() - mref).abs() <= e).all()
+        # full rank, singular values of 0.1 and more after the first step: 12 steps
+        # in fp32 of the default polynomial, whose slope past that is 3.9 at most and
+        # 1.4 on average, lose 2^-22 (16 + 64) 1.4^12 < 2^-9
+        assert float((w.cpu().double() - ref).norm()) <= s * 2.0 ** -9 * float(min(w.shape)) ** 0.5 \
+            + 2.0 ** -22 * float(ref.norm())
