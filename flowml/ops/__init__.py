@@ -740,7 +740,9 @@ def layer_norm(
     """Y = act((X − mean) · rstd · weight + bias), each row by its own mean and
     variance. Returns (Y like X, mean N, rstd N); the statistics are fp32 and
     are what ``layer_norm_grad`` takes. rstd = 1/√(var + eps), var over D.
-    Rows may lie any distance apart; N = 0 gives empty results.
+    Rows may lie any distance apart; N = 0 gives empty results. On a GPU
+    autograd does not record the call, as with the other ops: its backward pass
+    is ``layer_norm_grad``.
     """
     act = _check_norm(X, activation)
     X = _unit_columns(X)
@@ -897,7 +899,8 @@ def newton_schulz(
     type, is rounded to it once. All
     matrices of a call share their kernel launches; on a GPU one may have about
     2^30 values, its shorter side padded to 64 if it is over 16. A matrix that
-    holds a NaN or an infinity comes out as NaN, an empty one as it is.
+    holds a NaN or an infinity comes out as NaN, an empty one as it is. Autograd
+    does not record the call: the result is a constant to it.
     """
     coefficients = tuple(float(v) for v in coefficients)
     scale = _ns_scale(steps, coefficients)
@@ -922,8 +925,9 @@ def newton_schulz(
         get_ext().newton_schulz([G[k].contiguous() for k in live], [outs[k] for k in live],
                                 steps, coefficients, eps, scale)
     else:
-        for k in live:
-            outs[k].copy_(_ns_torch(G[k], steps, coefficients, eps))
+        with torch.no_grad():
+            for k in live:
+                outs[k].copy_(_ns_torch(G[k], steps, coefficients, eps))
     return out
 
 

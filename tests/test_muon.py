@@ -435,3 +435,15 @@ def test_update_in_many_steps(dev):
         # 1.4 on average, lose 2^-22 (16 + 64) 1.4^12 < 2^-9
         assert float((w.cpu().double() - ref).norm()) <= s * 2.0 ** -9 * float(min(w.shape)) ** 0.5 \
             + 2.0 ** -22 * float(ref.norm())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_no_gradient_passes(dev):
+    """The result has no autograd graph, on either device and in every form."""
+    G = gradient("full", 4, 6).to(dev).requires_grad_()
+    S = torch.stack([gradient("full", 20, 30, seed=k) for k in range(3)]).to(dev).requires_grad_()
+    for leaf, outs in ((G, [ops.newton_schulz(G, steps=2)]), (G, ops.newton_schulz([G], steps=2)),
+                       (S, [ops.newton_schulz(S, steps=2)])):
+        for o in outs:
+            assert not o.requires_grad and o.grad_fn is None
+            assert torch.equal(o, ops.newton_schulz(leaf.detach(), steps=2))
