@@ -816,6 +816,17 @@ def layer_norm_grad(
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
+def _ns_steps(steps) -> int:
+    # before the cache below, to which 5.0 and 5 are one key
+    try:
+        whole = int(steps)
+    except (TypeError, ValueError, OverflowError):
+        whole = 0
+    if whole < 1 or whole != steps:
+        raise ValueError(f"steps must be a whole number >= 1, got {steps!r}")
+    return whole
+
+
 @functools.lru_cache(maxsize=64)
 def _ns_scale(steps: int, coefficients: Tuple[float, float, float]) -> float:
     """Check the polynomial a·s + b·s³ + c·s⁵ and find the power of two that
@@ -825,8 +836,6 @@ def _ns_scale(steps: int, coefficients: Tuple[float, float, float]) -> float:
     pairs scaled by 2^14, so they must stay under 1.9; a polynomial that lets
     them grow further does not orthogonalise either.
     """
-    if not math.isfinite(steps) or steps < 1 or int(steps) != steps:
-        raise ValueError(f"steps must be a whole number >= 1, got {steps!r}")
     if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
         raise ValueError(f"coefficients must be three finite numbers, got {coefficients!r}")
     a, b, c = coefficients
@@ -903,8 +912,8 @@ def newton_schulz(
     does not record the call: the result is a constant to it.
     """
     coefficients = tuple(float(v) for v in coefficients)
+    steps = _ns_steps(steps)
     scale = _ns_scale(steps, coefficients)
-    steps = int(steps)
     if not 1e-30 <= eps < math.inf:
         raise ValueError(f"eps must be finite and at least 1e-30, got {eps!r}")
     if isinstance(G, torch.Tensor):
@@ -956,8 +965,8 @@ def muon_update(
     captured with.
     """
     coefficients = tuple(float(v) for v in coefficients)
+    steps = _ns_steps(steps)
     scale = _ns_scale(steps, coefficients)
-    steps = int(steps)
     if not 1e-30 <= eps < math.inf:
         raise ValueError(f"eps must be finite and at least 1e-30, got {eps!r}")
     if not 0 <= momentum < 1:

@@ -447,3 +447,21 @@ def test_no_gradient_passes(dev):
         for o in outs:
             assert not o.requires_grad and o.grad_fn is None
             assert torch.equal(o, ops.newton_schulz(leaf.detach(), steps=2))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_steps_as_a_float(dev):
+    """A whole number is one, whatever its type and whatever was called before."""
+    G = gradient("full", 20, 30).to(dev)
+    ops._ns_scale.cache_clear()
+    first = ops.newton_schulz(G, steps=7.0)
+    assert torch.equal(first, ops.newton_schulz(G, steps=7))
+    ops._ns_scale.cache_clear()
+    w, m = [torch.zeros_like(G)], [torch.zeros_like(G)]
+    ops.muon_update(w, [G], m, lr=1.0, steps=3.0)
+    v, m = [torch.zeros_like(G)], [torch.zeros_like(G)]
+    ops.muon_update(v, [G], m, lr=1.0, steps=3)
+    assert torch.equal(w[0], v[0])
+    for steps in (2.5, "5", None, float("nan"), -1.0):
+        with pytest.raises(ValueError):
+            ops.newton_schulz(G, steps=steps)
