@@ -298,3 +298,19 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             print("not refused:", i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d,dtype", [
+    (70_001, 64, torch.float32), (20_011, 500, torch.float16), (9001, 1100, torch.float32),
+    (3000, 4099, torch.float32), (3000, 4099, torch.float16), (4101, 8192, torch.float32),
+    (2101, 16384, torch.float32), (2101, 16384, torch.float16)])
+def test_many_rows_of_other_types(n, d, dtype):
+    """More rows than the grid holds, so that blocks go through several, and (8192
+    and 16384 columns of f32) results of over 128 MB."""
+    x, w, b, dy = make(n, d, dtype, seed=d, dev="cuda")
+    for act in ("relu", "none") if d < 4000 else ("relu",):
+        y, mean, rstd = out = ops.layer_norm(x, w, b, activation=act)
+        check_forward(x, w, b, 1e-5, act, out)
+        got = ops.layer_norm_grad(dy, x, mean, rstd, w, y=y, activation=act)
+        check_backward(dy, x, y, mean, rstd, w, act, got)

@@ -465,3 +465,33 @@ def test_steps_as_a_float(dev):
     for steps in (2.5, "5", None, float("nan"), -1.0):
         with pytest.raises(ValueError):
             ops.newton_schulz(G, steps=steps)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("coef,steps", [((1.5, -0.5, 0.0), 12), ((2.0, -1.5, 0.5), 9), (COEF, 1),
+                                        (COEF, 3), ((0.5, 0.0, 0.0), 2)])
+def test_other_polynomials_of_thin_matrices(coef, steps, dev):
+    for m, n in ((5, 64), (64, 5), (16, 16), (12, 12), (9, 3000), (257, 3), (1, 1)):
+        G = gradient("offset", m, n).to(dev)
+        check(G, ops.newton_schulz(G, steps=steps, coefficients=coef), steps, coef)
+
+
+@pytest.mark.gpu
+def test_many_steps_in_a_graph():
+    """Runs of steps of long and short thin matrices, captured: the eager bits."""
+    gs = [gradient("low", *s, seed=1).cuda() for s in ((5, 1300), (16, 16), (40, 60))]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.newton_schulz(gs, steps=13)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.newton_schulz(gs, steps=13)
+    for turn in range(4):
+        for g in gs:
+            g.copy_(gradient("full", *g.shape, seed=20 + turn))
+        eager = ops.newton_schulz(gs, steps=13)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, eager))
