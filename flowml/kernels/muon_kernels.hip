@@ -14,9 +14,11 @@
 // in 8 or 11 bits lose gradients of low rank (error 2e-2 to 9e-2 of the
 // result).  The iterates are bounded, so they are kept here as sums of two
 // fp16 numbers, x 2^s = hi + lo, 22 bits, and a product is three fp16 matrix
-// products accumulated in fp32: hi hi + hi lo + lo hi.  That is as exact as
-// fp32 (1.0 to 1.25 times its error on full-rank, low-rank and rank-1
-// gradients) at a third of the fp16 matrix rate, 3 times the fp32 rate.
+// products accumulated in fp32: hi hi + hi lo + lo hi.  By norms that is about
+// as exact as fp32 (0.2 to 1.6 times its error after five steps, on full-rank,
+// low-rank, rank-1 and graded gradients) at a third of the fp16 matrix rate, 3
+// times the fp32 rate.  The last place of lo is 2^-24: x under 2^-17 has fewer
+// than 22 bits, to the nearest 2^-39 (a row of 1e-9 of the norm comes out to 1 %).
 // Results of 16 bits are computed in the same way and rounded at the store: a
 // bf16 result is as good as its rounding (4096 x 4096: off by 1.66e-3 of its
 // norm; with hi hi alone in A and A^2, and hi (hi + lo) in B X, 1.82e-3, in 1854
@@ -25,8 +27,8 @@
 // A and A^2 are symmetric: tiles on or above the diagonal are computed, and
 // each is written to both places.
 //
-// Three ways, by size: matrices of 16 rows or fewer are iterated as their small
-// square alone, in fp64; those that fit a CU's LDS are held there, in one launch
+// Three ways, by size: matrices whose shorter side is 16 or less are iterated as
+// their small square alone, in fp64, a launch or two for five steps; those that fit a CU's LDS are held there, in one launch
 // for all of a call; the rest goes through working planes in memory, padded with
 // zeros to whole tiles, which the iteration keeps, so that only the first and
 // the last kernel look at ragged edges.  These share their launches too: 2 + 3 *
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(256) void flowml_ns_norm(Table tab) {
 
 // ---- the first iterate: 64 x 64 tiles of the caller's matrix -------------------
 
-// Bound by memory: 4096 x 4096 bf16, 33 MB in and 67 MB out, 20 us.
+// Bound by memory: 4096 x 4096 bf16, 33 MB in and 67 MB out, 21 us.
 
 __global__ __launch_bounds__(256) void flowml_ns_first(Table tab) {
   __shared__ double red[4];
@@ -674,7 +676,7 @@ __device__ __forceinline__ void tile_of_triangle(int b, int rows, int& ti, int& 
 constexpr int most(int a, int b) { return a > b ? a : b; }
 
 // One tile of A, B, X' or the result.  Bound by the matrix rate where there are
-// tiles enough (4096 x 4096: B X 330 us, 1.25 PFLOP/s; A 206 us, 1.0), by the
+// tiles enough (4096 x 4096: B X 301 us, 1.37 PFLOP/s; A 180 us, 1.14), by the
 // time of a copy into LDS and by the tiles' ends where there are not (1024 x
 // 4096: B X 26 us, 0.98 PFLOP/s, A 17 and 7 to join).
 template <class T, int BK, int S, int TO>
@@ -1308,7 +1310,7 @@ int pad(int v, int t) { return (v + t - 1) / t * t; }
 
 // Tile sides of a call's products, and the parts of K of A.  Large tiles run at
 // twice the rate of small ones, but are worth it only if there are enough for
-// the 256 CUs.  Measured, us a product (tiles):
+// the 256 CUs.  Measured on normally distributed values, us a product (tiles):
 //   A of 1024 x 4096:    64 (136) 28   96 (66) 53    128 (36) 58
 //   A of 2048 x 4096:    64 (528) 92   96 (253) 80   128 (136) 83   192 (66) 128
 //   its A^2:             64 (528) 47   96 (253) 42   128 (136) 45   192 (66) 70

@@ -774,7 +774,9 @@ def layer_norm_grad(
     """Backward pass of ``layer_norm``: (dX like X, dweight D f32, dbias D f32).
 
     The activation's derivative is taken from the output ``y`` (relu: y > 0,
-    sigmoid: y·(1 − y)), as in the rest of the MLP backward. dweight and dbias
+    sigmoid: y·(1 − y)), as in the rest of the MLP backward, and so from its
+    rounding: a sigmoid in bf16 is 1 from about 6.2 on, with derivative 0 there
+    instead of 0.002. dweight and dbias
     are sums over the local rows in a fixed order (two runs agree bit for bit);
     they are given for a missing weight or bias too. N = 0 gives zeros.
     """
@@ -903,13 +905,20 @@ def newton_schulz(
 
     X₀ = G / max(‖G‖_F, eps), then `steps` times, with A = X·Xᵀ on the shorter
     side, X ← a·X + (b·A + c·A²)·X. The polynomial moves every singular value
-    towards 1 (the default one into [0.7, 1.2], fast for small ones). Every
-    type is computed in fp32 or as exactly, and the result, which has G's
-    type, is rounded to it once. All
-    matrices of a call share their kernel launches; on a GPU one may have about
-    2^30 values, its shorter side padded to 64 if it is over 16. A matrix that
-    holds a NaN or an infinity comes out as NaN, an empty one as it is. Autograd
-    does not record the call: the result is a constant to it.
+    towards 1 (the default one into [0.7, 1.2], fast for small ones), and with
+    many steps also what is only rounding, in G or on the way. The result has
+    G's type, to which it is rounded once.
+
+    On a GPU iterates have 22 bits and products are summed in fp32, which taken
+    by norms is about as exact as fp32; but values under 2^-17 of the norm keep
+    fewer bits, 2^-39 of it being the smallest difference. Shorter sides of 16
+    or less are computed in 64 bits. Up to 24 matrices of a call share their
+    kernel launches. How the work is divided depends on all matrices of a call,
+    so the last bits of a result may differ with its company. One may have about
+    2^30 values, its shorter side padded to 64 if it is over 16.
+
+    A matrix that holds a NaN or an infinity comes out as NaN, an empty one as
+    it is. Autograd does not record the call: the result is a constant to it.
     """
     coefficients = tuple(float(v) for v in coefficients)
     steps = _ns_steps(steps)

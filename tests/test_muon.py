@@ -495,3 +495,23 @@ def test_many_steps_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, eager))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(30, 50), (120, 100), (300, 400)])
+@pytest.mark.parametrize("steps", [5, 10])
+def test_rows_far_apart(m, n, steps):
+    """Rows far below the others: off by what the pairs' last place comes to. X is held
+    to 2^-39 of the norm; a step adds that again, and A's and B's last places (2^-39
+    and 2^-38, times |b| + 2c < 9 and 1) times a column of X, which is 1 long at most
+    and meets them with any signs: three times their half steps, 16 for all. A later
+    step multiplies by a in these rows: 1 + 17 (1 / a + 1 / a^2 + ...) < 8 of the first.
+    """
+    G = gradient("full", m, n, seed=2) * torch.logspace(0, -9, m)[:, None]
+    got = ops.newton_schulz(G.cuda(), steps=steps).cpu()
+    check(G, got, steps)
+    ref = reference(G, steps)[0]
+    low = G.norm(dim=1) / G.norm() < 2.0 ** -24
+    assert low.sum() >= m // 6
+    worst = float((got.double() - ref)[low].abs().max())
+    assert worst <= 8 * 2.0 ** -39 * COEF[0] ** steps
