@@ -8,14 +8,20 @@
 //   dx = rstd (p - mean(p) - xh mean(p xh))
 //   dg = sum_rows dz xh         db = sum_rows dz
 //
-// Both passes are bound by HBM: each input is read once and each output is
-// written once.  A row lives in the registers of the lanes that share it, so
-// the variance is the centred sum of a second look at registers, not of a
-// second read (no E[x^2] - E[x]^2 cancellation).  The number of lanes on a
-// row is the smallest power of two that holds it in 16-byte pieces: a row of
-// 128 bf16 takes 16 lanes, four rows share a wave, and their sums are DPP
-// moves without LDS.  All sums and statistics are fp32; values are rounded
-// to the tensor's type once, at the store.
+// Both passes are bound by HBM.  A row of up to 16384 values lives in the
+// registers of the lanes that share it, so each input is read once and each
+// output is written once, and the variance is the centred sum of a second look
+// at registers, not of a second read (no E[x^2] - E[x]^2 cancellation).  Longer
+// rows are read three times.  How many lanes take a row, with how many 16-byte
+// pieces each, follows from its length (forward_shape, backward_shape): of 128
+// bf16, 16 lanes with one piece, so that four rows share a wave and their sums
+// are DPP moves without LDS; a row that is more than a wave holds has a block to
+// itself, of as many waves as it needs.  All sums and statistics are fp32;
+// values are rounded to the tensor's type once, at the store.
+//
+// Times in the comments are of the kernels alone: beside a kernel over inputs
+// that no cache holds, for two ways of one thing in a loop over one input, of
+// which the last-level cache keeps a part.
 //
 // The activation's derivative is taken from the stored output y (relu: y > 0,
 // sigmoid: y (1 - y)), as the dgrad kernel of the GEMM stack does: a sign
@@ -183,7 +189,7 @@ __device__ __forceinline__ float activate_grad(float dy, float y, int act) {
 
 // The next row of a group is under way while this one is worked on: 32 waves
 // a CU with 16 bytes a lane are not quite enough to keep HBM busy.  1M x 128
-// bf16: 87 us, 5.9 TB/s; 5003 x 4099 f32: 28 us, 5.9 TB/s; 256 x 64 f32: 3 us.
+// bf16: 94 us, 5.5 TB/s; 5003 x 4099 f32: 30 us, 5.4 TB/s; 256 x 64 f32: 3 us.
 template <typename T, int LANES, int NV>
 __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm(
     const T* __restrict__ X, long long ldx, const float* __restrict__ gamma,
@@ -263,7 +269,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm(
 }
 
 // Rows longer than a block's registers: three looks at the row (8000 x 30000 bf16:
-// 278 us, 3.5 TB/s of what has to move).
+// 285 us, 3.4 TB/s of what has to move).
 template <typename T>
 __global__ __launch_bounds__(1024) void flowml_layer_norm_long(
     const T* __restrict__ X, long long ldx, const float* __restrict__ gamma,
@@ -308,8 +314,8 @@ __global__ __launch_bounds__(1024) void flowml_layer_norm_long(
 
 // ---------------------------------------------------------------------------
 // backward: dx, and one slab (dg, db) per block in part[block][2][D].  1M x 128
-// bf16 with relu: 189 us and 5 for the slabs, 5.3 TB/s; 8192 x 8192 f16: 81 us
-// and 5, 4.7 TB/s
+// bf16 with relu: 193 us and 5 for the slabs, 5.2 TB/s; 8192 x 8192 f16: 83 us
+// and 5, 4.6 TB/s
 // ---------------------------------------------------------------------------
 
 template <typename T, int LANES, int NV, bool ACT>
@@ -432,7 +438,7 @@ __global__ __launch_bounds__(block_of(LANES)) void flowml_layer_norm_grad(
 }
 
 // Long rows: dx alone, two looks at the row (2000 x 30000 bf16, with the columns:
-// 206 us, 1.7 TB/s of what has to move) ...
+// 210 us, 1.7 TB/s of what has to move) ...
 template <typename T>
 __global__ __launch_bounds__(1024) void flowml_layer_norm_grad_long(
     const T* __restrict__ dY, long long lddy, const T* __restrict__ X, long long ldx,
