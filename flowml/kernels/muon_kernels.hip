@@ -18,7 +18,7 @@
 // as exact as fp32 (0.2 to 1.6 times its error after five steps, on full-rank,
 // low-rank, rank-1 and graded gradients) at a third of the fp16 matrix rate, 3
 // times the fp32 rate.  The last place of lo is 2^-24: x under 2^-17 has fewer
-// than 22 bits, to the nearest 2^-39 (a row of 1e-9 of the norm comes out to 1 %).
+// than 22 bits, to the nearest 2^-39 (rows of 1e-9 of the norm are 1 to 6 % off).
 // Results of 16 bits are computed in the same way and rounded at the store: a
 // bf16 result is as good as its rounding (4096 x 4096: off by 1.66e-3 of its
 // norm; with hi hi alone in A and A^2, and hi (hi + lo) in B X, 1.82e-3, in 1854
@@ -28,11 +28,12 @@
 // each is written to both places.
 //
 // Three ways, by size: matrices whose shorter side is 16 or less are iterated as
-// their small square alone, in fp64, a launch or two for five steps; those that fit a CU's LDS are held there, in one launch
-// for all of a call; the rest goes through working planes in memory, padded with
-// zeros to whole tiles, which the iteration keeps, so that only the first and
-// the last kernel look at ragged edges.  These share their launches too: 2 + 3 *
-// steps, and one more a step where sums are shared out.
+// their small square alone, in fp64, in a launch or two for five steps; those that
+// fit a CU's LDS are held there, in one launch for all of a table; the rest goes
+// through working planes in memory, padded with zeros to whole tiles, which the
+// iteration keeps, so that only the first and the last kernel look at ragged edges.
+// These share their launches too: 2 + 3 * steps, and one more a step where sums are
+// shared out.
 
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>
